@@ -5,5 +5,6 @@ from .ops import (  # noqa: F401
     check_status, decode_parents, htree_backward, htree_forward, htree_forward_autograd, htree_forward_triton_autograd,
     recompute_parents, rope_cache,
 )
+from .cache import cache_append, cache_gather, cache_plan, draft_attention  # noqa: F401
 
 __version__ = "0.1.0"

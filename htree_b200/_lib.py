@@ -50,6 +50,11 @@ SYMBOLS = (
     "htree_b200_backward",
     "htree_b200_static_scratch_bytes",
     "htree_b200_backward_static_scratch",
+    "htree_b200_cache_plan",
+    "htree_b200_cache_append",
+    "htree_b200_cache_gather",
+    "htree_b200_draft_workspace",
+    "htree_b200_draft_attention",
 )
 
 
@@ -71,6 +76,19 @@ class HtreeTypedGrads(ctypes.Structure):
 
 class HtreeTrace(ctypes.Structure):
     _fields_ = [("layer_max", ctypes.c_void_p), ("layer_sum", ctypes.c_void_p), ("layer_out", ctypes.c_void_p)]
+
+
+class HtreeCache(ctypes.Structure):
+    _fields_ = ([("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] +
+                [(n, ctypes.c_int64) for n in ("k_page", "k_row", "k_head", "v_page", "v_row", "v_head")] +
+                [(n, ctypes.c_int32) for n in ("pages", "page_size", "H_kv", "K", "V", "dtype")])
+
+
+class HtreeDrafts(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v")] +
+                [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")] +
+                [(n, ctypes.c_void_p) for n in ("table", "lengths", "parents", "out", "lse")] + [("table_stride", ctypes.c_int64)] +
+                [(n, ctypes.c_int32) for n in ("B", "N", "H", "M")] + [("scale", ctypes.c_float)])
 
 
 class HtreeError(RuntimeError):
@@ -145,6 +163,16 @@ def lib() -> ctypes.CDLL:
         L.htree_b200_backward_static_scratch.restype = ctypes.c_int
         L.htree_b200_backward_static_scratch.argtypes = [ctypes.POINTER(HtreeShape), vp, vp, vp, vp, vp, vp, vp, vp, i32, f32, vp,
                                                          vp, vp, vp, vp, vp, vp, vp, vp, u32, vp]
+        L.htree_b200_cache_plan.restype = ctypes.c_int
+        L.htree_b200_cache_plan.argtypes = [i32, i32, i32, i32, vp, vp, vp, ctypes.c_int64, vp, i32, vp, vp, vp, vp, vp]
+        L.htree_b200_cache_append.restype = ctypes.c_int
+        L.htree_b200_cache_append.argtypes = [ctypes.POINTER(HtreeCache), i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]
+        L.htree_b200_cache_gather.restype = ctypes.c_int
+        L.htree_b200_cache_gather.argtypes = [ctypes.POINTER(HtreeCache), i32, i32, i32, vp, ctypes.c_int64, vp, vp, vp, vp, vp]
+        L.htree_b200_draft_workspace.restype = ctypes.c_int64
+        L.htree_b200_draft_workspace.argtypes = [ctypes.POINTER(HtreeCache), ctypes.POINTER(HtreeDrafts)]
+        L.htree_b200_draft_attention.restype = ctypes.c_int
+        L.htree_b200_draft_attention.argtypes = [ctypes.POINTER(HtreeCache), ctypes.POINTER(HtreeDrafts), vp, ctypes.c_int64, vp, vp]
         _lib = L
     return _lib
 

@@ -78,21 +78,21 @@ def build(force: bool = False, verbose: bool = False, defines=(), out: str = LIB
 
 
 def build_glue(force: bool = False) -> str:
-    """The torch-side call path (csrc/torch_glue.cpp) as a Python extension next to the library, which it links."""
-    src = os.path.join(CSRC, "torch_glue.cpp")
+    """The torch-side call path (csrc/torch_glue.cpp, cache_glue.cpp) as a Python extension next to the library, which it links."""
+    srcs = [os.path.join(CSRC, f) for f in ("torch_glue.cpp", "cache_glue.cpp")]
     header = os.path.join(HERE, "..", "include", "htree_b200.h")
-    if force or _stale(GLUE_LIB, [src, header]):
+    if force or _stale(GLUE_LIB, [*srcs, header]):
         import sysconfig
         import torch
         from torch.utils import cpp_extension as ce
         inc = [f"-isystem{p}" for p in [*ce.include_paths(), sysconfig.get_paths()["include"], "/usr/local/cuda/include"]]
         libs = [f"-L{p}" for p in ce.library_paths()] + ["-L/usr/local/cuda/lib64"]
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_torch_glue", "-DTORCH_API_INCLUDE_EXTENSION_H",
-               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, src, "-o", GLUE_LIB, *libs, "-lc10", "-lc10_cuda",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, *srcs, "-o", GLUE_LIB, *libs, "-lc10", "-lc10_cuda",
                "-ltorch_cpu", "-ltorch", "-ltorch_python", f"-L{HERE}", "-lhtree_b200", "-Wl,-rpath,$ORIGIN"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError(f"g++ failed on {src}:\n{r.stdout}\n{r.stderr}")
+            raise RuntimeError(f"g++ failed on {' '.join(srcs)}:\n{r.stdout}\n{r.stderr}")
     return GLUE_LIB
 
 

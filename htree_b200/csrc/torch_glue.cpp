@@ -143,7 +143,10 @@ c10::optional<at::Tensor> plain_forward(const at::Tensor& q, const at::Tensor& k
 
 }  // namespace
 
+void bind_cache(py::module& m);      // cache_glue.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    bind_cache(m);
     m.def("autograd_forward", &autograd_forward, py::call_guard<py::gil_scoped_release>());
     m.def("plain_forward", &plain_forward, py::call_guard<py::gil_scoped_release>());
 }

@@ -157,8 +157,8 @@ def _status(device) -> torch.Tensor:
 
 
 def check_status(device=None) -> None:
-    """Synchronise and raise if a kernel flagged a problem since the last check: an out-of-range node index (bits 0-3), or a
-    bounded wait of the pipelined forward that ran out (bit 4)."""
+    """Synchronise and raise if a kernel flagged a problem since the last check: an out-of-range node index (bits 0-3), a
+    bounded wait of the pipelined forward that ran out (bit 4), or tables of a paged cache that do not fit it (bits 5 and 6)."""
     device = torch.device(device if device is not None else torch.cuda.current_device())
     if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
@@ -173,6 +173,10 @@ def check_status(device=None) -> None:
             if v & 16:
                 what.append("an asynchronous operand copy of the pipelined forward did not complete within its bounded wait "
                             "(the affected outputs were not written)")
+            if v & 32:
+                what.append("a page, slot, length or token index outside the cache, or a draft before its parent (left out)")
+            if v & 64:
+                what.append("a request longer than its row of the block table, or more new tokens than the slot map has room for (not served)")
             raise RuntimeError(f"htree_b200 kernels reported device-side status 0x{v:x}: " + "; ".join(what or ["unknown bits"]))
 
 

@@ -320,6 +320,73 @@ int htree_b200_backward_static_scratch(const HtreeShape* shape, const void* q, v
                                        const void* dO, const float* gmax, const float* gsum, int32_t* const* parents,
                                        float* dq, float* dk, float* dv, int32_t* status, uint32_t flags, void* stream);
 
+/* ---- A paged key/value cache and the attention that reads it (no counterpart in the reference) --------------------------------
+ *
+ * A cache holds the keys and values of many requests in pages of `page_size` tokens: k [pages, page_size, H_kv, K] and
+ * v [pages, page_size, H_kv, V] with any strides whose rows are dense and 16-byte aligned.  Row b of the block table
+ * table[b*table_stride + i] names the page of tokens i*page_size .. of request b, lengths[b] says how many tokens it holds; the
+ * free pages are the entries 0 .. *top - 1 of `pool`.  A slot is page * page_size + place in the page.
+ * Kernels check every page and slot that they use against the cache: what is outside is left out and reported in `status`
+ * (bit 32).  status may be NULL. */
+typedef struct HtreeCache {
+    void* k;
+    void* v;
+    int64_t k_page, k_row, k_head;  /* strides in elements: of a page, of a token in its page, of a key/value head */
+    int64_t v_page, v_row, v_head;
+    int32_t pages, page_size, H_kv, K, V, dtype;
+} HtreeCache;
+
+#define HTREE_STATUS_CACHE 32      /* a page, slot, length or token index outside the cache (left out) */
+#define HTREE_STATUS_ROW 64        /* htree_b200_cache_plan: a count above n or a request longer than its row of the table (not served) */
+
+/* Block tables and slot maps from request lengths.  Rows with counts[b] < 0 end: in row order their ceil(lengths[b] / page_size)
+ * pages go back on the pool's end (in the table's order), their table entries become -1 and their lengths 0.  Then rows with
+ * counts[b] > 0 grow, in row order, by pages from the pool's end, as long as the pool holds what the rows up to and including
+ * it need; a row that gets its pages, or needs none, is served: taken[b] = counts[b], lengths[b] += counts[b] and
+ * slots[b*n + i] = slot of the i-th new token for i < counts[b].  All other slots are -1, all other taken 0.
+ * lengths, table, pool and top are updated in place. */
+int htree_b200_cache_plan(int32_t B, int32_t M, int32_t page_size, int32_t n, int32_t* lengths, const int32_t* counts, int32_t* table,
+                          int64_t table_stride, int32_t* pool, int32_t pool_size, int32_t* top, int64_t* slots, int32_t* taken,
+                          int32_t* status, void* stream);
+
+/* Token index[b*n + i] (NULL: token i) of request b of k [B,N,H_kv,K] and v [B,N,H_kv,V] into slots[b*n + i]; -1 = not written.
+ * k_stride, v_stride: strides in elements of a request, a token, a head.  Of several tokens for one slot any may be the one kept. */
+int htree_b200_cache_append(const HtreeCache* cache, int32_t B, int32_t N, int32_t n, const void* k, const int64_t* k_stride,
+                            const void* v, const int64_t* v_stride, const int64_t* slots, const int32_t* index, int32_t* status,
+                            void* stream);
+
+/* The first min(lengths[b], T) tokens of every request as contiguous k [B,T,H_kv,K], v [B,T,H_kv,V], zeros behind them. */
+int htree_b200_cache_gather(const HtreeCache* cache, int32_t B, int32_t M, int32_t T, const int32_t* table, int64_t table_stride,
+                            const int32_t* lengths, void* k, void* v, int32_t* status, void* stream);
+
+/* Attention of N drafted tokens per request over its cached tokens and over the drafts that lead to it:
+ *     s_ij = scale * q_i . k_j     over j = the lengths[b] cached tokens and the drafts i, parent(i), parent(parent(i)), ...
+ *     lse_i = log sum_j exp(s_ij),   out_i = sum_j exp(s_ij - lse_i) v_j
+ * parents[b*N + i] < i is the draft that draft i continues, -1 where it continues the cached tokens, below -1 where there is no
+ * such draft (its rows become out = 0, lse = -inf and no other draft reads its k, v); a parent >= i is taken as -1 and reported
+ * (bit 32).  parents = NULL: every draft continues the one before it.
+ *   q [B,N,H,K], k [B,N,H_kv,K], v [B,N,H_kv,V]: strides in elements of a request, a token, a head; rows 16-byte aligned
+ *   out [B,N,H,V] of the cache's type and lse [B,N,H] fp32 (may be NULL): contiguous
+ *   workspace  htree_b200_draft_workspace() bytes, 16-byte aligned, of this call alone until its kernels have run
+ * K, V: multiples of 8 up to 256; trees of up to 1024 drafts. */
+typedef struct HtreeDrafts {
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* parents;
+    void* out;
+    float* lse;
+    int64_t table_stride;
+    int32_t B, N, H, M;
+    float scale;
+} HtreeDrafts;
+int64_t htree_b200_draft_workspace(const HtreeCache* cache, const HtreeDrafts* drafts);
+int htree_b200_draft_attention(const HtreeCache* cache, const HtreeDrafts* drafts, void* workspace, int64_t workspace_bytes,
+                               int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
