@@ -32,6 +32,8 @@ struct DraftParams {
     int64_t table_stride;
     int32_t B, N, H, Hkv, G, K, V, M, pages;
     int32_t rows, row_tiles, draft_tiles, grid;                            // rows of a tile
+    int32_t variant;          // which kernel (choose)
+    int32_t neg;              // tensor-core kernels: the scale is negative, c its magnitude and q's signs are turned
     float c;                  // scale * log2 e
     FastDiv page, group;      // by G
 };
@@ -354,6 +356,383 @@ __global__ void __launch_bounds__(kGenThreads) draft_generic_kernel(const __grid
     if (bad && p.status) atomicOr(p.status, HTREE_STATUS_CACHE);
 }
 
+// ---- 16-bit types: mma.sync -----------------------------------------------------------------------------------------------------
+
+// Up to 64 query rows: HBM bounds these, so the tiles stream through a ring of cp.async stages and the products only have to keep up.  A
+// warp owns 16 keys of every tile and RM x 16 rows with a softmax of its own (reference, mass and sums in registers); the four warps that
+// share rows are joined when the unit ends.  With the rows a block holds, WR = 1 or 2 rows of warps.
+//
+// The reference of a row is not its running maximum but within kLag of it (powers of two that P may grow by before the sums are
+// rescaled), so almost every tile needs one vote and no shuffles.  P is rounded to the type, half a step each; for fp16 the reference
+// lies kBias below the maximum, so that weights down to 2^-22 of the largest keep all their digits and the largest stays below 2^15.
+template <typename T> constexpr float kLag = 8.f;
+template <> constexpr float kLag<__half> = 7.f;
+template <typename T> constexpr float kBias = 0.f;
+template <> constexpr float kBias<__half> = 8.f;
+
+template <typename T> constexpr uint32_t kExpMask = 0x7f80u;
+template <> constexpr uint32_t kExpMask<__half> = 0x7c00u;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+
+// Values of drafts that are not finite must not meet the zero weights of the rows that do not read them: they are taken out of the tile
+// (their rows noted) and added to the rows that do.  `piece`: 16 bytes in shared memory.  True if it held any.
+template <typename T>
+__device__ __forceinline__ bool take_out(uint32_t piece) {
+    uint32_t u[4];
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(piece) : "memory");
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool lo = (u[i] & kExpMask<T>) == kExpMask<T>, hi = (u[i] >> 16 & kExpMask<T>) == kExpMask<T>;
+        any |= lo | hi;
+        u[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+    }
+    if (any) asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(piece), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+    return any;
+}
+// ... and what such a value adds to a row that reads it
+template <typename T>
+__device__ __forceinline__ float put_back(float o, const char* v, int col) {
+    const float x = to_f<T>(reinterpret_cast<const T*>(v)[col]);
+    return fabsf(x) <= 3.4028234e38f ? o : o + x;
+}
+
+struct RowPtr { const char* k; const char* v; };
+
+template <int DK, int DV, int WR> struct MmaShape {
+    static constexpr int threads = WR * 128, stage = kTile * (DK + DV) * 2;
+    static constexpr int stages = WR == 1 ? (stage > 24576 ? 3 : stage > 16384 ? 4 : 5) : (stage > 24576 ? 4 : 6);
+    static constexpr int ring = 8;                             // of row pointers and key masks: at least stages + 2
+    static_assert(stages + 2 <= ring, "");
+    static constexpr int chunk = 32 + 4;                       // columns of a joining round, padded
+};
+
+template <typename T, int DK, int DV, int WR, int RM>
+struct MmaSmem {
+    using S = MmaShape<DK, DV, WR>;
+    static constexpr int rows = WR * RM * 16;
+    static constexpr int tiles = 0, ptrs = S::stages * S::stage, there = ptrs + S::ring * kTile * (int)sizeof(RowPtr), bad = there + S::ring * 8,
+                         wm = bad + S::ring * 8, wl = wm + 4 * rows * 4, join = wl + 4 * rows * 4, total = join + 4 * rows * S::chunk * 4;
+};
+
+template <typename T, int DK, int DV, int WR, int RM>
+__global__ void __launch_bounds__(WR * 128, WR == 1 ? 2 : 1) draft_mma_kernel(const __grid_constant__ DraftParams p) {
+    using S = MmaShape<DK, DV, WR>;
+    using L = MmaSmem<T, DK, DV, WR, RM>;
+    constexpr int NT = S::threads, ST = S::stages, RING = S::ring, ROWS = L::rows, KP = DK / 8, VP = DV / 8;
+    extern __shared__ __align__(128) unsigned char sm[];
+    RowPtr* ptrs = reinterpret_cast<RowPtr*>(sm + L::ptrs);
+    uint32_t* there = reinterpret_cast<uint32_t*>(sm + L::there);       // [ring][2]
+    uint32_t* badw = reinterpret_cast<uint32_t*>(sm + L::bad);
+    float* wm = reinterpret_cast<float*>(sm + L::wm);
+    float* wl = reinterpret_cast<float*>(sm + L::wl);
+    float* joinb = reinterpret_cast<float*>(sm + L::join);
+    chain_enter();
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, wk = w & 3, wr = w >> 2, kw = wk * 16, g = lane >> 2, r4 = lane & 3;
+    Place at;
+    int64_t x0 = 0, x1 = 0;
+    const int64_t all = find_place<NT>(p, [&](int64_t n) {
+        const int64_t parts = parts_of(p, n);
+        x0 = part_start(blockIdx.x < parts ? blockIdx.x : 0, n, parts);
+        x1 = part_start(blockIdx.x < parts ? blockIdx.x + 1 : 1, n, parts);
+        return x0;
+    }, at);
+    if (blockIdx.x >= parts_of(p, all)) return;
+    const int n_tiles = (int)(x1 - x0);
+    bool bad = false;
+    { bool b = false; draft_length(p, at.b, &b); bad |= b; }
+    if (tid < 2 * RING) badw[tid] = 0;
+
+    Place ahead = at;                  // of the tile whose row pointers are made next
+    int made = 0;
+    auto make_row = [&](const Place& pl, int tile, int j) {
+        RowPtr rp{p.q, p.q};           // (never read: copies of rows that are not there have no source)
+        const bool on = key_row(p, pl, pl.unit / p.row_tiles, j, rp.k, rp.v, &bad);
+        const uint32_t m = __ballot_sync(0xffffffffu, on);
+        if (lane == 0) there[(tile % RING) * 2 + (j >> 5)] = m;
+        if (!on) rp = RowPtr{nullptr, nullptr};
+        ptrs[(tile % RING) * kTile + j] = rp;
+    };
+    // the first stages' pointers at once: threads 0-63 the first tile, 64-127 the second, ...
+    for (int i = 0; i < ST && i < n_tiles; ++i) {
+        if ((i * 2) % (NT / 32) <= w && w < (i * 2) % (NT / 32) + 2) make_row(ahead, i, tid % 64);
+        ahead.next(p);
+        ++made;
+    }
+    __syncthreads();
+    const uint32_t tiles_u = smem_u32(sm);
+    auto issue = [&](int tile) {
+        const uint32_t base = tiles_u + (tile % ST) * S::stage;
+        const RowPtr* rows = ptrs + (tile % RING) * kTile;
+#pragma unroll
+        for (int i = 0; i < kTile * KP / NT; ++i) {
+            const int x = i * NT + tid, j = x / KP, c = x % KP;
+            const char* src = rows[j].k;
+            const bool on = src != nullptr && c * 8 < p.K;
+            cp_async16(base + j * (DK * 2) + ((c ^ (j & 7)) << 4), on ? src + c * 16 : p.q, on);
+        }
+#pragma unroll
+        for (int i = 0; i < kTile * VP / NT; ++i) {
+            const int x = i * NT + tid, j = x / VP, c = x % VP;
+            const char* src = rows[j].v;
+            const bool on = src != nullptr && c * 8 < p.V;
+            cp_async16(base + kTile * DK * 2 + j * (DV * 2) + ((c ^ (j & 7)) << 4), on ? src + c * 16 : p.q, on);
+        }
+    };
+    for (int i = 0; i < ST - 1; ++i) {
+        if (i < n_tiles) issue(i);
+        cp_async_commit();
+    }
+
+    uint32_t qf[RM][DK / 16][4];
+    float o[RM][DV / 8][4], ref[RM][2], mass[RM][2];
+    int first_tile = at.tile;
+    bool fresh = true, first_piece = true;
+    const uint32_t flip = p.neg ? 0x80008000u : 0u;
+    for (int it = 0; it < n_tiles; ++it) {
+        const bool draft = at.tile >= at.tiles - p.draft_tiles;
+        if (fresh) {
+            first_tile = at.tile;
+            fresh = false;
+#pragma unroll
+            for (int m = 0; m < RM; ++m) {
+                ref[m][0] = ref[m][1] = -INFINITY;
+                mass[m][0] = mass[m][1] = 0.f;
+#pragma unroll
+                for (int d = 0; d < DV / 8; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[m][d][e] = 0.f;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    int n, h;
+                    const bool on = row_of(p, at.unit, (wr * RM + m) * 16 + half * 8 + g, n, h);
+                    const char* src = p.q + at.b * p.q_b + n * p.q_n + h * p.q_h + 4 * r4;
+#pragma unroll
+                    for (int ks = 0; ks < DK / 16; ++ks)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            qf[m][ks][half + 2 * e] = on && ks * 16 + e * 8 < p.K ? __ldg(reinterpret_cast<const uint32_t*>(src + ks * 32 + e * 16)) ^ flip : 0u;
+                }
+            }
+        }
+        cp_async_wait<ST - 2>();
+        if (draft) {                   // what this thread has copied of the tile's values
+            const uint32_t base = tiles_u + (it % ST) * S::stage + kTile * DK * 2;
+#pragma unroll
+            for (int i = 0; i < kTile * VP / NT; ++i) {
+                const int x = i * NT + tid, j = x / VP, c = x % VP;
+                if (take_out<T>(base + j * (DV * 2) + ((c ^ (j & 7)) << 4))) atomicOr(&badw[(it % RING) * 2 + (j >> 5)], 1u << (j & 31));
+            }
+        }
+        __syncthreads();               // the tile is there, and so are the pointers made one round ago; its predecessor's stage is free
+        if (it + ST - 1 < n_tiles) issue(it + ST - 1);
+        cp_async_commit();
+        if (made < n_tiles && made <= it + ST) {
+            if (w < 2) make_row(ahead, made, tid);
+            ahead.next(p);
+            ++made;
+        }
+        if (tid < 2) badw[((it + 4) % RING) * 2 + tid] = 0;
+
+        const uint32_t kbase = tiles_u + (it % ST) * S::stage, vbase = kbase + kTile * DK * 2;
+        float s[RM][2][4];
+#pragma unroll
+        for (int m = 0; m < RM; ++m)
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[m][nt][e] = 0.f;
+        {
+            const int row = kw + ((lane >> 4) << 3) + (lane & 7), c0 = (lane >> 3) & 1;
+#pragma unroll
+            for (int ks = 0; ks < DK / 16; ++ks) {
+                uint32_t b[4];
+                ldmatrix4(b, kbase + row * (DK * 2) + (((ks * 2 + c0) ^ (row & 7)) << 4));
+#pragma unroll
+                for (int m = 0; m < RM; ++m) {
+                    Frag<T>::mma(s[m][0], qf[m][ks][0], qf[m][ks][1], qf[m][ks][2], qf[m][ks][3], b[0], b[1]);
+                    Frag<T>::mma(s[m][1], qf[m][ks][0], qf[m][ks][1], qf[m][ks][2], qf[m][ks][3], b[2], b[3]);
+                }
+            }
+        }
+        const uint32_t keys = there[(it % RING) * 2 + (wk >> 1)] >> ((wk & 1) * 16) & 0xffffu;
+        const uint32_t spoilt = draft ? badw[(it % RING) * 2 + (wk >> 1)] >> ((wk & 1) * 16) & 0xffffu : 0u;
+        uint32_t seen[RM][2];
+#pragma unroll
+        for (int m = 0; m < RM; ++m) seen[m][0] = seen[m][1] = keys;
+        if (draft) {
+#pragma unroll
+            for (int m = 0; m < RM; ++m) {
+                int n, h;
+                uint32_t mine = 0;
+                const int tile0 = (at.tile - (at.tiles - p.draft_tiles)) * kTile;
+                if (lane < 16 && row_of(p, at.unit, (wr * RM + m) * 16 + lane, n, h)) mine = (uint32_t)(draft_mask(p, at.b, n, tile0, &bad) >> kw) & 0xffffu;
+                seen[m][0] &= __shfl_sync(0xffffffffu, mine, g);
+                seen[m][1] &= __shfl_sync(0xffffffffu, mine, g + 8);
+            }
+        }
+        if (draft || keys != 0xffffu) {
+#pragma unroll
+            for (int m = 0; m < RM; ++m)
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(seen[m][e >> 1] >> (nt * 8 + 2 * r4 + (e & 1)) & 1)) s[m][nt][e] = -INFINITY;
+        }
+        uint32_t pf[RM][4];
+#pragma unroll
+        for (int m = 0; m < RM; ++m) {
+            float top[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                top[half] = p.c * fmaxf(fmaxf(s[m][0][2 * half], s[m][0][2 * half + 1]), fmaxf(s[m][1][2 * half], s[m][1][2 * half + 1]));
+            if (__any_sync(0xffffffffu, top[0] > ref[m][0] + (kLag<T> + kBias<T>) || top[1] > ref[m][1] + (kLag<T> + kBias<T>))) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float t = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                    const float now = fmaxf(ref[m][half], t - kBias<T>);
+                    const float keep = now == -INFINITY ? 1.f : ex2_approx(ref[m][half] - now);
+                    ref[m][half] = now;
+                    mass[m][half] *= keep;
+#pragma unroll
+                    for (int d = 0; d < DV / 8; ++d) {
+                        o[m][d][2 * half] *= keep;
+                        o[m][d][2 * half + 1] *= keep;
+                    }
+                }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float base = ref[m][half] == -INFINITY ? 0.f : -ref[m][half];
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[i] = ex2_approx(fmaf(s[m][i >> 1][2 * half + (i & 1)], p.c, base));
+                mass[m][half] += (e[0] + e[1]) + (e[2] + e[3]);
+                pf[m][half] = Frag<T>::pack(e[0], e[1]);
+                pf[m][half + 2] = Frag<T>::pack(e[2], e[3]);
+            }
+        }
+        {
+            const int row = kw + (((lane >> 3) & 1) << 3) + (lane & 7), c0 = lane >> 4;
+#pragma unroll
+            for (int d = 0; d < DV / 16; ++d) {
+                uint32_t b[4];
+                ldmatrix4_trans(b, vbase + row * (DV * 2) + (((d * 2 + c0) ^ (row & 7)) << 4));
+#pragma unroll
+                for (int m = 0; m < RM; ++m) {
+                    Frag<T>::mma(o[m][2 * d], pf[m][0], pf[m][1], pf[m][2], pf[m][3], b[0], b[1]);
+                    Frag<T>::mma(o[m][2 * d + 1], pf[m][0], pf[m][1], pf[m][2], pf[m][3], b[2], b[3]);
+                }
+            }
+        }
+        if (spoilt)
+            for (int j = 0; j < 16; ++j) {
+                if (!(spoilt >> j & 1)) continue;
+                const int n = (at.tile - (at.tiles - p.draft_tiles)) * kTile + kw + j;
+                const char* v = p.v + at.b * p.v_b + n * p.v_n + at.unit / p.row_tiles * p.v_h;
+#pragma unroll
+                for (int m = 0; m < RM; ++m)
+#pragma unroll
+                    for (int d = 0; d < DV / 8; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int col = d * 8 + 2 * r4 + (e & 1);
+                            if ((seen[m][e >> 1] >> j & 1) && col < p.V) o[m][d][e] = put_back<T>(o[m][d][e], v, col);
+                        }
+            }
+        const bool done = at.tile + 1 == at.tiles;
+        if (done || it + 1 == n_tiles) {
+            // the four warps of a row: one reference, sums added, 32 columns at a time
+#pragma unroll
+            for (int m = 0; m < RM; ++m)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float x = mass[m][half];
+                    x += __shfl_xor_sync(0xffffffffu, x, 1);
+                    x += __shfl_xor_sync(0xffffffffu, x, 2);
+                    const int row = (wr * RM + m) * 16 + half * 8 + g;
+                    if (r4 == 0) { wm[wk * ROWS + row] = ref[m][half]; wl[wk * ROWS + row] = x; }
+                }
+            __syncthreads();
+            const bool whole = done && first_tile == 0;
+            float* slot = p.part + (int64_t)(2 * blockIdx.x + (first_piece ? 0 : 1)) * ROWS * (p.V + 2);
+            float f[RM][2];
+#pragma unroll
+            for (int m = 0; m < RM; ++m)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int row = (wr * RM + m) * 16 + half * 8 + g;
+                    const float t = fmaxf(fmaxf(wm[row], wm[ROWS + row]), fmaxf(wm[2 * ROWS + row], wm[3 * ROWS + row]));
+                    f[m][half] = t == -INFINITY ? 1.f : ex2_approx(ref[m][half] - t);
+                }
+#pragma unroll
+            for (int c = 0; c < DV / 32; ++c) {
+#pragma unroll
+                for (int m = 0; m < RM; ++m)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const int row = (wr * RM + m) * 16 + half * 8 + g;
+                            *reinterpret_cast<float2*>(joinb + (wk * ROWS + row) * S::chunk + d * 8 + 2 * r4) =
+                                make_float2(o[m][c * 4 + d][2 * half] * f[m][half], o[m][c * 4 + d][2 * half + 1] * f[m][half]);
+                        }
+                __syncthreads();
+                for (int x = tid; x < ROWS * 8; x += NT) {
+                    const int row = x >> 3, q = (x & 7) * 4, col = c * 32 + q;
+                    int n, h;
+                    if (!row_of(p, at.unit, row, n, h) || col >= p.V) continue;
+                    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 y = *reinterpret_cast<const float4*>(joinb + (i * ROWS + row) * S::chunk + q);
+                        sum.x += y.x; sum.y += y.y; sum.z += y.z; sum.w += y.w;
+                    }
+                    float t = -INFINITY, all_mass = 0.f;
+                    if (whole || c == 0) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) t = fmaxf(t, wm[i * ROWS + row]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) all_mass += t == -INFINITY ? wl[i * ROWS + row] : wl[i * ROWS + row] * ex2_approx(wm[i * ROWS + row] - t);
+                    }
+                    if (whole) {
+                        const bool real = is_draft(p, at.b, n);
+                        const float inv = real ? finish_scale(all_mass) : 0.f;
+                        const int64_t at_out = ((int64_t)at.b * p.N + n) * p.H + h;
+                        uint2 y = make_uint2(Frag<T>::pack(sum.x * inv, sum.y * inv), Frag<T>::pack(sum.z * inv, sum.w * inv));
+                        if (!real) y = make_uint2(0u, 0u);
+                        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + at_out * p.V + col) = y;
+                        if (p.lse && c == 0 && q == 0) p.lse[at_out] = real ? finish_lse(t, all_mass) : -INFINITY;
+                    } else {
+                        *reinterpret_cast<float4*>(slot + row * p.V + col) = sum;
+                        if (c == 0 && q == 0) *reinterpret_cast<float2*>(slot + ROWS * p.V + 2 * row) = make_float2(t, all_mass);
+                    }
+                }
+                __syncthreads();
+            }
+            first_piece = false;
+            fresh = true;
+        }
+        const int b = at.b;
+        at.next(p);
+        if (at.b != b) { bool d = false; draft_length(p, at.b, &d); bad |= d; }
+    }
+    if (bad && p.status) atomicOr(p.status, HTREE_STATUS_CACHE);
+}
+
 // ---- joining the parts -------------------------------------------------------------------------------------------------------
 
 // Block (c, r) joins row r of the unit in which part c starts, if it is the first part that does.
@@ -443,23 +822,54 @@ static void fit_rows(DraftParams& p, int rows, int blocks) {
     p.grid = blocks;
 }
 
+// Which kernel: 16-bit rows of up to 128 go to the tensor cores, with as many rows to a block as there are (16, 32 or 64).
+enum { kGeneric = 0, kMma16, kMma32, kMma64 };
 static void choose(DraftParams& p, int dtype) {
-    const int sms = sm_count() > 0 ? sm_count() : 148;
+    const int sms = sm_count() > 0 ? sm_count() : 148, rows = p.N * p.G;
+    if (dtype == HTREE_F32 || p.K > 128 || p.V > 128) {
+        p.variant = kGeneric;
+        fit_rows(p, kGenRows, sms * (generic_smem(p) <= 110 * 1024 ? 2 : 1));
+        return;
+    }
+    p.variant = rows <= 16 ? kMma16 : rows <= 32 ? kMma32 : kMma64;
+    fit_rows(p, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, rows <= 16 ? 2 * sms : sms);
+    if (p.c < 0.f) { p.neg = 1; p.c = -p.c; }
+    if (p.c < 1.1754944e-38f) p.c = 1.1754944e-38f;        // a scale of zero: scores of zero, but what is masked stays minus infinity
+}
+
+template <typename T, int DK, int DV, int WR, int RM>
+static int launch_mma(const DraftParams& p, cudaStream_t st) {
+    static SmemLimit limit;
+    constexpr size_t smem = MmaSmem<T, DK, DV, WR, RM>::total;
+    if (const cudaError_t e = limit.raise((const void*)draft_mma_kernel<T, DK, DV, WR, RM>, smem)) return (int)e;
+    return launch_chained(draft_mma_kernel<T, DK, DV, WR, RM>, dim3(p.grid), dim3(WR * 128), smem, st, p);
+}
+template <typename T, int DK, int DV>
+static int launch_mma(const DraftParams& p, cudaStream_t st) {
+    return p.variant == kMma16 ? launch_mma<T, DK, DV, 1, 1>(p, st) : p.variant == kMma32 ? launch_mma<T, DK, DV, 2, 1>(p, st) : launch_mma<T, DK, DV, 2, 2>(p, st);
+}
+
+template <typename T>
+static int launch_generic(const DraftParams& p, cudaStream_t st) {
+    static SmemLimit limit1, limit2;
     const size_t smem = generic_smem(p);
-    fit_rows(p, kGenRows, sms * (smem <= 110 * 1024 ? 2 : 1));
+    if (p.V <= 128) {
+        if (const cudaError_t e = limit1.raise((const void*)draft_generic_kernel<T, 1>, smem)) return (int)e;
+        return launch_chained(draft_generic_kernel<T, 1>, dim3(p.grid), dim3(kGenThreads), smem, st, p);
+    }
+    if (const cudaError_t e = limit2.raise((const void*)draft_generic_kernel<T, 2>, smem)) return (int)e;
+    return launch_chained(draft_generic_kernel<T, 2>, dim3(p.grid), dim3(kGenThreads), smem, st, p);
 }
 
 template <typename T>
 static int launch_draft(const DraftParams& p, cudaStream_t st) {
     int rc;
-    static SmemLimit limit1, limit2;
-    const size_t smem = generic_smem(p);
-    if (p.V <= 128) {
-        if (const cudaError_t e = limit1.raise((const void*)draft_generic_kernel<T, 1>, smem)) return (int)e;
-        rc = launch_chained(draft_generic_kernel<T, 1>, dim3(p.grid), dim3(kGenThreads), smem, st, p);
+    if constexpr (sizeof(T) == 4) {
+        rc = launch_generic<T>(p, st);
     } else {
-        if (const cudaError_t e = limit2.raise((const void*)draft_generic_kernel<T, 2>, smem)) return (int)e;
-        rc = launch_chained(draft_generic_kernel<T, 2>, dim3(p.grid), dim3(kGenThreads), smem, st, p);
+        rc = p.variant == kGeneric ? launch_generic<T>(p, st)
+           : p.K <= 64 ? (p.V <= 64 ? launch_mma<T, 64, 64>(p, st) : launch_mma<T, 64, 128>(p, st))
+                       : (p.V <= 64 ? launch_mma<T, 128, 64>(p, st) : launch_mma<T, 128, 128>(p, st));
     }
     if (rc || p.grid == 1) return rc;
     return launch_chained(draft_join_kernel<T>, dim3(p.grid - 1, p.rows), dim3(kJoinThreads), 0, st, p);
