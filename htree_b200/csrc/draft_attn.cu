@@ -1,18 +1,18 @@
 // Attention of drafted tokens over a paged cache and over the drafts that lead to them.
 //
 // Work: the query rows that share a key/value head (drafts x heads of the group) are cut into row tiles; a unit is a request, a key/value
-// head and a row tile, and its keys are tiles of 64: the cached tokens first, then the drafts.  All tiles of all units stand in one line
-// that is cut into equal parts, one per block, whatever the lengths (which only the device knows).  A unit that lies in one part is
-// finished there; of the others every part leaves its unnormalised sum, its maximum and its mass, which a second kernel joins in the order
-// of the parts: the result does not depend on timing.
+// head and a row tile, and its keys are tiles: the cached tokens first, then the drafts.  All tiles of all units stand in one line that is
+// cut into equal parts, one per block, whatever the lengths (which only the device knows).  A unit that lies in one part is finished
+// there; of the others every part leaves its unnormalised sum, its reference and its mass, which a second kernel joins in the order of the
+// parts: the result does not depend on timing.
 #include "cache.cuh"
 #include "mma_common.cuh"
 
 namespace htree {
 
-constexpr int kTile = 64;                 // keys of a tile
 constexpr int kMaxTree = 1024;
 constexpr int64_t kMaxLength = int64_t(1) << 30;
+constexpr int kSlice = 16, kTile = 64;    // keys of a tile: tensor-core kernel, fp32 kernel
 
 struct DraftParams {
     const char* q;
@@ -25,30 +25,33 @@ struct DraftParams {
     const int32_t* parents;
     void* out;
     float* lse;
-    float* part;              // per slot: rows x V sums, then rows x {maximum, mass}; slots 2c and 2c+1 are block c's first and last unit
+    float* part;              // per slot: rows x V sums, then rows x {reference, mass}; slots 2c and 2c+1 are part c's first and last unit
+    int4* tasks;              // what there is to join: per unit, or per part where there are more units than parts (see Task)
     int32_t* status;
     int64_t q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h;                  // strides in bytes
     int64_t ck_page, ck_row, ck_h, cv_page, cv_row, cv_h;
     int64_t table_stride;
     int32_t B, N, H, Hkv, G, K, V, M, pages;
-    int32_t rows, row_tiles, draft_tiles, grid;                            // rows of a tile
+    int32_t rows, row_tiles, shift, draft_tiles;                           // rows of a row tile, log2 of the keys of a tile
+    int32_t room;             // tokens that a row of the table can name
+    int32_t grid, least, by_unit;                                          // parts at most; tiles of a part at least; how tasks are indexed
     int32_t variant;          // which kernel (choose)
     int32_t neg;              // tensor-core kernels: the scale is negative, c its magnitude and q's signs are turned
     float c;                  // scale * log2 e
-    FastDiv page, group;      // by G
+    FastDiv page, group, per_head;      // by the page size, by G, by row_tiles
 };
 
 // ---- the line of tiles -------------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ int draft_length(const DraftParams& p, int b, bool* bad) {
-    int64_t len = p.lengths[b], room = (int64_t)p.M * p.page.d;
-    if (room > kMaxLength) room = kMaxLength;
-    if (len < 0 || len > room) { *bad = true; len = len < 0 ? 0 : room; }
-    return (int)len;
+    const int len = p.lengths[b], in = min(max(len, 0), p.room);
+    if (in != len) *bad = true;
+    return in;
 }
+__device__ __forceinline__ int tiles_for(const DraftParams& p, int len) { return ((len + (1 << p.shift) - 1) >> p.shift) + p.draft_tiles; }
 __device__ __forceinline__ int draft_tiles_of(const DraftParams& p, int b) {
     bool dull = false;
-    return (draft_length(p, b, &dull) + kTile - 1) / kTile + p.draft_tiles;
+    return tiles_for(p, draft_length(p, b, &dull));
 }
 
 // Where a part of the line is: request, unit of the request (head * row_tiles + row tile), tile of the unit.
@@ -58,7 +61,7 @@ struct Place {
         bool dull = false;
         b = b_;
         len = draft_length(p, b, &dull);
-        tiles = (len + kTile - 1) / kTile + p.draft_tiles;
+        tiles = tiles_for(p, len);
     }
     __device__ __forceinline__ void next(const DraftParams& p) {
         if (++tile < tiles) return;
@@ -69,52 +72,101 @@ struct Place {
     }
 };
 
-// Blocks that take part, and where block c's part starts.
-__device__ __forceinline__ int64_t parts_of(const DraftParams& p, int64_t all) { return all < p.grid ? all : p.grid; }
-__device__ __forceinline__ int64_t part_start(int64_t c, int64_t all, int64_t parts) { return c * all / parts; }
+// The line and its parts, in 32 bits where it fits them (a 64-bit division takes as long as a load): the first `more` parts have each + 1
+// tiles, the others `each`.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) { return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b); }
+struct Line {
+    int64_t all, each, more;
+    int parts;
+    Line() = default;
+    __device__ __forceinline__ Line(const DraftParams& p, int64_t all_) : all(all_) {
+        parts = all >= (int64_t)p.grid * p.least ? p.grid : (int)(((uint32_t)all + p.least - 1) / (uint32_t)p.least);
+        each = divide(all, parts);
+        more = all - each * parts;
+    }
+    __device__ __forceinline__ int64_t start(int64_t c) const { return c * each + (c < more ? c : more); }
+    __device__ __forceinline__ int part_of(int64_t x) const {
+        const int64_t big = more * (each + 1);
+        return (int)(x < big ? divide(x, each + 1) : more + divide(x - big, each));
+    }
+};
 
-// All tiles of the line (returned), and the place of tile x(all): every thread takes a stretch of requests, one scan over the block.
-template <int NT, typename X>
-__device__ __forceinline__ int64_t find_place(const DraftParams& p, X x, Place& at) {
-    __shared__ int64_t scratch[NT / 32];
-    __shared__ int64_t found[2];
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, per = (p.B + NT - 1) / NT;
-    const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B), units = p.Hkv * p.row_tiles;
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += draft_tiles_of(p, b);
-    int64_t in = mine;
+// The line, and the place where this block's part starts (x0; it ends before x1).  False for a block without a part.  Every thread takes a
+// stretch of requests: of a warp's where there are few, so that no warp waits for another, of the block's where there are many.
+__device__ __forceinline__ uint32_t scan_tiles(const DraftParams& p, int me, int threads, uint32_t& mine, uint32_t& before, int& b0) {
+    const int per = threads == 32 ? (p.B + 31) >> 5 : (p.B + threads - 1) / threads, b1 = min(me * per + per, p.B);
+    b0 = min(me * per, p.B);
+    mine = 0;
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) mine += (uint32_t)draft_tiles_of(p, b);
+    uint32_t in = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, in, o);
-        if (lane >= o) in += y;
+        const uint32_t y = __shfl_up_sync(0xffffffffu, in, o);
+        if ((me & 31) >= o) in += y;
     }
-    if (lane == 31) scratch[w] = in;
-    __syncthreads();
-    int64_t before = 0, all = 0;
-    for (int i = 0; i < NT / 32; ++i) {
-        if (i < w) before += scratch[i];
-        all += scratch[i];
+    before = in - mine;
+    return __shfl_sync(0xffffffffu, in, 31);
+}
+// (The tiles of all requests for one unit are below 2^31, which the launch has checked; those of all units need not be.)
+template <int NT>
+__device__ __forceinline__ bool find_part(const DraftParams& p, Place& at, Line& line, int64_t& x0, int64_t& x1) {
+    __shared__ uint32_t scratch[NT / 32], found[2];
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, units = p.Hkv * p.row_tiles;
+    const bool few = p.B <= 128;
+    uint32_t mine, before;
+    int b0;
+    uint32_t all = scan_tiles(p, few ? lane : tid, few ? 32 : NT, mine, before, b0);
+    if (!few) {
+        if (lane == 0) scratch[w] = all;
+        __syncthreads();
+        all = 0;
+#pragma unroll 1
+        for (int i = 0; i < NT / 32; ++i) {
+            if (i < w) before += scratch[i];
+            all += scratch[i];
+        }
     }
-    all *= units;
-    const int64_t want = x(all);
-    before = (before + in - mine) * units;
-    if (want >= before && want < before + mine * units) {
-        int b = b0;
-        int64_t t = draft_tiles_of(p, b);
-        while (want >= before + t * units) { before += t * units; t = draft_tiles_of(p, ++b); }
-        found[0] = b;
-        found[1] = want - before;
+    line = Line(p, (int64_t)all * units);
+    if ((int)blockIdx.x >= line.parts) return false;
+    x0 = line.start(blockIdx.x);
+    x1 = line.start(blockIdx.x + 1);
+    const uint32_t want = (uint32_t)divide(x0, units);               // which tile of the requests, were there one unit each
+    const bool here = want >= before && want < before + mine;
+    int b = b0;
+    if (here)
+#pragma unroll 1
+        for (uint32_t t = draft_tiles_of(p, b); want >= before + t; t = draft_tiles_of(p, ++b)) before += t;
+    if (few) {
+        const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+        b = __shfl_sync(0xffffffffu, b, from);
+        before = __shfl_sync(0xffffffffu, before, from);
+    } else {
+        if (here) { found[0] = (uint32_t)b; found[1] = before; }
+        __syncthreads();
+        b = (int)found[0];
+        before = found[1];
     }
-    __syncthreads();
-    at.enter(p, (int)found[0]);
-    at.unit = (int)(found[1] / at.tiles);
-    at.tile = (int)(found[1] - (int64_t)at.unit * at.tiles);
-    return all;
+    at.enter(p, b);
+    const int64_t in = x0 - (int64_t)before * units;
+    at.unit = (int)divide(in, at.tiles);
+    at.tile = (int)(in - (int64_t)at.unit * at.tiles);
+    return true;
 }
 
+// What there is to join of the unit that starts with tile u0 of the line, in part c: x = its request (-1: nothing), y = the unit of the
+// request, z = part c, w = 2 * parts + (another unit came before it in part c).
+__device__ __forceinline__ void leave_task(const DraftParams& p, const Place& at, int64_t u0, int64_t x0, int c, const Line& line, bool whole) {
+    int4 t = make_int4(-1, 0, 0, 0);
+    if (!whole) t = make_int4(at.b, at.unit, c, 2 * (line.part_of(u0 + at.tiles - 1) - c + 1) + (x0 < u0 ? 1 : 0));
+    if (p.by_unit) p.tasks[(int64_t)at.b * p.Hkv * p.row_tiles + at.unit] = t;
+    else if (!whole) p.tasks[c] = t;
+}
+
+__device__ __forceinline__ int head_of(const DraftParams& p, int unit) { return (int)p.per_head.div((uint32_t)unit); }     // key/value head
 // Row r of a row tile: draft and head.  False behind the last row.
 __device__ __forceinline__ bool row_of(const DraftParams& p, int unit, int r, int& n, int& h) {
-    const int kv = unit / p.row_tiles, row = (unit - kv * p.row_tiles) * p.rows + r;
+    const int kv = head_of(p, unit), row = (unit - kv * p.row_tiles) * p.rows + r;
     n = (int)p.group.div((uint32_t)row);
     h = kv * p.G + row - n * p.G;
     return row < p.N * p.G;
@@ -143,7 +195,7 @@ __device__ __forceinline__ bool is_draft(const DraftParams& p, int b, int n) { r
 __device__ __forceinline__ bool key_row(const DraftParams& p, const Place& at, int kv, int j, const char*& k, const char*& v, bool* bad) {
     const int cached = at.tiles - p.draft_tiles;
     if (at.tile < cached) {
-        const int pos = at.tile * kTile + j;
+        const int pos = (at.tile << p.shift) + j;
         if (pos >= at.len) return false;
         const uint32_t i = p.page.div((uint32_t)pos);
         const int pg = __ldg(p.table + (int64_t)at.b * p.table_stride + i);
@@ -153,7 +205,7 @@ __device__ __forceinline__ bool key_row(const DraftParams& p, const Place& at, i
         v = p.cv + pg * p.cv_page + in * p.cv_row + kv * p.cv_h;
         return true;
     }
-    const int n = (at.tile - cached) * kTile + j;
+    const int n = ((at.tile - cached) << p.shift) + j;
     if (n >= p.N || !is_draft(p, at.b, n)) return false;
     k = p.k + at.b * p.k_b + n * p.k_n + kv * p.k_h;
     v = p.v + at.b * p.v_b + n * p.v_n + kv * p.v_h;
@@ -203,21 +255,17 @@ __global__ void __launch_bounds__(kGenThreads) draft_generic_kernel(const __grid
     chain_enter();
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
     Place at;
-    int64_t x0 = 0, x1 = 0;
-    const int64_t all = find_place<kGenThreads>(p, [&](int64_t n) {
-        const int64_t parts = parts_of(p, n);
-        x0 = part_start(blockIdx.x < parts ? blockIdx.x : 0, n, parts);
-        x1 = part_start(blockIdx.x < parts ? blockIdx.x + 1 : 1, n, parts);
-        return x0;
-    }, at);
-    if (blockIdx.x >= parts_of(p, all)) return;
+    Line line;
+    int64_t x0, x1;
+    if (tid == 0 && !p.by_unit) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (!find_part<kGenThreads>(p, at, line, x0, x1)) return;
     bool bad = false;
     { bool b = false; draft_length(p, at.b, &b); bad |= b; }
     float m[4], mass[4], o[4][4 * VC];
     int first_tile = at.tile;                       // of the unit's part in this block
     bool fresh = true, first_piece = true;
     for (int64_t x = x0; x < x1; ++x) {
-        const int kv = at.unit / p.row_tiles;
+        const int kv = head_of(p, at.unit);
         if (fresh) {
             first_tile = at.tile;
 #pragma unroll
@@ -346,6 +394,7 @@ __global__ void __launch_bounds__(kGenThreads) draft_generic_kernel(const __grid
                     }
                 }
             }
+            if (tid == 0 && first_tile == 0) leave_task(p, at, x - at.tile, x0, blockIdx.x, line, whole);
             first_piece = false;
             fresh = true;
         }
@@ -356,11 +405,12 @@ __global__ void __launch_bounds__(kGenThreads) draft_generic_kernel(const __grid
     if (bad && p.status) atomicOr(p.status, HTREE_STATUS_CACHE);
 }
 
-// ---- 16-bit types: mma.sync -----------------------------------------------------------------------------------------------------
+// ---- 16-bit types, up to 32 query rows: mma.sync ---------------------------------------------------------------------------------
 
-// Up to 64 query rows: HBM bounds these, so the tiles stream through a ring of cp.async stages and the products only have to keep up.  A
-// warp owns 16 keys of every tile and RM x 16 rows with a softmax of its own (reference, mass and sums in registers); the four warps that
-// share rows are joined when the unit ends.  With the rows a block holds, WR = 1 or 2 rows of warps.
+// HBM bounds these: the products only have to keep up.  A tile is 16 keys and belongs to one warp, with a softmax of its own (reference,
+// mass and sums in registers) and a ring of its own in shared memory that the warp fills by cp.async: the warps of a block do not wait for
+// one another until the unit ends.  The line is cut into parts of whole blocks; the tiles of a part go round the block's warps.
+// (One bulk copy of 256 bytes per lane and row instead: the compiler issues them lane by lane, 790 instructions a tile.)
 //
 // The reference of a row is not its running maximum but within kLag of it (powers of two that P may grow by before the sums are
 // rescaled), so almost every tile needs one vote and no shuffles.  P is rounded to the type, half a step each; for fp16 the reference
@@ -373,16 +423,17 @@ template <> constexpr float kBias<__half> = 8.f;
 template <typename T> constexpr uint32_t kExpMask = 0x7f80u;
 template <> constexpr uint32_t kExpMask<__half> = 0x7c00u;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool on) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 
 // Values of drafts that are not finite must not meet the zero weights of the rows that do not read them: they are taken out of the tile
@@ -408,103 +459,196 @@ __device__ __forceinline__ float put_back(float o, const char* v, int col) {
     return fabsf(x) <= 3.4028234e38f ? o : o + x;
 }
 
-struct RowPtr { const char* k; const char* v; };
-
-template <int DK, int DV, int WR> struct MmaShape {
-    static constexpr int threads = WR * 128, stage = kTile * (DK + DV) * 2;
-    static constexpr int stages = WR == 1 ? (stage > 24576 ? 3 : stage > 16384 ? 4 : 5) : (stage > 24576 ? 4 : 6);
-    static constexpr int ring = 8;                             // of row pointers and key masks: at least stages + 2
-    static_assert(stages + 2 <= ring, "");
-    static constexpr int chunk = 32 + 4;                       // columns of a joining round, padded
+template <int DK, int DV, int RM> struct MmaShape {
+    static constexpr int warps = RM == 1 ? 12 : 8, threads = warps * 32, rows = RM * 16;
+    static constexpr int krow = DK * 2 + 16, vrow = DV * 2 + 16;             // 16 bytes more than a row: eight rows meet in no bank
+    static constexpr int stage = kSlice * (krow + vrow);
+    // columns of a joining round: what fits into the stage that the unit's last tile has left
+    static constexpr int cols = DV == 128 && rows * 132 * 4 <= stage ? 128 : rows * 68 * 4 <= stage ? 64 : 32, jrow = cols + 4;
+    static_assert(rows * jrow * 4 <= stage, "");
+    static constexpr int fixed = 2 * warps * rows * 4 + 2 * rows * 4 + rows * krow;
+    static constexpr int fit = (232448 - 512 - fixed) / (warps * stage);
+    static constexpr int stages = fit > 4 ? 4 : fit;
+    static_assert(stages >= 2, "");
+    static constexpr int wm = 0, wl = wm + warps * rows * 4, sums = wl + warps * rows * 4, q = sums + 2 * rows * 4, ring = (q + rows * krow + 127) / 128 * 128,
+                         total = ring + warps * stages * stage;
 };
 
-template <typename T, int DK, int DV, int WR, int RM>
-struct MmaSmem {
-    using S = MmaShape<DK, DV, WR>;
-    static constexpr int rows = WR * RM * 16;
-    static constexpr int tiles = 0, ptrs = S::stages * S::stage, there = ptrs + S::ring * kTile * (int)sizeof(RowPtr), bad = there + S::ring * 8,
-                         wm = bad + S::ring * 8, wl = wm + 4 * rows * 4, join = wl + 4 * rows * 4, total = join + 4 * rows * S::chunk * 4;
-};
-
-template <typename T, int DK, int DV, int WR, int RM>
-__global__ void __launch_bounds__(WR * 128, WR == 1 ? 2 : 1) draft_mma_kernel(const __grid_constant__ DraftParams p) {
-    using S = MmaShape<DK, DV, WR>;
-    using L = MmaSmem<T, DK, DV, WR, RM>;
-    constexpr int NT = S::threads, ST = S::stages, RING = S::ring, ROWS = L::rows, KP = DK / 8, VP = DV / 8;
+// The code of a part runs few times over (a handful of tiles, one or two joins), and instructions that run for the first time come at 8 to
+// 10 cycles each: one loop, in which fetching, computing and joining stand once each, nothing unrolled that need not be.  (Unrolled, with
+// the prologue and every refill inlined, a call of 1024 cached tokens took 38,000 cycles, 26,000 of them outside the tiles.)
+template <typename T, int DK, int DV, int RM>
+__global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_kernel(const __grid_constant__ DraftParams p) {
+    using S = MmaShape<DK, DV, RM>;
+    constexpr int NT = S::threads, NW = S::warps, ST = S::stages, ROWS = S::rows;
     extern __shared__ __align__(128) unsigned char sm[];
-    RowPtr* ptrs = reinterpret_cast<RowPtr*>(sm + L::ptrs);
-    uint32_t* there = reinterpret_cast<uint32_t*>(sm + L::there);       // [ring][2]
-    uint32_t* badw = reinterpret_cast<uint32_t*>(sm + L::bad);
-    float* wm = reinterpret_cast<float*>(sm + L::wm);
-    float* wl = reinterpret_cast<float*>(sm + L::wl);
-    float* joinb = reinterpret_cast<float*>(sm + L::join);
+    float* wm = reinterpret_cast<float*>(sm + S::wm);
+    float* wl = reinterpret_cast<float*>(sm + S::wl);
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, r4 = lane & 3;
+    float* scale_of = reinterpret_cast<float*>(sm + S::sums);
+    int* stage_of = reinterpret_cast<int*>(sm + S::sums) + ROWS;
+    unsigned char* ring = sm + S::ring + w * ST * S::stage;
+    const uint32_t ring_u = smem_u32(ring), q_u = smem_u32(sm + S::q);
+    if (p.K < DK || p.V < DV) {        // columns that no copy writes
+        for (int i = lane; i < ST * S::stage / 16; i += 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < ROWS * S::krow / 16; i += NT) reinterpret_cast<uint4*>(sm + S::q)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
     chain_enter();
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, wk = w & 3, wr = w >> 2, kw = wk * 16, g = lane >> 2, r4 = lane & 3;
     Place at;
-    int64_t x0 = 0, x1 = 0;
-    const int64_t all = find_place<NT>(p, [&](int64_t n) {
-        const int64_t parts = parts_of(p, n);
-        x0 = part_start(blockIdx.x < parts ? blockIdx.x : 0, n, parts);
-        x1 = part_start(blockIdx.x < parts ? blockIdx.x + 1 : 1, n, parts);
-        return x0;
-    }, at);
-    if (blockIdx.x >= parts_of(p, all)) return;
+    Line line;
+    int64_t x0, x1;
+    if (tid == 0 && !p.by_unit) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (!find_part<NT>(p, at, line, x0, x1)) return;
     const int n_tiles = (int)(x1 - x0);
     bool bad = false;
     { bool b = false; draft_length(p, at.b, &b); bad |= b; }
-    if (tid < 2 * RING) badw[tid] = 0;
 
-    Place ahead = at;                  // of the tile whose row pointers are made next
-    int made = 0;
-    auto make_row = [&](const Place& pl, int tile, int j) {
-        RowPtr rp{p.q, p.q};           // (never read: copies of rows that are not there have no source)
-        const bool on = key_row(p, pl, pl.unit / p.row_tiles, j, rp.k, rp.v, &bad);
-        const uint32_t m = __ballot_sync(0xffffffffu, on);
-        if (lane == 0) there[(tile % RING) * 2 + (j >> 5)] = m;
-        if (!on) rp = RowPtr{nullptr, nullptr};
-        ptrs[(tile % RING) * kTile + j] = rp;
-    };
-    // the first stages' pointers at once: threads 0-63 the first tile, 64-127 the second, ...
-    for (int i = 0; i < ST && i < n_tiles; ++i) {
-        if ((i * 2) % (NT / 32) <= w && w < (i * 2) % (NT / 32) + 2) make_row(ahead, i, tid % 64);
-        ahead.next(p);
-        ++made;
-    }
-    __syncthreads();
-    const uint32_t tiles_u = smem_u32(sm);
-    auto issue = [&](int tile) {
-        const uint32_t base = tiles_u + (tile % ST) * S::stage;
-        const RowPtr* rows = ptrs + (tile % RING) * kTile;
-#pragma unroll
-        for (int i = 0; i < kTile * KP / NT; ++i) {
-            const int x = i * NT + tid, j = x / KP, c = x % KP;
-            const char* src = rows[j].k;
-            const bool on = src != nullptr && c * 8 < p.K;
-            cp_async16(base + j * (DK * 2) + ((c ^ (j & 7)) << 4), on ? src + c * 16 : p.q, on);
-        }
-#pragma unroll
-        for (int i = 0; i < kTile * VP / NT; ++i) {
-            const int x = i * NT + tid, j = x / VP, c = x % VP;
-            const char* src = rows[j].v;
-            const bool on = src != nullptr && c * 8 < p.V;
-            cp_async16(base + kTile * DK * 2 + j * (DV * 2) + ((c ^ (j & 7)) << 4), on ? src + c * 16 : p.q, on);
+    // The rows of q of a unit, to shared memory.
+    auto fetch_q = [&](const Place& pl) {
+#pragma unroll 1
+        for (int i = tid; i < ROWS * (DK / 8); i += NT) {
+            const int r = i / (DK / 8), c = i % (DK / 8);
+            int n, h;
+            const bool on = row_of(p, pl.unit, r, n, h);
+            if (c * 8 < p.K) cp_async16_or_zero(q_u + r * S::krow + c * 16, on ? p.q + pl.b * p.q_b + n * p.q_n + h * p.q_h + c * 16 : p.q, on);
         }
     };
-    for (int i = 0; i < ST - 1; ++i) {
-        if (i < n_tiles) issue(i);
-        cp_async_commit();
-    }
+    fetch_q(at);
 
-    uint32_t qf[RM][DK / 16][4];
+    // This warp's tiles are w, w + NW, ...  `ahead` is the next one to fetch; lane j (and j + 16) knows the page of its key j, read one fetch
+    // before it is needed.
+    Place ahead = at;
+    auto look = [&](const Place& pl) {
+        const int pos = pl.tile * kSlice + (lane & 15);
+        return pl.tile < pl.tiles - p.draft_tiles && pos < pl.len ? __ldg(p.table + (int64_t)pl.b * p.table_stride + p.page.div((uint32_t)pos)) : -1;
+    };
+    constexpr int KL = DK / 8, VL = DV / 8;              // lanes of a row
+    const uint32_t kdst = ring_u + lane / KL * S::krow + lane % KL * 16, vdst = ring_u + kSlice * S::krow + lane / VL * S::vrow + lane % VL * 16;
+    const bool kcol = lane % KL * 8 < p.K, vcol = lane % VL * 8 < p.V;
+    const int64_t kstep = p.ck_row * (32 / KL), vstep = p.cv_row * (32 / VL);
+    uint64_t keys_of = 0;                  // which keys a stage has: 16 bits each
+
     float o[RM][DV / 8][4], ref[RM][2], mass[RM][2];
-    int first_tile = at.tile;
-    bool fresh = true, first_piece = true;
-    const uint32_t flip = p.neg ? 0x80008000u : 0u;
-    for (int it = 0; it < n_tiles; ++it) {
-        const bool draft = at.tile >= at.tiles - p.draft_tiles;
-        if (fresh) {
-            first_tile = at.tile;
-            fresh = false;
+    uint32_t qf[RM][DK / 16][4];
+    int piece = 0, first = 0, end = 0;     // tiles first .. end of the part: the share of the present unit
+    int had = -1;                          // the stage of this warp's last tile of the unit, or -1: it had none
+    bool first_piece = true, q_ready = false;
+    int step = w;                          // how far `ahead` has to go before the next fetch
+    int page_next = -1;
+    for (int k = 0;; ++k) {
+        const int t = k - (ST - 1), mine = w + t * NW;   // the tile to compute in this round
+        while (t >= 0 && mine >= end) {
+            if (piece > 0) {
+                // the block's warps, those that had a tile of the unit: one reference, the sums added, through the stages that they have left
+                if (had >= 0) {
+#pragma unroll
+                    for (int m = 0; m < RM; ++m)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            float x = mass[m][half];
+                            x += __shfl_xor_sync(0xffffffffu, x, 1);
+                            x += __shfl_xor_sync(0xffffffffu, x, 2);
+                            if (r4 == 0) { wm[w * ROWS + m * 16 + half * 8 + g] = ref[m][half]; wl[w * ROWS + m * 16 + half * 8 + g] = x; }
+                        }
+                    if (lane == 0) stage_of[w] = had;
+                }
+                __syncthreads();
+                const int w0 = first % NW, some = piece < NW ? piece : NW;       // warps w0, w0 + 1, ... (round the block)
+                const bool whole = at.tile == 0 && piece == at.tiles;
+                float* slot = p.part + (int64_t)(2 * blockIdx.x + (first_piece ? 0 : 1)) * ROWS * (p.V + 2);
+                float joint = -INFINITY;                 // lane: of row `lane` (or lane & 15)
+                const int jr = lane & (ROWS - 1);
+#pragma unroll 4
+                for (int i = 0, x = w0; i < some; ++i, x = x + 1 == NW ? 0 : x + 1) joint = fmaxf(joint, wm[x * ROWS + jr]);
+                if (w == 0 && lane < ROWS) {
+                    float sum = 0.f, f = 1.f;
+#pragma unroll 1
+                    for (int i = 0, x = w0; i < some; ++i, x = x + 1 == NW ? 0 : x + 1)
+                        sum += joint == -INFINITY ? wl[x * ROWS + lane] : wl[x * ROWS + lane] * ex2_approx(wm[x * ROWS + lane] - joint);
+                    int n, h;
+                    if (row_of(p, at.unit, lane, n, h)) {
+                        if (whole) {
+                            const bool real = is_draft(p, at.b, n);
+                            f = real ? finish_scale(sum) : -1.f;            // (a scale is never negative: -1 marks what is no draft)
+                            if (p.lse) p.lse[((int64_t)at.b * p.N + n) * p.H + h] = real ? finish_lse(joint, sum) : -INFINITY;
+                        } else {
+                            *reinterpret_cast<float2*>(slot + ROWS * p.V + 2 * lane) = make_float2(joint, sum);
+                        }
+                    }
+                    scale_of[lane] = f;
+                }
+                float f[RM][2];
+#pragma unroll
+                for (int m = 0; m < RM; ++m)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const float j = __shfl_sync(0xffffffffu, joint, m * 16 + half * 8 + g);
+                        f[m][half] = j == -INFINITY ? 1.f : ex2_approx(ref[m][half] - j);
+                    }
+#pragma unroll
+                for (int c = 0; c < DV / S::cols; ++c) {
+                    if (c > 0) __syncthreads();
+                    if (had >= 0) {
+                        float* own = reinterpret_cast<float*>(ring + had * S::stage);
+#pragma unroll
+                        for (int m = 0; m < RM; ++m)
+#pragma unroll
+                            for (int d = 0; d < S::cols / 8; ++d)
+#pragma unroll
+                                for (int half = 0; half < 2; ++half)
+                                    *reinterpret_cast<float2*>(own + (m * 16 + half * 8 + g) * S::jrow + d * 8 + 2 * r4) =
+                                        make_float2(o[m][c * (S::cols / 8) + d][2 * half] * f[m][half], o[m][c * (S::cols / 8) + d][2 * half + 1] * f[m][half]);
+                    }
+                    __syncthreads();
+#pragma unroll 1
+                    for (int y = tid; y < ROWS * (S::cols / 4); y += NT) {
+                        const int row = y / (S::cols / 4), q = y % (S::cols / 4) * 4, col = c * S::cols + q;
+                        int n, h;
+                        if (row_of(p, at.unit, row, n, h) && col < p.V) {
+                            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                            for (int i = 0, x = w0; i < some; ++i, x = x + 1 == NW ? 0 : x + 1) {
+                                const float4 v = *reinterpret_cast<const float4*>(sm + S::ring + (x * ST + stage_of[x]) * S::stage + (row * S::jrow + q) * 4);
+                                sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+                            }
+                            if (whole) {
+                                const float z = scale_of[row];
+                                uint2 v = make_uint2(Frag<T>::pack(sum.x * z, sum.y * z), Frag<T>::pack(sum.z * z, sum.w * z));
+                                if (z < 0.f) v = make_uint2(0u, 0u);
+                                *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + (((int64_t)at.b * p.N + n) * p.H + h) * p.V + col) = v;
+                            } else {
+                                *reinterpret_cast<float4*>(slot + row * p.V + col) = sum;
+                            }
+                        }
+                    }
+                }
+                if (tid == 0 && at.tile == 0) leave_task(p, at, x0 + first, x0, blockIdx.x, line, whole);
+                first_piece = false;
+                if (end == n_tiles) {
+                    if (bad && p.status) atomicOr(p.status, HTREE_STATUS_CACHE);
+                    return;
+                }
+                const int b = at.b;
+                at.tile += piece - 1;
+                at.next(p);
+                if (at.b != b) { bool d = false; draft_length(p, at.b, &d); bad |= d; }
+                fetch_q(at);
+                cp_async_commit();
+                cp_async_wait<0>();
+                __syncthreads();
+                if (had >= 0 && (p.K < DK || p.V < DV)) {
+                    for (int i = lane; i < S::stage / 16; i += 32) reinterpret_cast<uint4*>(ring + had * S::stage)[i] = make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+                }
+            } else {
+                cp_async_wait<0>();                      // q, with the first tiles
+                __syncthreads();
+            }
+            first = end;
+            piece = min(n_tiles - first, at.tiles - at.tile);
+            end = first + piece;
+            had = -1;
 #pragma unroll
             for (int m = 0; m < RM; ++m) {
                 ref[m][0] = ref[m][1] = -INFINITY;
@@ -513,39 +657,105 @@ __global__ void __launch_bounds__(WR * 128, WR == 1 ? 2 : 1) draft_mma_kernel(co
                 for (int d = 0; d < DV / 8; ++d)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[m][d][e] = 0.f;
+                const uint32_t a = q_u + (m * 16 + (lane & 15)) * S::krow + (lane >> 4) * 16;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    int n, h;
-                    const bool on = row_of(p, at.unit, (wr * RM + m) * 16 + half * 8 + g, n, h);
-                    const char* src = p.q + at.b * p.q_b + n * p.q_n + h * p.q_h + 4 * r4;
+                for (int ks = 0; ks < DK / 16; ++ks) ldmatrix4(qf[m][ks], a + ks * 32);
+            }
+            if (p.neg)
+#pragma unroll
+                for (int m = 0; m < RM; ++m)
 #pragma unroll
                     for (int ks = 0; ks < DK / 16; ++ks)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            qf[m][ks][half + 2 * e] = on && ks * 16 + e * 8 < p.K ? __ldg(reinterpret_cast<const uint32_t*>(src + ks * 32 + e * 16)) ^ flip : 0u;
+                        for (int e = 0; e < 4; ++e) qf[m][ks][e] ^= 0x80008000u;
+        }
+
+        // fetch tile k of this warp
+        const int stage = k % ST;
+        if (w + k * NW < n_tiles) {
+            ahead.tile += step;
+            step = NW;
+            while (ahead.tile >= ahead.tiles) {
+                ahead.tile -= ahead.tiles;
+                if (++ahead.unit == p.Hkv * p.row_tiles) {
+                    ahead.unit = 0;
+                    ahead.enter(p, ahead.b + 1);
+                }
+                page_next = -2;
+            }
+            int page_of = k == 0 || page_next == -2 ? look(ahead) : page_next;
+            const int kv = head_of(p, ahead.unit), pos0 = ahead.tile * kSlice;
+            const uint32_t in0 = (uint32_t)pos0 - p.page.div((uint32_t)pos0) * p.page.d;
+            uint32_t m = 0xffffu;
+            const uint32_t kd = kdst + stage * S::stage, vd = vdst + stage * S::stage;
+            __syncwarp();                  // every lane has read what the stage held
+            if (ahead.tile < ahead.tiles - p.draft_tiles && pos0 + kSlice <= ahead.len && in0 + kSlice <= p.page.d && page_of >= 0 && page_of < p.pages) {
+                // sixteen tokens of one page (the same one in every lane)
+                const char* ks = p.ck + page_of * p.ck_page + (in0 + lane / KL) * p.ck_row + kv * p.ck_h + lane % KL * 16;
+                const char* vs = p.cv + page_of * p.cv_page + (in0 + lane / VL) * p.cv_row + kv * p.cv_h + lane % VL * 16;
+                if (kcol)
+#pragma unroll
+                    for (int i = 0; i < kSlice * KL / 32; ++i, ks += kstep) cp_async16(kd + i * (32 / KL) * S::krow, ks);
+                if (vcol)
+#pragma unroll
+                    for (int i = 0; i < kSlice * VL / 32; ++i, vs += vstep) cp_async16(vd + i * (32 / VL) * S::vrow, vs);
+            } else {
+                const char *ks = p.q, *vs = p.q;         // (a row that is not there has no source)
+                bool on = false;
+                if (ahead.tile < ahead.tiles - p.draft_tiles) {
+                    const int pos = pos0 + (lane & 15);
+                    on = pos < ahead.len;
+                    if (on && (page_of < 0 || page_of >= p.pages)) { bad = true; on = false; }
+                    if (on) {
+                        const int64_t in = (int64_t)(pos - p.page.div((uint32_t)pos) * p.page.d);
+                        ks = p.ck + page_of * p.ck_page + in * p.ck_row + kv * p.ck_h;
+                        vs = p.cv + page_of * p.cv_page + in * p.cv_row + kv * p.cv_h;
+                    }
+                } else {
+                    const int n = (ahead.tile - (ahead.tiles - p.draft_tiles)) * kSlice + (lane & 15);
+                    on = n < p.N && is_draft(p, ahead.b, n);
+                    if (on) {
+                        ks = p.k + ahead.b * p.k_b + n * p.k_n + kv * p.k_h;
+                        vs = p.v + ahead.b * p.v_b + n * p.v_n + kv * p.v_h;
+                    }
+                }
+                m = __ballot_sync(0xffffffffu, on) & 0xffffu;
+#pragma unroll 1
+                for (int i = 0; i < kSlice * KL / 32; ++i) {
+                    const int j = i * (32 / KL) + lane / KL;
+                    const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ks), j));
+                    if (kcol) cp_async16_or_zero(kd + i * (32 / KL) * S::krow, (m >> j & 1) ? src + lane % KL * 16 : p.q, m >> j & 1);
+                }
+#pragma unroll 1
+                for (int i = 0; i < kSlice * VL / 32; ++i) {
+                    const int j = i * (32 / VL) + lane / VL;
+                    const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vs), j));
+                    if (vcol) cp_async16_or_zero(vd + i * (32 / VL) * S::vrow, (m >> j & 1) ? src + lane % VL * 16 : p.q, m >> j & 1);
                 }
             }
+            keys_of = (keys_of & ~(0xffffull << (16 * stage))) | (uint64_t)m << (16 * stage);
+            Place pl = ahead;
+            pl.tile += NW;
+            page_next = look(pl);          // (of no use where the unit ends before: looked up again)
         }
-        cp_async_wait<ST - 2>();
-        if (draft) {                   // what this thread has copied of the tile's values
-            const uint32_t base = tiles_u + (it % ST) * S::stage + kTile * DK * 2;
-#pragma unroll
-            for (int i = 0; i < kTile * VP / NT; ++i) {
-                const int x = i * NT + tid, j = x / VP, c = x % VP;
-                if (take_out<T>(base + j * (DV * 2) + ((c ^ (j & 7)) << 4))) atomicOr(&badw[(it % RING) * 2 + (j >> 5)], 1u << (j & 31));
-            }
-        }
-        __syncthreads();               // the tile is there, and so are the pointers made one round ago; its predecessor's stage is free
-        if (it + ST - 1 < n_tiles) issue(it + ST - 1);
         cp_async_commit();
-        if (made < n_tiles && made <= it + ST) {
-            if (w < 2) make_row(ahead, made, tid);
-            ahead.next(p);
-            ++made;
-        }
-        if (tid < 2) badw[((it + 4) % RING) * 2 + tid] = 0;
+        if (t < 0) continue;
 
-        const uint32_t kbase = tiles_u + (it % ST) * S::stage, vbase = kbase + kTile * DK * 2;
+        const int cached = at.tiles - p.draft_tiles, tile = at.tile + (mine - first), cur = t % ST;
+        const bool draft = tile >= cached;
+        had = cur;
+        cp_async_wait<ST - 1>();
+        __syncwarp();
+        const uint32_t kbase = ring_u + cur * S::stage, vbase = kbase + kSlice * S::krow;
+        const uint32_t keys = (uint32_t)(keys_of >> (16 * cur)) & 0xffffu;
+        uint32_t spoilt = 0;
+        if (draft) {
+#pragma unroll 1
+            for (int x = lane; x < kSlice * (DV / 8); x += 32)
+                if (take_out<T>(vbase + x / (DV / 8) * S::vrow + x % (DV / 8) * 16)) spoilt |= 1u << (x / (DV / 8));
+            spoilt = __reduce_or_sync(0xffffffffu, spoilt);
+            __syncwarp();
+        }
         float s[RM][2][4];
 #pragma unroll
         for (int m = 0; m < RM; ++m)
@@ -554,11 +764,11 @@ __global__ void __launch_bounds__(WR * 128, WR == 1 ? 2 : 1) draft_mma_kernel(co
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[m][nt][e] = 0.f;
         {
-            const int row = kw + ((lane >> 4) << 3) + (lane & 7), c0 = (lane >> 3) & 1;
+            const uint32_t a = kbase + (((lane >> 4) << 3) + (lane & 7)) * S::krow + ((lane >> 3) & 1) * 16;
 #pragma unroll
             for (int ks = 0; ks < DK / 16; ++ks) {
                 uint32_t b[4];
-                ldmatrix4(b, kbase + row * (DK * 2) + (((ks * 2 + c0) ^ (row & 7)) << 4));
+                ldmatrix4(b, a + ks * 32);
 #pragma unroll
                 for (int m = 0; m < RM; ++m) {
                     Frag<T>::mma(s[m][0], qf[m][ks][0], qf[m][ks][1], qf[m][ks][2], qf[m][ks][3], b[0], b[1]);
@@ -566,20 +776,18 @@ __global__ void __launch_bounds__(WR * 128, WR == 1 ? 2 : 1) draft_mma_kernel(co
                 }
             }
         }
-        const uint32_t keys = there[(it % RING) * 2 + (wk >> 1)] >> ((wk & 1) * 16) & 0xffffu;
-        const uint32_t spoilt = draft ? badw[(it % RING) * 2 + (wk >> 1)] >> ((wk & 1) * 16) & 0xffffu : 0u;
         uint32_t seen[RM][2];
 #pragma unroll
         for (int m = 0; m < RM; ++m) seen[m][0] = seen[m][1] = keys;
         if (draft) {
-#pragma unroll
+#pragma unroll 1
             for (int m = 0; m < RM; ++m) {
                 int n, h;
-                uint32_t mine = 0;
-                const int tile0 = (at.tile - (at.tiles - p.draft_tiles)) * kTile;
-                if (lane < 16 && row_of(p, at.unit, (wr * RM + m) * 16 + lane, n, h)) mine = (uint32_t)(draft_mask(p, at.b, n, tile0, &bad) >> kw) & 0xffffu;
-                seen[m][0] &= __shfl_sync(0xffffffffu, mine, g);
-                seen[m][1] &= __shfl_sync(0xffffffffu, mine, g + 8);
+                uint32_t own = 0;
+                if (lane < 16 && row_of(p, at.unit, m * 16 + lane, n, h)) own = (uint32_t)draft_mask(p, at.b, n, (tile - cached) * kSlice, &bad) & 0xffffu;
+                const uint32_t lo = __shfl_sync(0xffffffffu, own, g), hi = __shfl_sync(0xffffffffu, own, g + 8);
+#pragma unroll
+                for (int i = 0; i < RM; ++i) if (i == m) { seen[i][0] &= lo; seen[i][1] &= hi; }
             }
         }
         if (draft || keys != 0xffffu) {
@@ -601,9 +809,9 @@ __global__ void __launch_bounds__(WR * 128, WR == 1 ? 2 : 1) draft_mma_kernel(co
             if (__any_sync(0xffffffffu, top[0] > ref[m][0] + (kLag<T> + kBias<T>) || top[1] > ref[m][1] + (kLag<T> + kBias<T>))) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    float t = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
-                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-                    const float now = fmaxf(ref[m][half], t - kBias<T>);
+                    float x = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                    const float now = fmaxf(ref[m][half], x - kBias<T>);
                     const float keep = now == -INFINITY ? 1.f : ex2_approx(ref[m][half] - now);
                     ref[m][half] = now;
                     mass[m][half] *= keep;
@@ -626,11 +834,11 @@ __global__ void __launch_bounds__(WR * 128, WR == 1 ? 2 : 1) draft_mma_kernel(co
             }
         }
         {
-            const int row = kw + (((lane >> 3) & 1) << 3) + (lane & 7), c0 = lane >> 4;
+            const uint32_t a = vbase + ((((lane >> 3) & 1) << 3) + (lane & 7)) * S::vrow + (lane >> 4) * 16;
 #pragma unroll
             for (int d = 0; d < DV / 16; ++d) {
                 uint32_t b[4];
-                ldmatrix4_trans(b, vbase + row * (DV * 2) + (((d * 2 + c0) ^ (row & 7)) << 4));
+                ldmatrix4_trans(b, a + d * 32);
 #pragma unroll
                 for (int m = 0; m < RM; ++m) {
                     Frag<T>::mma(o[m][2 * d], pf[m][0], pf[m][1], pf[m][2], pf[m][3], b[0], b[1]);
@@ -639,10 +847,10 @@ __global__ void __launch_bounds__(WR * 128, WR == 1 ? 2 : 1) draft_mma_kernel(co
             }
         }
         if (spoilt)
-            for (int j = 0; j < 16; ++j) {
+#pragma unroll 1
+            for (int j = 0; j < kSlice; ++j) {
                 if (!(spoilt >> j & 1)) continue;
-                const int n = (at.tile - (at.tiles - p.draft_tiles)) * kTile + kw + j;
-                const char* v = p.v + at.b * p.v_b + n * p.v_n + at.unit / p.row_tiles * p.v_h;
+                const char* v = p.v + at.b * p.v_b + ((tile - cached) * kSlice + j) * p.v_n + head_of(p, at.unit) * p.v_h;
 #pragma unroll
                 for (int m = 0; m < RM; ++m)
 #pragma unroll
@@ -653,142 +861,66 @@ __global__ void __launch_bounds__(WR * 128, WR == 1 ? 2 : 1) draft_mma_kernel(co
                             if ((seen[m][e >> 1] >> j & 1) && col < p.V) o[m][d][e] = put_back<T>(o[m][d][e], v, col);
                         }
             }
-        const bool done = at.tile + 1 == at.tiles;
-        if (done || it + 1 == n_tiles) {
-            // the four warps of a row: one reference, sums added, 32 columns at a time
-#pragma unroll
-            for (int m = 0; m < RM; ++m)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    float x = mass[m][half];
-                    x += __shfl_xor_sync(0xffffffffu, x, 1);
-                    x += __shfl_xor_sync(0xffffffffu, x, 2);
-                    const int row = (wr * RM + m) * 16 + half * 8 + g;
-                    if (r4 == 0) { wm[wk * ROWS + row] = ref[m][half]; wl[wk * ROWS + row] = x; }
-                }
-            __syncthreads();
-            const bool whole = done && first_tile == 0;
-            float* slot = p.part + (int64_t)(2 * blockIdx.x + (first_piece ? 0 : 1)) * ROWS * (p.V + 2);
-            float f[RM][2];
-#pragma unroll
-            for (int m = 0; m < RM; ++m)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int row = (wr * RM + m) * 16 + half * 8 + g;
-                    const float t = fmaxf(fmaxf(wm[row], wm[ROWS + row]), fmaxf(wm[2 * ROWS + row], wm[3 * ROWS + row]));
-                    f[m][half] = t == -INFINITY ? 1.f : ex2_approx(ref[m][half] - t);
-                }
-#pragma unroll
-            for (int c = 0; c < DV / 32; ++c) {
-#pragma unroll
-                for (int m = 0; m < RM; ++m)
-#pragma unroll
-                    for (int d = 0; d < 4; ++d)
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const int row = (wr * RM + m) * 16 + half * 8 + g;
-                            *reinterpret_cast<float2*>(joinb + (wk * ROWS + row) * S::chunk + d * 8 + 2 * r4) =
-                                make_float2(o[m][c * 4 + d][2 * half] * f[m][half], o[m][c * 4 + d][2 * half + 1] * f[m][half]);
-                        }
-                __syncthreads();
-                for (int x = tid; x < ROWS * 8; x += NT) {
-                    const int row = x >> 3, q = (x & 7) * 4, col = c * 32 + q;
-                    int n, h;
-                    if (!row_of(p, at.unit, row, n, h) || col >= p.V) continue;
-                    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float4 y = *reinterpret_cast<const float4*>(joinb + (i * ROWS + row) * S::chunk + q);
-                        sum.x += y.x; sum.y += y.y; sum.z += y.z; sum.w += y.w;
-                    }
-                    float t = -INFINITY, all_mass = 0.f;
-                    if (whole || c == 0) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) t = fmaxf(t, wm[i * ROWS + row]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) all_mass += t == -INFINITY ? wl[i * ROWS + row] : wl[i * ROWS + row] * ex2_approx(wm[i * ROWS + row] - t);
-                    }
-                    if (whole) {
-                        const bool real = is_draft(p, at.b, n);
-                        const float inv = real ? finish_scale(all_mass) : 0.f;
-                        const int64_t at_out = ((int64_t)at.b * p.N + n) * p.H + h;
-                        uint2 y = make_uint2(Frag<T>::pack(sum.x * inv, sum.y * inv), Frag<T>::pack(sum.z * inv, sum.w * inv));
-                        if (!real) y = make_uint2(0u, 0u);
-                        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + at_out * p.V + col) = y;
-                        if (p.lse && c == 0 && q == 0) p.lse[at_out] = real ? finish_lse(t, all_mass) : -INFINITY;
-                    } else {
-                        *reinterpret_cast<float4*>(slot + row * p.V + col) = sum;
-                        if (c == 0 && q == 0) *reinterpret_cast<float2*>(slot + ROWS * p.V + 2 * row) = make_float2(t, all_mass);
-                    }
-                }
-                __syncthreads();
-            }
-            first_piece = false;
-            fresh = true;
-        }
-        const int b = at.b;
-        at.next(p);
-        if (at.b != b) { bool d = false; draft_length(p, at.b, &d); bad |= d; }
     }
-    if (bad && p.status) atomicOr(p.status, HTREE_STATUS_CACHE);
 }
 
 // ---- joining the parts -------------------------------------------------------------------------------------------------------
 
-// Block (c, r) joins row r of the unit in which part c starts, if it is the first part that does.
+// By unit: a block a row, whose warps share the parts (few units, many parts each).  By part: a warp a row, of the unit that part c
+// starts and does not finish.
 constexpr int kJoinThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) draft_join_kernel(const __grid_constant__ DraftParams p) {
     __shared__ float red[kJoinThreads / 32][256];
     __shared__ float wm[kJoinThreads / 32], wl[kJoinThreads / 32];
     chain_enter();
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, r = blockIdx.y;
-    const int64_t c0 = blockIdx.x + 1;
-    Place at;
-    int64_t parts = 0, x0 = 0;
-    const int64_t all = find_place<kJoinThreads>(p, [&](int64_t n) {
-        parts = parts_of(p, n);
-        x0 = c0 < parts ? part_start(c0, n, parts) : 0;
-        return x0;
-    }, at);
-    if (c0 >= parts || at.tile == 0) return;                                 // (a part that starts with a unit)
-    const int64_t u0 = x0 - at.tile, u1 = u0 + at.tiles;
-    if (part_start(c0 - 1, all, parts) > u0) return;
-    int n, h;
-    if (!row_of(p, at.unit, r, n, h)) return;
-    // parts c0 - 1 .. last touch the unit; the first of them in its last slot, unless the unit is all that it has
-    int64_t last = c0;
-    while (last + 1 < parts && part_start(last + 1, all, parts) < u1) ++last;
-    const int64_t slots = last - c0 + 2, size = (int64_t)p.rows * (p.V + 2);
-    auto slot_of = [&](int64_t i) {
-        const int64_t c = c0 - 1 + i;
-        return p.part + (2 * c + (i == 0 && part_start(c, all, parts) < u0 ? 1 : 0)) * size;
-    };
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    const int4 task = p.tasks[blockIdx.x];
+    if (task.x < 0) return;
+    const int slots = task.w >> 1, by = p.by_unit ? kJoinThreads / 32 : 1;          // warps of a row
+    const int64_t size = (int64_t)p.rows * (p.V + 2);
+    const float* slot0 = p.part + 2 * (int64_t)task.z * size;
+    const int64_t in_first = (task.w & 1) ? size : 0;
+    auto slot_of = [&](int i) { return slot0 + (i == 0 ? in_first : 2 * i * size); };
+    const int r = p.by_unit ? blockIdx.y : blockIdx.y * (kJoinThreads / 32) + w;
+    int n = 0, h = 0;
+    const bool on = r < p.rows && row_of(p, task.y, r, n, h);
+    if (!on) return;                       // (by unit: the whole block)
+    const int i0 = p.by_unit ? w : 0;
     float top = -INFINITY;
-    for (int64_t i = tid; i < slots; i += kJoinThreads) top = fmaxf(top, slot_of(i)[p.rows * p.V + 2 * r]);
+    for (int i = lane; i < slots; i += 32) top = fmaxf(top, slot_of(i)[p.rows * p.V + 2 * r]);
     top = warp_max(top);
-    if (lane == 0) wm[w] = top;
-    __syncthreads();
-    top = wm[0];
-#pragma unroll
-    for (int i = 1; i < kJoinThreads / 32; ++i) top = fmaxf(top, wm[i]);
     const float ref = top == -INFINITY ? 0.f : top;
     float mass = 0.f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};                       // columns lane*4 and lane*4 + 128
-    for (int64_t i = w; i < slots; i += kJoinThreads / 32) {
+#pragma unroll 4
+    for (int i = i0; i < slots; i += by) {
         const float* s = slot_of(i);
-        const float f = exp2f(s[p.rows * p.V + 2 * r] - ref);
-        mass = fmaf(f, s[p.rows * p.V + 2 * r + 1], mass);
+        const float2 rm = *reinterpret_cast<const float2*>(s + p.rows * p.V + 2 * r);
+        float4 x[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+            x[half] = half * 128 + lane * 4 < p.V ? *reinterpret_cast<const float4*>(s + r * p.V + half * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float f = exp2f(rm.x - ref);
+        mass = fmaf(f, rm.y, mass);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const int col = half * 128 + lane * 4;
-            if (col < p.V) {
-                const float4 x = *reinterpret_cast<const float4*>(s + r * p.V + col);
-                o[4 * half] = fmaf(f, x.x, o[4 * half]);
-                o[4 * half + 1] = fmaf(f, x.y, o[4 * half + 1]);
-                o[4 * half + 2] = fmaf(f, x.z, o[4 * half + 2]);
-                o[4 * half + 3] = fmaf(f, x.w, o[4 * half + 3]);
-            }
+            o[4 * half] = fmaf(f, x[half].x, o[4 * half]);
+            o[4 * half + 1] = fmaf(f, x[half].y, o[4 * half + 1]);
+            o[4 * half + 2] = fmaf(f, x[half].z, o[4 * half + 2]);
+            o[4 * half + 3] = fmaf(f, x[half].w, o[4 * half + 3]);
         }
+    }
+    const bool real = is_draft(p, task.x, n);
+    const int64_t row = ((int64_t)task.x * p.N + n) * p.H + h;
+    if (!p.by_unit) {
+        const float inv = finish_scale(mass);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int col = (i >> 2) * 128 + lane * 4 + (i & 3);
+            if (col < p.V) reinterpret_cast<T*>(p.out)[row * p.V + col] = from_f<T>(real ? o[i] * inv : 0.f);
+        }
+        if (p.lse && lane == 0) p.lse[row] = real ? finish_lse(top, mass) : -INFINITY;
+        return;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) red[w][(i >> 2) * 128 + lane * 4 + (i & 3)] = o[i];
@@ -797,9 +929,7 @@ __global__ void __launch_bounds__(kJoinThreads) draft_join_kernel(const __grid_c
     mass = 0.f;
 #pragma unroll
     for (int i = 0; i < kJoinThreads / 32; ++i) mass += wl[i];
-    const bool real = is_draft(p, at.b, n);
     const float inv = finish_scale(mass);
-    const int64_t row = ((int64_t)at.b * p.N + n) * p.H + h;
     if (tid < p.V) {
         float x = 0.f;
 #pragma unroll
@@ -816,37 +946,47 @@ static size_t generic_smem(const DraftParams& p) {
     return ((size_t)kTile * (p.K + 4) + (size_t)kTile * VS + (size_t)kGenRows * p.K + (size_t)kGenRows * kTile) * 4;
 }
 
-static void fit_rows(DraftParams& p, int rows, int blocks) {
+static int64_t units_of(const DraftParams& p) { return (int64_t)p.B * p.Hkv * p.row_tiles; }
+
+// least: tiles that a part has at least (a block's warps, each of which takes one at a time).
+static void fit(DraftParams& p, int rows, int tile, int blocks, int least) {
     p.rows = rows;
     p.row_tiles = (p.N * p.G + rows - 1) / rows;
+    p.per_head = FastDiv((uint32_t)p.row_tiles);
+    p.shift = tile == 16 ? 4 : tile == 64 ? 6 : 7;
+    p.draft_tiles = (p.N + tile - 1) / tile;
     p.grid = blocks;
+    p.least = least;
+    p.by_unit = units_of(p) <= p.grid;
 }
+static int64_t part_bytes(const DraftParams& p) { return (int64_t)p.grid * 2 * p.rows * (p.V + 2) * 4; }
+static int64_t workspace_of(const DraftParams& p) { return part_bytes(p) + p.grid * 16; }           // tasks: per unit or per part, never more than parts
 
-// Which kernel: 16-bit rows of up to 128 go to the tensor cores, with as many rows to a block as there are (16, 32 or 64).
-enum { kGeneric = 0, kMma16, kMma32, kMma64 };
+// Which kernel: 16-bit rows of up to 128 go to the tensor cores.
+enum { kGeneric = 0, kMma16, kMma32 };
 static void choose(DraftParams& p, int dtype) {
     const int sms = sm_count() > 0 ? sm_count() : 148, rows = p.N * p.G;
     if (dtype == HTREE_F32 || p.K > 128 || p.V > 128) {
         p.variant = kGeneric;
-        fit_rows(p, kGenRows, sms * (generic_smem(p) <= 110 * 1024 ? 2 : 1));
+        fit(p, kGenRows, kTile, sms * (generic_smem(p) <= 110 * 1024 ? 2 : 1), 1);
         return;
     }
-    p.variant = rows <= 16 ? kMma16 : rows <= 32 ? kMma32 : kMma64;
-    fit_rows(p, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, rows <= 16 ? 2 * sms : sms);
+    p.variant = rows <= 16 ? kMma16 : kMma32;
+    fit(p, rows <= 16 ? 16 : 32, kSlice, sms, rows <= 16 ? 12 : 8);
     if (p.c < 0.f) { p.neg = 1; p.c = -p.c; }
     if (p.c < 1.1754944e-38f) p.c = 1.1754944e-38f;        // a scale of zero: scores of zero, but what is masked stays minus infinity
 }
 
-template <typename T, int DK, int DV, int WR, int RM>
+template <typename T, int DK, int DV, int RM>
 static int launch_mma(const DraftParams& p, cudaStream_t st) {
     static SmemLimit limit;
-    constexpr size_t smem = MmaSmem<T, DK, DV, WR, RM>::total;
-    if (const cudaError_t e = limit.raise((const void*)draft_mma_kernel<T, DK, DV, WR, RM>, smem)) return (int)e;
-    return launch_chained(draft_mma_kernel<T, DK, DV, WR, RM>, dim3(p.grid), dim3(WR * 128), smem, st, p);
+    using S = MmaShape<DK, DV, RM>;
+    if (const cudaError_t e = limit.raise((const void*)draft_mma_kernel<T, DK, DV, RM>, S::total)) return (int)e;
+    return launch_chained(draft_mma_kernel<T, DK, DV, RM>, dim3(p.grid), dim3(S::threads), S::total, st, p);
 }
 template <typename T, int DK, int DV>
 static int launch_mma(const DraftParams& p, cudaStream_t st) {
-    return p.variant == kMma16 ? launch_mma<T, DK, DV, 1, 1>(p, st) : p.variant == kMma32 ? launch_mma<T, DK, DV, 2, 1>(p, st) : launch_mma<T, DK, DV, 2, 2>(p, st);
+    return p.variant == kMma16 ? launch_mma<T, DK, DV, 1>(p, st) : launch_mma<T, DK, DV, 2>(p, st);
 }
 
 template <typename T>
@@ -871,8 +1011,9 @@ static int launch_draft(const DraftParams& p, cudaStream_t st) {
            : p.K <= 64 ? (p.V <= 64 ? launch_mma<T, 64, 64>(p, st) : launch_mma<T, 64, 128>(p, st))
                        : (p.V <= 64 ? launch_mma<T, 128, 64>(p, st) : launch_mma<T, 128, 128>(p, st));
     }
-    if (rc || p.grid == 1) return rc;
-    return launch_chained(draft_join_kernel<T>, dim3(p.grid - 1, p.rows), dim3(kJoinThreads), 0, st, p);
+    if (rc) return rc;
+    const dim3 grid = p.by_unit ? dim3((unsigned)units_of(p), p.N * p.G < p.rows ? p.N * p.G : p.rows) : dim3(p.grid, (p.rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
+    return launch_chained(draft_join_kernel<T>, grid, dim3(kJoinThreads), 0, st, p);
 }
 
 static int fill_draft(DraftParams& p, const HtreeCache* c, const HtreeDrafts* d) {
@@ -893,7 +1034,9 @@ static int fill_draft(DraftParams& p, const HtreeCache* c, const HtreeDrafts* d)
     p.cv_page = c->v_page * es; p.cv_row = c->v_row * es; p.cv_h = c->v_head * es;
     p.table_stride = d->table_stride;
     p.B = d->B; p.N = d->N; p.H = d->H; p.Hkv = c->H_kv; p.G = d->H / c->H_kv; p.K = c->K; p.V = c->V; p.M = d->M; p.pages = c->pages;
-    p.draft_tiles = (d->N + kTile - 1) / kTile;
+    const int64_t room = (int64_t)d->M * c->page_size;
+    p.room = (int32_t)(room < kMaxLength ? room : kMaxLength);
+    if ((int64_t)d->B * ((p.room + kSlice - 1) / kSlice + (d->N + kSlice - 1) / kSlice) >= (int64_t(1) << 31)) return HTREE_E_UNSUPPORTED;
     p.c = d->scale * kLog2e;
     p.page = FastDiv((uint32_t)c->page_size);
     p.group = FastDiv((uint32_t)p.G);
@@ -910,7 +1053,7 @@ extern "C" {
 int64_t htree_b200_draft_workspace(const HtreeCache* cache, const HtreeDrafts* drafts) {
     DraftParams p;
     if (const int rc = fill_draft(p, cache, drafts)) return rc;
-    return (int64_t)p.grid * 2 * p.rows * (p.V + 2) * 4;
+    return workspace_of(p);
 }
 
 int htree_b200_draft_attention(const HtreeCache* cache, const HtreeDrafts* drafts, void* workspace, int64_t workspace_bytes,
@@ -922,8 +1065,9 @@ int htree_b200_draft_attention(const HtreeCache* cache, const HtreeDrafts* draft
     if (!cache_aligned(p.q) || !cache_aligned(p.k) || !cache_aligned(p.v) || !cache_aligned(p.out) || !cache_aligned(workspace) ||
         !cache_strides_ok(drafts->q_stride, es) || !cache_strides_ok(drafts->k_stride, es) || !cache_strides_ok(drafts->v_stride, es))
         return HTREE_E_ALIGN;
-    if (workspace_bytes < (int64_t)p.grid * 2 * p.rows * (p.V + 2) * 4) return HTREE_E_SCRATCH;
+    if (workspace_bytes < workspace_of(p)) return HTREE_E_SCRATCH;
     p.part = (float*)workspace;
+    p.tasks = (int4*)((char*)workspace + part_bytes(p));
     p.status = status;
     const cudaStream_t st = (cudaStream_t)stream;
     return cache->dtype == HTREE_F32 ? launch_draft<float>(p, st)
