@@ -864,6 +864,463 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
     }
 }
 
+// ---- 16-bit types, more than 32 query rows: tcgen05 -----------------------------------------------------------------------------------
+
+// 128 or 256 query rows a block against tiles of 128 keys, which come from HBM once for all of them.  Per tile and half (128 rows, the
+// lanes of tensor memory): S = Q K^T (operands in shared memory, accumulator in tensor memory), P = 2^(cS - reference) by one thread a row,
+// written over S in 16 bits, O += P V with P read from tensor memory.  The two halves take turns: while one's softmax runs, the other's
+// products do.  Tensor memory: S and O of each half, 128 columns each; shared memory: Q (64 KB), two stages each of K and V (32 KB).
+// Roles: warps 0-3 and 4-7 the softmax of a half, 8 the products, 9-11 the copies.
+// At 256 rows of 128 a tile is 16.8 MFLOP, 2048 cycles of the tensor pipe, and 32768 exponentials, 2048 cycles of the special function
+// units: the two bound it alike, HBM (64 KB a tile) does below about 250 rows.
+constexpr int kTcTile = 128, kTcThreads = 384, kTcProducers = 3;
+constexpr int kTcWaitCap = 1 << 20;
+
+__device__ __forceinline__ uint32_t tc_idesc(bool bf16, bool negate, bool v_major, int n) {
+    // fp32 accumulator; A and B f16 (0) or bf16 (1); A negated; B with N (1) or K (0) contiguous; N / 8; M = 128
+    const uint32_t type = bf16 ? 1u : 0u;
+    return 1u << 4 | type << 7 | type << 10 | (negate ? 1u : 0u) << 13 | (v_major ? 1u : 0u) << 16 | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+}
+// Rows of 128 bytes, 128-byte swizzle: `lead` is the distance of 64-element blocks along a contiguous N, 8 rows are 1024 bytes.
+__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lead) {
+    return (uint64_t)(addr >> 4 & 0x3fffu) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, 1, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc) : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+#define TC_R8(x, i) "=r"((x)[i]), "=r"((x)[i + 1]), "=r"((x)[i + 2]), "=r"((x)[i + 3]), "=r"((x)[i + 4]), "=r"((x)[i + 5]), "=r"((x)[i + 6]), "=r"((x)[i + 7])
+#define TC_U8(x, i) "+r"((x)[i]), "+r"((x)[i + 1]), "+r"((x)[i + 2]), "+r"((x)[i + 3]), "+r"((x)[i + 4]), "+r"((x)[i + 5]), "+r"((x)[i + 6]), "+r"((x)[i + 7])
+#define TC_W8(x, i) "r"((x)[i]), "r"((x)[i + 1]), "r"((x)[i + 2]), "r"((x)[i + 3]), "r"((x)[i + 4]), "r"((x)[i + 5]), "r"((x)[i + 6]), "r"((x)[i + 7])
+// 32 columns of this warp's 32 lanes, a lane a thread; not to be read before tc_wait_ld
+__device__ __forceinline__ void tc_ld32(uint32_t (&x)[32], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+                 "%29,%30,%31}, [%32];\n"
+                 : TC_R8(x, 0), TC_R8(x, 8), TC_R8(x, 16), TC_R8(x, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&x)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" : TC_U8(x, 0), TC_U8(x, 8), TC_U8(x, 16), TC_U8(x, 24)::"memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* x) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+                 "%29,%30,%31,%32};\n" ::"r"(addr), TC_W8(x, 0), TC_W8(x, 8), TC_W8(x, 16), TC_W8(x, 24) : "memory");
+}
+
+template <int DK, int DV> struct TcShape {
+    static constexpr int kst = kTcTile * DK * 2, vst = kTcTile * DV * 2, qhalf = 128 * DK * 2;
+    static constexpr int stages = DK + DV > 192 ? 2 : 3;
+    static constexpr int q = 0, k = 2 * qhalf, v = k + stages * kst, end = v + stages * vst;
+    static constexpr int bars = end, valid = bars + 256, spoilt = valid + 4 * 16, slot = spoilt + 8 * 16, total = slot + 16 + 1024;
+};
+// mbarriers
+enum { kQFull = 0, kQEmpty, kSFull, kPReady = kSFull + 2, kOFull = kPReady + 2, kKFull = kOFull + 2, kKEmpty = kKFull + 3, kVFull = kKEmpty + 3, kVEmpty = kVFull + 3, kTcBars = kVEmpty + 3 };
+static_assert(kTcBars * 8 <= 256, "");
+
+template <typename T, int DK, int DV>
+__global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_constant__ DraftParams p) {
+    using S = TcShape<DK, DV>;
+    constexpr int ST = S::stages;
+    constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ unsigned char sm_raw[];
+    unsigned char* sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::bars);
+    uint32_t* valid = reinterpret_cast<uint32_t*>(sm + S::valid);            // [4][4]: which keys a tile has
+    uint32_t* spoilt = reinterpret_cast<uint32_t*>(sm + S::spoilt);          // [8][4]: drafts with values that are not finite
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + S::slot);
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    if (tid == 0) {
+        mbar_init(bars + kQFull, kTcProducers); mbar_init(bars + kQEmpty, 1);
+        for (int i = 0; i < 2; ++i) { mbar_init(bars + kSFull + i, 1); mbar_init(bars + kPReady + i, 128); mbar_init(bars + kOFull + i, 1); }
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(bars + kKFull + i, kTcProducers); mbar_init(bars + kKEmpty + i, 1);
+            mbar_init(bars + kVFull + i, kTcProducers); mbar_init(bars + kVEmpty + i, 1);
+        }
+        fence_barrier_init();
+    }
+    if (tid < 32) spoilt[tid] = 0;
+    chain_enter();
+    Place at;
+    Line line;
+    int64_t x0, x1;
+    if (tid == 0 && !p.by_unit) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (!find_part<kTcThreads>(p, at, line, x0, x1)) return;
+    const int n_tiles = (int)(x1 - x0);
+    if (w == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;                     // columns: S of half 0, S of half 1, O of half 0, O of half 1
+    bool bad = false, late = false;
+    auto wait = [&](int bar, uint32_t parity) {
+        if (!late && !mbar_wait_bounded(bars + bar, parity, kTcWaitCap)) late = true;      // (then nothing is waited for any more: wrong numbers, reported, no hang)
+    };
+    auto two_halves = [&](const Place& pl) { return p.N * p.G - (pl.unit - head_of(p, pl.unit) * p.row_tiles) * p.rows > 128 && p.rows > 128; };
+
+    if (w >= 9) {
+        // ---- copies
+        constexpr int KL = DK / 8, VL = DV / 8;
+        const uint32_t base = smem_u32(sm);
+        int g = 0, unit_no = 0;
+        int done = 0;
+        // where lane's piece of row r goes within a 128-row operand: 64 columns to a block of 128-byte rows, 16-byte pieces swizzled by the row
+        auto place_of = [&](int r, int c) { return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
+        // what this warp has copied is there, and the products may read it
+        auto tell = [&](int bar) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bars + bar)) : "memory");
+        };
+        auto tell_v = [&](int g_, bool draft) {
+            if (draft) {
+                const uint32_t dst = base + S::v + g_ % ST * S::vst;
+#pragma unroll 1
+                for (int sl = w - 9; sl < 8; sl += kTcProducers)
+#pragma unroll 1
+                    for (int r = 0; r < 16; r += 32 / VL) {
+                        const int x = sl * 16 + r + lane / VL;
+                        if (take_out<T>(dst + place_of(x, lane % VL))) atomicOr(&spoilt[(g_ & 7) * 4 + (x >> 5)], 1u << (x & 31));
+                    }
+            }
+            tell(kVFull + g_ % ST);
+        };
+        while (done < n_tiles) {
+            const int piece = min(n_tiles - done, at.tiles - at.tile), cached = at.tiles - p.draft_tiles, kv = head_of(p, at.unit);
+            { bool b = false; draft_length(p, at.b, &b); bad |= b; }
+            wait(kQEmpty, (unit_no & 1) ^ 1);
+            const int halves = two_halves(at) ? 2 : 1;
+#pragma unroll 1
+            for (int r0 = (w - 9) * (32 / KL); r0 < halves * 128; r0 += kTcProducers * (32 / KL)) {
+                const int r = r0 + lane / KL, c = lane % KL;
+                int n, h;
+                const bool on = row_of(p, at.unit, r, n, h) && c * 8 < p.K;
+                if (r < halves * 128)
+                    cp_async16_or_zero(base + S::q + (r >> 7) * S::qhalf + place_of(r & 127, c), on ? p.q + at.b * p.q_b + n * p.q_n + h * p.q_h + c * 16 : p.q, on);
+            }
+            cp_async_commit();
+            for (int j = 0; j < piece; ++j, ++g) {
+                const int tile = at.tile + j, st = g % ST;
+                const uint32_t ph = (uint32_t)(g / ST) & 1u;
+                // the rows of this warp's slices of sixteen keys: lane x (and x + 16) knows key x
+                const char *kr[3], *vr[3];
+                uint32_t m[3];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    const int sl = w - 9 + i * kTcProducers;
+                    kr[i] = vr[i] = p.q;
+                    bool on = false;
+                    if (sl < 8) {
+                        const char *k = p.q, *v = p.q;
+                        on = key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, sl * 16 + (lane & 15), k, v, &bad);
+                        kr[i] = k; vr[i] = v;
+                    }
+                    m[i] = __ballot_sync(0xffffffffu, on) & 0xffffu;
+                }
+                auto copy = [&](const char* const (&row)[3], uint32_t dst, int lanes, int width) {
+                    // lanes: 16-byte pieces of a row; 32 / lanes rows at a time
+                    const int per = 32 / lanes, c = lane % lanes;
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) {
+                        const int sl = w - 9 + i * kTcProducers;
+                        if (sl >= 8) break;
+#pragma unroll 2
+                        for (int r = 0; r < 16; r += per) {
+                            const int x = r + lane / lanes;
+                            const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row[i]), x));
+                            const bool on = (m[i] >> x & 1) && c * 8 < width;
+                            cp_async16_or_zero(dst + place_of(sl * 16 + x, c), on ? src + c * 16 : p.q, on);
+                        }
+                    }
+                };
+                wait(kKEmpty + st, ph ^ 1);
+                if (lane == 0)
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) {
+                        const int sl = w - 9 + i * kTcProducers;
+                        if (sl < 8) reinterpret_cast<uint16_t*>(valid + (g & 3) * 4)[sl] = (uint16_t)m[i];
+                    }
+                copy(kr, base + S::k + st * S::kst, KL, p.K);
+                cp_async_commit();
+                if (j == 0) {
+                    cp_async_wait<1>();
+                    tell(kQFull);
+                }
+                if (j > 0) {
+                    cp_async_wait<1>();
+                    tell_v(g - 1, tile - 1 >= cached);
+                }
+                wait(kVEmpty + st, ph ^ 1);
+                if (w == 9 && lane < 4) spoilt[((g - ST) & 7) * 4 + lane] = 0;
+                copy(vr, base + S::v + st * S::vst, VL, p.V);
+                cp_async_commit();
+                cp_async_wait<1>();
+                tell(kKFull + st);
+            }
+            cp_async_wait<0>();
+            tell_v(g - 1, at.tile + piece - 1 >= cached);
+            done += piece;
+            ++unit_no;
+            at.tile += piece - 1;
+            at.next(p);
+        }
+    } else if (w == 8) {
+        // ---- products
+        if (lane == 0) {
+            const uint32_t base = smem_u32(sm), iqk = tc_idesc(BF, p.neg, false, kTcTile), ipv = tc_idesc(BF, false, true, DV);
+            auto qk = [&](int half, int st) {
+                const uint32_t a = base + S::q + half * S::qhalf, b = base + S::k + st * S::kst;
+#pragma unroll
+                for (int ks = 0; ks < DK / 16; ++ks) {
+                    const uint32_t off = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
+                    tc_mma_ss(tmem + half * 128, tc_desc(a + off, 16), tc_desc(b + off, 16), iqk, ks > 0);
+                }
+            };
+            auto pv = [&](int half, int st) {
+                const uint32_t b = base + S::v + st * S::vst;
+#pragma unroll
+                for (int ks = 0; ks < kTcTile / 16; ++ks) tc_mma_ts(tmem + 256 + half * 128, tmem + half * 128 + ks * 8, tc_desc(b + ks * 2048, 128 * 128), ipv);
+            };
+            int g = 0, unit_no = 0, done = 0;
+            uint32_t pa = 0, pb = 0;                      // tiles whose P a half has had
+            while (done < n_tiles) {
+                const int piece = min(n_tiles - done, at.tiles - at.tile);
+                const bool two = two_halves(at);
+                wait(kQFull, unit_no & 1);
+                wait(kKFull + g % ST, (uint32_t)(g / ST) & 1u);
+                tc_fence_after();
+                qk(0, g % ST);
+                tc_commit(bars + kSFull);
+                if (two) {
+                    qk(1, g % ST);
+                    tc_commit(bars + kSFull + 1);
+                }
+                tc_commit(bars + kKEmpty + g % ST);
+                for (int j = 0; j < piece; ++j, ++g) {
+                    const int st = g % ST, nx = (g + 1) % ST;
+                    const bool more = j + 1 < piece;
+                    wait(kVFull + st, (uint32_t)(g / ST) & 1u);
+                    wait(kPReady, pa++ & 1u);
+                    tc_fence_after();
+                    pv(0, st);
+                    if (!more) tc_commit(bars + kOFull);
+                    if (more) {
+                        wait(kKFull + nx, (uint32_t)((g + 1) / ST) & 1u);
+                        tc_fence_after();
+                        qk(0, nx);
+                        tc_commit(bars + kSFull);
+                    }
+                    if (two) {
+                        wait(kPReady + 1, pb++ & 1u);
+                        tc_fence_after();
+                        pv(1, st);
+                        if (!more) tc_commit(bars + kOFull + 1);
+                    }
+                    tc_commit(bars + kVEmpty + st);
+                    if (more) {
+                        if (two) {
+                            qk(1, nx);
+                            tc_commit(bars + kSFull + 1);
+                        }
+                        tc_commit(bars + kKEmpty + nx);
+                    }
+                }
+                tc_commit(bars + kQEmpty);
+                done += piece;
+                ++unit_no;
+                at.tile += piece - 1;
+                at.next(p);
+            }
+            wait(kQEmpty, (unit_no - 1) & 1);             // all products are done
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: a thread a row
+        const int half = w >> 2, row = half * 128 + (w & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)(w & 3) << 21;   // lane 32 * (w & 3) of tensor memory
+        const uint32_t ts = tmem + lanes + half * 128, to = tmem + lanes + 256 + half * 128;
+        int g = 0, done = 0;
+        uint32_t turns = 0, units_had = 0;
+        bool first_piece = true;
+        while (done < n_tiles) {
+            const int piece = min(n_tiles - done, at.tiles - at.tile), cached = at.tiles - p.draft_tiles;
+            const bool whole = at.tile == 0 && piece == at.tiles;
+            if (tid == 0 && at.tile == 0) leave_task(p, at, x0 + done, x0, blockIdx.x, line, whole);
+            if (half == 0 || two_halves(at)) {
+                int n, h;
+                const bool on = row_of(p, at.unit, row, n, h);
+                uint32_t x[2][32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[0][i] = 0;
+#pragma unroll
+                for (int c = 0; c < DV / 32; ++c) tc_st32(to + c * 32, x[0]);
+                float ref = -INFINITY, mass = 0.f;
+                for (int j = 0; j < piece; ++j) {
+                    const int tile = at.tile + j, gg = g + j;
+                    const bool draft = tile >= cached;
+                    wait(kSFull + half, turns++ & 1u);
+                    tc_fence_after();
+                    uint32_t seen[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) seen[i] = valid[(gg & 3) * 4 + i];
+                    if (draft) {
+                        const int tile0 = (tile - cached) * kTcTile;
+                        const uint64_t lo = on ? draft_mask(p, at.b, n, tile0, &bad) : 0ull, hi = on ? draft_mask(p, at.b, n, tile0 + 64, &bad) : 0ull;
+                        seen[0] &= (uint32_t)lo; seen[1] &= (uint32_t)(lo >> 32); seen[2] &= (uint32_t)hi; seen[3] &= (uint32_t)(hi >> 32);
+                        wait(kVFull + gg % ST, (uint32_t)(gg / ST) & 1u);
+                        uint32_t sp[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sp[i] = spoilt[(gg & 7) * 4 + i];
+                        if (sp[0] | sp[1] | sp[2] | sp[3]) {
+                            tc_wait_st();
+                            const char* v0 = p.v + at.b * p.v_b + head_of(p, at.unit) * p.v_h;
+#pragma unroll 1
+                            for (int key = 0; key < kTcTile; ++key) {
+                                const uint32_t word = key < 32 ? sp[0] : key < 64 ? sp[1] : key < 96 ? sp[2] : sp[3];
+                                if (!(word >> (key & 31) & 1)) continue;
+                                const uint32_t mine = key < 32 ? seen[0] : key < 64 ? seen[1] : key < 96 ? seen[2] : seen[3];
+#pragma unroll 1
+                                for (int c = 0; c < DV; c += 32) {
+                                    tc_ld32(x[0], to + c);
+                                    tc_wait_ld(x[0]);
+                                    if (mine >> (key & 31) & 1)
+#pragma unroll
+                                        for (int i = 0; i < 32; ++i)
+                                            if (c + i < p.V) x[0][i] = __float_as_uint(put_back<T>(__uint_as_float(x[0][i]), v0 + (int64_t)(tile0 + key) * p.v_n, c + i));
+                                    tc_st32(to + c, x[0]);
+                                    tc_wait_st();
+                                }
+                            }
+                        }
+                    }
+                    const bool gaps = (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu;
+                    const bool masked = __any_sync(0xffffffffu, gaps);
+                    uint32_t pk[64];
+                    float top = -INFINITY, sum = 0.f;
+                    // One pass: P with the present reference, and the row's maximum; if that is further above the reference than P may grow,
+                    // (for the first tile always) the reference moves, the sums with it, and P is made again.
+                    bool again = j == 0;
+                    for (int pass = again ? 1 : 0;; ++pass) {
+                        const float base = ref == -INFINITY ? 0.f : -ref;
+                        sum = 0.f;
+                        const bool only_max = again && pass == 1;
+                        tc_ld32(x[0], ts);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t(&y)[32] = x[c & 1];
+                            tc_wait_ld(y);
+                            if (c < 3) tc_ld32(x[(c + 1) & 1], ts + (c + 1) * 32);
+                            if (masked)
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) y[i] = (seen[c] >> i & 1) ? y[i] : 0xff800000u;
+                            if (pass < 2) {
+                                float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                                for (int i = 0; i < 32; i += 4) {
+                                    t0 = fmaxf(t0, fmaxf(__uint_as_float(y[i]), __uint_as_float(y[i + 1])));
+                                    t1 = fmaxf(t1, fmaxf(__uint_as_float(y[i + 2]), __uint_as_float(y[i + 3])));
+                                }
+                                top = fmaxf(top, fmaxf(t0, t1));
+                            }
+                            if (!only_max) {
+                                float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                                for (int i = 0; i < 32; i += 2) {
+                                    const float e0 = ex2_approx(fmaf(__uint_as_float(y[i]), p.c, base)), e1 = ex2_approx(fmaf(__uint_as_float(y[i + 1]), p.c, base));
+                                    s0 += e0;
+                                    s1 += e1;
+                                    pk[c * 16 + (i >> 1)] = Frag<T>::pack(e0, e1);
+                                }
+                                sum += s0 + s1;
+                            }
+                        }
+                        if (pass >= 2) break;
+                        const float t = top * p.c;
+                        if (!only_max && !__any_sync(0xffffffffu, t > ref + (kLag<T> + kBias<T>))) break;
+                        const float now = fmaxf(ref, t - kBias<T>);
+                        const float keep = now == -INFINITY ? 1.f : ex2_approx(ref - now);
+                        ref = now;
+                        mass *= keep;
+                        if (j > 0) {
+#pragma unroll 1
+                            for (int c = 0; c < DV; c += 32) {
+                                tc_ld32(x[0], to + c);
+                                tc_wait_ld(x[0]);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) x[0][i] = __float_as_uint(__uint_as_float(x[0][i]) * keep);
+                                tc_st32(to + c, x[0]);
+                            }
+                        }
+                        pass = 1;
+                    }
+                    mass += sum;
+                    tc_st32(ts, pk);
+                    tc_st32(ts + 32, pk + 32);
+                    tc_wait_st();
+                    tc_fence_before();
+                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bars + kPReady + half)) : "memory");
+                }
+                wait(kOFull + half, units_had++ & 1u);
+                tc_fence_after();
+                const bool real = on && is_draft(p, at.b, n);
+                const float f = whole ? (real ? finish_scale(mass) : 0.f) : 1.f;
+                const int64_t at_out = ((int64_t)at.b * p.N + n) * p.H + h;
+                float* slot = p.part + (int64_t)(2 * blockIdx.x + (first_piece ? 0 : 1)) * p.rows * (p.V + 2);
+#pragma unroll 1
+                for (int c = 0; c < DV; c += 32) {
+                    tc_ld32(x[0], to + c);
+                    tc_wait_ld(x[0]);
+                    if (!on) continue;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        if (c + i >= p.V) break;
+                        float o[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(x[0][i + e]) * f;
+                        if (whole) {
+                            uint4 y = make_uint4(Frag<T>::pack(o[0], o[1]), Frag<T>::pack(o[2], o[3]), Frag<T>::pack(o[4], o[5]), Frag<T>::pack(o[6], o[7]));
+                            if (!real) y = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + at_out * p.V + c + i) = y;
+                        } else {
+                            *reinterpret_cast<float4*>(slot + row * p.V + c + i) = make_float4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<float4*>(slot + row * p.V + c + i + 4) = make_float4(o[4], o[5], o[6], o[7]);
+                        }
+                    }
+                }
+                if (on) {
+                    if (!whole) *reinterpret_cast<float2*>(slot + p.rows * p.V + 2 * row) = make_float2(ref, mass);
+                    else if (p.lse) p.lse[at_out] = real ? finish_lse(ref, mass) : -INFINITY;
+                }
+            }
+            g += piece;
+            first_piece = false;
+            done += piece;
+            at.tile += piece - 1;
+            at.next(p);
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (w == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+    }
+    if (p.status) {
+        if (bad) atomicOr(p.status, HTREE_STATUS_CACHE);
+        if (late) atomicOr(p.status, 16);
+    }
+}
+
 // ---- joining the parts -------------------------------------------------------------------------------------------------------
 
 // By unit: a block a row, whose warps share the parts (few units, many parts each).  By part: a warp a row, of the unit that part c
@@ -963,7 +1420,7 @@ static int64_t part_bytes(const DraftParams& p) { return (int64_t)p.grid * 2 * p
 static int64_t workspace_of(const DraftParams& p) { return part_bytes(p) + p.grid * 16; }           // tasks: per unit or per part, never more than parts
 
 // Which kernel: 16-bit rows of up to 128 go to the tensor cores.
-enum { kGeneric = 0, kMma16, kMma32 };
+enum { kGeneric = 0, kMma16, kMma32, kTc };
 static void choose(DraftParams& p, int dtype) {
     const int sms = sm_count() > 0 ? sm_count() : 148, rows = p.N * p.G;
     if (dtype == HTREE_F32 || p.K > 128 || p.V > 128) {
@@ -971,8 +1428,9 @@ static void choose(DraftParams& p, int dtype) {
         fit(p, kGenRows, kTile, sms * (generic_smem(p) <= 110 * 1024 ? 2 : 1), 1);
         return;
     }
-    p.variant = rows <= 16 ? kMma16 : kMma32;
-    fit(p, rows <= 16 ? 16 : 32, kSlice, sms, rows <= 16 ? 12 : 8);
+    p.variant = rows <= 16 ? kMma16 : rows <= 32 ? kMma32 : kTc;
+    if (p.variant == kTc) fit(p, rows <= 128 ? 128 : 256, kTcTile, sms, 1);
+    else fit(p, rows <= 16 ? 16 : 32, kSlice, sms, rows <= 16 ? 12 : 8);
     if (p.c < 0.f) { p.neg = 1; p.c = -p.c; }
     if (p.c < 1.1754944e-38f) p.c = 1.1754944e-38f;        // a scale of zero: scores of zero, but what is masked stays minus infinity
 }
@@ -986,6 +1444,11 @@ static int launch_mma(const DraftParams& p, cudaStream_t st) {
 }
 template <typename T, int DK, int DV>
 static int launch_mma(const DraftParams& p, cudaStream_t st) {
+    if (p.variant == kTc) {
+        static SmemLimit limit;
+        if (const cudaError_t e = limit.raise((const void*)draft_tc_kernel<T, DK, DV>, TcShape<DK, DV>::total)) return (int)e;
+        return launch_chained(draft_tc_kernel<T, DK, DV>, dim3(p.grid), dim3(kTcThreads), TcShape<DK, DV>::total, st, p);
+    }
     return p.variant == kMma16 ? launch_mma<T, DK, DV, 1>(p, st) : launch_mma<T, DK, DV, 2>(p, st);
 }
 
