@@ -8,6 +8,8 @@
 #include "cache.cuh"
 #include "mma_common.cuh"
 
+#include <cuda.h>
+
 namespace htree {
 
 constexpr int kMaxTree = 1024;
@@ -34,8 +36,9 @@ struct DraftParams {
     int32_t B, N, H, Hkv, G, K, V, M, pages;
     int32_t rows, row_tiles, shift, draft_tiles;                           // rows of a row tile, log2 of the keys of a tile
     int32_t room;             // tokens that a row of the table can name
-    int32_t grid, least, by_unit;                                          // parts at most; tiles of a part at least; how tasks are indexed
+    int32_t grid, least, by_unit, team;                                    // parts at most; tiles of a part at least; how tasks are indexed, and joined
     int32_t variant;          // which kernel (choose)
+    int32_t boxes;            // tcgen05 kernel: pages of whole slices of sixteen tokens come by the tensor maps
     int32_t neg;              // tensor-core kernels: the scale is negative, c its magnitude and q's signs are turned
     float c;                  // scale * log2 e
     FastDiv page, group, per_head;      // by the page size, by G, by row_tiles
@@ -915,6 +918,8 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* x) {
                  "%29,%30,%31,%32};\n" ::"r"(addr), TC_W8(x, 0), TC_W8(x, 8), TC_W8(x, 16), TC_W8(x, 24) : "memory");
 }
 
+struct TcMaps { CUtensorMap k, v; };       // the caches as [page][head][token][element], boxes of 16 tokens and 128 bytes
+
 template <int DK, int DV> struct TcShape {
     static constexpr int kst = kTcTile * DK * 2, vst = kTcTile * DV * 2, qhalf = 128 * DK * 2;
     static constexpr int stages = DK + DV > 192 ? 2 : 3;
@@ -926,7 +931,7 @@ enum { kQFull = 0, kQEmpty, kSFull, kPReady = kSFull + 2, kOFull = kPReady + 2, 
 static_assert(kTcBars * 8 <= 256, "");
 
 template <typename T, int DK, int DV>
-__global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_constant__ DraftParams p) {
+__global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_constant__ DraftParams p, const __grid_constant__ TcMaps maps) {
     using S = TcShape<DK, DV>;
     constexpr int ST = S::stages;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
@@ -976,25 +981,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
         int done = 0;
         // where lane's piece of row r goes within a 128-row operand: 64 columns to a block of 128-byte rows, 16-byte pieces swizzled by the row
         auto place_of = [&](int r, int c) { return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
-        // what this warp has copied is there, and the products may read it
-        auto tell = [&](int bar) {
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bars + bar)) : "memory");
-        };
-        auto tell_v = [&](int g_, bool draft) {
-            if (draft) {
-                const uint32_t dst = base + S::v + g_ % ST * S::vst;
-#pragma unroll 1
-                for (int sl = w - 9; sl < 8; sl += kTcProducers)
-#pragma unroll 1
-                    for (int r = 0; r < 16; r += 32 / VL) {
-                        const int x = sl * 16 + r + lane / VL;
-                        if (take_out<T>(dst + place_of(x, lane % VL))) atomicOr(&spoilt[(g_ & 7) * 4 + (x >> 5)], 1u << (x & 31));
-                    }
-            }
-            tell(kVFull + g_ % ST);
-        };
         while (done < n_tiles) {
             const int piece = min(n_tiles - done, at.tiles - at.tile), cached = at.tiles - p.draft_tiles, kv = head_of(p, at.unit);
             { bool b = false; draft_length(p, at.b, &b); bad |= b; }
@@ -1005,44 +991,86 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 const int r = r0 + lane / KL, c = lane % KL;
                 int n, h;
                 const bool on = row_of(p, at.unit, r, n, h) && c * 8 < p.K;
-                if (r < halves * 128)
-                    cp_async16_or_zero(base + S::q + (r >> 7) * S::qhalf + place_of(r & 127, c), on ? p.q + at.b * p.q_b + n * p.q_n + h * p.q_h + c * 16 : p.q, on);
+                cp_async16_or_zero(base + S::q + (r >> 7) * S::qhalf + place_of(r & 127, c), on ? p.q + at.b * p.q_b + n * p.q_n + h * p.q_h + c * 16 : p.q, on);
             }
             cp_async_commit();
             for (int j = 0; j < piece; ++j, ++g) {
                 const int tile = at.tile + j, st = g % ST;
                 const uint32_t ph = (uint32_t)(g / ST) & 1u;
-                // the rows of this warp's slices of sixteen keys: lane x (and x + 16) knows key x
+                // This warp's slices of sixteen keys, w - 9, w - 6, w - 3.  Sixteen cached tokens of one page are a box of the tensor maps; of
+                // others (a sequence's end, drafts, small pages) lane x (and x + 16) knows the row of key x.
                 const char *kr[3], *vr[3];
                 uint32_t m[3];
+                int page[3], in[3];
+                bool rows = false;
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    const int sl = w - 9 + i * kTcProducers, pos = tile * kTcTile + sl * 16;
+                    page[i] = -1;
+                    m[i] = 0;
+                    if (p.boxes && sl < 8 && tile < cached && pos + 16 <= at.len) {
+                        const int no = (int)p.page.div((uint32_t)pos);
+                        in[i] = pos - no * (int)p.page.d;
+                        page[i] = __ldg(p.table + (int64_t)at.b * p.table_stride + no);
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 3; ++i) {
                     const int sl = w - 9 + i * kTcProducers;
                     kr[i] = vr[i] = p.q;
-                    bool on = false;
-                    if (sl < 8) {
-                        const char *k = p.q, *v = p.q;
-                        on = key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, sl * 16 + (lane & 15), k, v, &bad);
-                        kr[i] = k; vr[i] = v;
-                    }
+                    if (page[i] >= 0 && page[i] < p.pages) { m[i] = 0xffffu; continue; }
+                    page[i] = -1;
+                    if (sl >= 8) continue;
+                    const char *k = p.q, *v = p.q;
+                    const bool on = key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, sl * 16 + (lane & 15), k, v, &bad);
+                    kr[i] = k; vr[i] = v;
                     m[i] = __ballot_sync(0xffffffffu, on) & 0xffffu;
+                    rows = true;
                 }
-                auto copy = [&](const char* const (&row)[3], uint32_t dst, int lanes, int width) {
-                    // lanes: 16-byte pieces of a row; 32 / lanes rows at a time
-                    const int per = 32 / lanes, c = lane % lanes;
+                auto copy = [&](const CUtensorMap& map, int full, int empty, const char* const (&row)[3], uint32_t dst, int lanes, int width, bool values) {
+                    wait(empty, ph ^ 1);
+                    uint32_t bytes = 0;
 #pragma unroll
                     for (int i = 0; i < 3; ++i) {
                         const int sl = w - 9 + i * kTcProducers;
-                        if (sl >= 8) break;
-#pragma unroll 2
-                        for (int r = 0; r < 16; r += per) {
-                            const int x = r + lane / lanes;
-                            const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row[i]), x));
-                            const bool on = (m[i] >> x & 1) && c * 8 < width;
-                            cp_async16_or_zero(dst + place_of(sl * 16 + x, c), on ? src + c * 16 : p.q, on);
-                        }
+                        if (page[i] < 0) continue;
+                        bytes += 16 * 16 * lanes;
+                        if (lane == 0)
+                            for (int blk = 0; blk < lanes / 8; ++blk)
+                                asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
+                                                 dst + blk * (128 * 128) + sl * 2048), "l"(&map), "r"(blk * 64), "r"(in[i]), "r"(kv), "r"(page[i]),
+                                             "r"(smem_u32(bars + full)) : "memory");
                     }
+                    if (rows) {
+                        const int per = 32 / lanes, c = lane % lanes;
+#pragma unroll
+                        for (int i = 0; i < 3; ++i) {
+                            const int sl = w - 9 + i * kTcProducers;
+                            if (sl >= 8 || page[i] >= 0) continue;
+#pragma unroll 2
+                            for (int r = 0; r < 16; r += per) {
+                                const int x = r + lane / lanes;
+                                const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row[i]), x));
+                                const bool on = (m[i] >> x & 1) && c * 8 < width;
+                                cp_async16_or_zero(dst + place_of(sl * 16 + x, c), on ? src + c * 16 : p.q, on);
+                            }
+                        }
+                        cp_async_commit();
+                        cp_async_wait<0>();
+                        if (values && tile >= cached)
+#pragma unroll 1
+                            for (int sl = w - 9; sl < 8; sl += kTcProducers)
+#pragma unroll 1
+                                for (int r = 0; r < 16; r += per) {
+                                    const int x = sl * 16 + r + lane / lanes;
+                                    if (take_out<T>(dst + place_of(x, c))) atomicOr(&spoilt[(g & 7) * 4 + (x >> 5)], 1u << (x & 31));
+                                }
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(bars + full, bytes);
                 };
+                // (the words of the tile four before are no longer read: its products are done, or this stage would not be empty)
                 wait(kKEmpty + st, ph ^ 1);
                 if (lane == 0)
 #pragma unroll
@@ -1050,25 +1078,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                         const int sl = w - 9 + i * kTcProducers;
                         if (sl < 8) reinterpret_cast<uint16_t*>(valid + (g & 3) * 4)[sl] = (uint16_t)m[i];
                     }
-                copy(kr, base + S::k + st * S::kst, KL, p.K);
-                cp_async_commit();
+                copy(maps.k, kKFull + st, kKEmpty + st, kr, base + S::k + st * S::kst, KL, p.K, false);
                 if (j == 0) {
-                    cp_async_wait<1>();
-                    tell(kQFull);
-                }
-                if (j > 0) {
-                    cp_async_wait<1>();
-                    tell_v(g - 1, tile - 1 >= cached);
+                    cp_async_wait<0>();
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bars + kQFull)) : "memory");
                 }
                 wait(kVEmpty + st, ph ^ 1);
                 if (w == 9 && lane < 4) spoilt[((g - ST) & 7) * 4 + lane] = 0;
-                copy(vr, base + S::v + st * S::vst, VL, p.V);
-                cp_async_commit();
-                cp_async_wait<1>();
-                tell(kKFull + st);
+                copy(maps.v, kVFull + st, kVEmpty + st, vr, base + S::v + st * S::vst, VL, p.V, true);
             }
-            cp_async_wait<0>();
-            tell_v(g - 1, at.tile + piece - 1 >= cached);
             done += piece;
             ++unit_no;
             at.tile += piece - 1;
@@ -1323,77 +1343,78 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
 
 // ---- joining the parts -------------------------------------------------------------------------------------------------------
 
-// By unit: a block a row, whose warps share the parts (few units, many parts each).  By part: a warp a row, of the unit that part c
-// starts and does not finish.
-constexpr int kJoinThreads = 256;
+// A task is the rows of a unit that several parts have left; by unit, or, where there are more units than parts, by the part that starts and
+// does not finish it.  A team of 1 to 8 warps joins a row (as many parts as a unit has on average, about four to a warp).
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) draft_join_kernel(const __grid_constant__ DraftParams p) {
-    __shared__ float red[kJoinThreads / 32][256];
-    __shared__ float wm[kJoinThreads / 32], wl[kJoinThreads / 32];
+    __shared__ float red[kJoinWarps][256], wl[kJoinWarps];
     chain_enter();
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, team = w / p.team, member = w - team * p.team;
     const int4 task = p.tasks[blockIdx.x];
     if (task.x < 0) return;
-    const int slots = task.w >> 1, by = p.by_unit ? kJoinThreads / 32 : 1;          // warps of a row
+    const int slots = task.w >> 1, r = blockIdx.y * (kJoinWarps / p.team) + team;
     const int64_t size = (int64_t)p.rows * (p.V + 2);
     const float* slot0 = p.part + 2 * (int64_t)task.z * size;
     const int64_t in_first = (task.w & 1) ? size : 0;
     auto slot_of = [&](int i) { return slot0 + (i == 0 ? in_first : 2 * i * size); };
-    const int r = p.by_unit ? blockIdx.y : blockIdx.y * (kJoinThreads / 32) + w;
     int n = 0, h = 0;
     const bool on = r < p.rows && row_of(p, task.y, r, n, h);
-    if (!on) return;                       // (by unit: the whole block)
-    const int i0 = p.by_unit ? w : 0;
-    float top = -INFINITY;
-    for (int i = lane; i < slots; i += 32) top = fmaxf(top, slot_of(i)[p.rows * p.V + 2 * r]);
-    top = warp_max(top);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float mass = 0.f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};                       // columns lane*4 and lane*4 + 128
+    float top = -INFINITY, mass = 0.f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};      // columns lane*4 and lane*4 + 128
+    if (on) {
+        for (int i = lane; i < slots; i += 32) top = fmaxf(top, slot_of(i)[p.rows * p.V + 2 * r]);
+        top = warp_max(top);
+        const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll 4
-    for (int i = i0; i < slots; i += by) {
-        const float* s = slot_of(i);
-        const float2 rm = *reinterpret_cast<const float2*>(s + p.rows * p.V + 2 * r);
-        float4 x[2];
+        for (int i = member; i < slots; i += p.team) {
+            const float* s = slot_of(i);
+            const float2 rm = *reinterpret_cast<const float2*>(s + p.rows * p.V + 2 * r);
+            float4 x[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                x[half] = half * 128 + lane * 4 < p.V ? *reinterpret_cast<const float4*>(s + r * p.V + half * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float f = exp2f(rm.x - ref);
+            mass = fmaf(f, rm.y, mass);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                o[4 * half] = fmaf(f, x[half].x, o[4 * half]);
+                o[4 * half + 1] = fmaf(f, x[half].y, o[4 * half + 1]);
+                o[4 * half + 2] = fmaf(f, x[half].z, o[4 * half + 2]);
+                o[4 * half + 3] = fmaf(f, x[half].w, o[4 * half + 3]);
+            }
+        }
+    }
+    if (p.team > 1) {
 #pragma unroll
         for (int half = 0; half < 2; ++half)
-            x[half] = half * 128 + lane * 4 < p.V ? *reinterpret_cast<const float4*>(s + r * p.V + half * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float f = exp2f(rm.x - ref);
-        mass = fmaf(f, rm.y, mass);
+            if (half * 128 < p.V) *reinterpret_cast<float4*>(&red[w][half * 128 + lane * 4]) = make_float4(o[4 * half], o[4 * half + 1], o[4 * half + 2], o[4 * half + 3]);
+        if (lane == 0) wl[w] = mass;
+        __syncthreads();
+        if (member > 0) return;
+        for (int i = 1; i < p.team; ++i) {
+            mass += wl[w + i];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            o[4 * half] = fmaf(f, x[half].x, o[4 * half]);
-            o[4 * half + 1] = fmaf(f, x[half].y, o[4 * half + 1]);
-            o[4 * half + 2] = fmaf(f, x[half].z, o[4 * half + 2]);
-            o[4 * half + 3] = fmaf(f, x[half].w, o[4 * half + 3]);
+            for (int half = 0; half < 2; ++half)
+                if (half * 128 < p.V) {
+                    const float4 x = *reinterpret_cast<const float4*>(&red[w + i][half * 128 + lane * 4]);
+                    o[4 * half] += x.x; o[4 * half + 1] += x.y; o[4 * half + 2] += x.z; o[4 * half + 3] += x.w;
+                }
         }
     }
+    if (!on) return;
     const bool real = is_draft(p, task.x, n);
     const int64_t row = ((int64_t)task.x * p.N + n) * p.H + h;
-    if (!p.by_unit) {
-        const float inv = finish_scale(mass);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int col = (i >> 2) * 128 + lane * 4 + (i & 3);
-            if (col < p.V) reinterpret_cast<T*>(p.out)[row * p.V + col] = from_f<T>(real ? o[i] * inv : 0.f);
-        }
-        if (p.lse && lane == 0) p.lse[row] = real ? finish_lse(top, mass) : -INFINITY;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) red[w][(i >> 2) * 128 + lane * 4 + (i & 3)] = o[i];
-    if (lane == 0) wl[w] = mass;
-    __syncthreads();
-    mass = 0.f;
-#pragma unroll
-    for (int i = 0; i < kJoinThreads / 32; ++i) mass += wl[i];
     const float inv = finish_scale(mass);
-    if (tid < p.V) {
-        float x = 0.f;
 #pragma unroll
-        for (int i = 0; i < kJoinThreads / 32; ++i) x += red[i][tid];
-        reinterpret_cast<T*>(p.out)[row * p.V + tid] = from_f<T>(real ? x * inv : 0.f);
+    for (int i = 0; i < 8; i += 2) {
+        const int col = (i >> 2) * 128 + lane * 4 + (i & 3);
+        if (col >= p.V) continue;
+        const float a = real ? o[i] * inv : 0.f, b = real ? o[i + 1] * inv : 0.f;
+        T* to = reinterpret_cast<T*>(p.out) + row * p.V + col;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to) = make_float2(a, b);
+        else *reinterpret_cast<uint32_t*>(to) = Frag<T>::pack(a, b);
     }
-    if (p.lse && tid == 0) p.lse[row] = real ? finish_lse(top, mass) : -INFINITY;
+    if (p.lse && lane == 0) p.lse[row] = real ? finish_lse(top, mass) : -INFINITY;
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------
@@ -1415,6 +1436,8 @@ static void fit(DraftParams& p, int rows, int tile, int blocks, int least) {
     p.grid = blocks;
     p.least = least;
     p.by_unit = units_of(p) <= p.grid;
+    const int64_t each = p.grid / units_of(p);         // parts of a unit
+    p.team = each >= 16 ? 8 : each >= 8 ? 4 : each >= 4 ? 2 : 1;
 }
 static int64_t part_bytes(const DraftParams& p) { return (int64_t)p.grid * 2 * p.rows * (p.V + 2) * 4; }
 static int64_t workspace_of(const DraftParams& p) { return part_bytes(p) + p.grid * 16; }           // tasks: per unit or per part, never more than parts
@@ -1435,6 +1458,29 @@ static void choose(DraftParams& p, int dtype) {
     if (p.c < 1.1754944e-38f) p.c = 1.1754944e-38f;        // a scale of zero: scores of zero, but what is masked stays minus infinity
 }
 
+// The tensor map of a cache; false where its strides are none that a map can have (an expanded dimension), or the driver has no such call.
+static bool cache_map(CUtensorMap& map, const char* base, int width, int64_t row, int64_t head, int64_t page, const DraftParams& p, bool bf16) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<Encode>(f);
+    }();
+    const cuuint64_t dims[4] = {(cuuint64_t)width, p.page.d, (cuuint64_t)p.Hkv, (cuuint64_t)p.pages};
+    // (the stride of a dimension of one element is never used, but has to be one)
+    const cuuint64_t strides[3] = {(cuuint64_t)(p.page.d > 1 ? row : 16), (cuuint64_t)(p.Hkv > 1 ? head : 16), (cuuint64_t)(p.pages > 1 ? page : 16)};
+    const cuuint32_t box[4] = {64, 16, 1, 1}, ones[4] = {1, 1, 1, 1};
+    for (const cuuint64_t x : strides) if (x == 0 || x >= (cuuint64_t(1) << 40)) return false;
+    return encode && encode(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<char*>(base), dims, strides, box, ones,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int DK, int DV, int RM>
 static int launch_mma(const DraftParams& p, cudaStream_t st) {
     static SmemLimit limit;
@@ -1447,7 +1493,11 @@ static int launch_mma(const DraftParams& p, cudaStream_t st) {
     if (p.variant == kTc) {
         static SmemLimit limit;
         if (const cudaError_t e = limit.raise((const void*)draft_tc_kernel<T, DK, DV>, TcShape<DK, DV>::total)) return (int)e;
-        return launch_chained(draft_tc_kernel<T, DK, DV>, dim3(p.grid), dim3(kTcThreads), TcShape<DK, DV>::total, st, p);
+        TcMaps maps{};
+        DraftParams q = p;
+        q.boxes = p.page.d % 16 == 0 && cache_map(maps.k, p.ck, p.K, p.ck_row, p.ck_h, p.ck_page, p, std::is_same<T, __nv_bfloat16>::value) &&
+                  cache_map(maps.v, p.cv, p.V, p.cv_row, p.cv_h, p.cv_page, p, std::is_same<T, __nv_bfloat16>::value);
+        return launch_chained(draft_tc_kernel<T, DK, DV>, dim3(p.grid), dim3(kTcThreads), TcShape<DK, DV>::total, st, q, maps);
     }
     return p.variant == kMma16 ? launch_mma<T, DK, DV, 1>(p, st) : launch_mma<T, DK, DV, 2>(p, st);
 }
@@ -1475,7 +1525,8 @@ static int launch_draft(const DraftParams& p, cudaStream_t st) {
                        : (p.V <= 64 ? launch_mma<T, 128, 64>(p, st) : launch_mma<T, 128, 128>(p, st));
     }
     if (rc) return rc;
-    const dim3 grid = p.by_unit ? dim3((unsigned)units_of(p), p.N * p.G < p.rows ? p.N * p.G : p.rows) : dim3(p.grid, (p.rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
+    const int rows = p.N * p.G < p.rows ? p.N * p.G : p.rows, block = kJoinWarps / p.team;
+    const dim3 grid(p.by_unit ? (unsigned)units_of(p) : (unsigned)p.grid, (rows + block - 1) / block);
     return launch_chained(draft_join_kernel<T>, grid, dim3(kJoinThreads), 0, st, p);
 }
 
