@@ -869,31 +869,66 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
 
 // ---- 16-bit types, more than 32 query rows: tcgen05 -----------------------------------------------------------------------------------
 
-// 128 or 256 query rows a block against tiles of 128 keys, which come from HBM once for all of them.  Per tile and half (128 rows, the
-// lanes of tensor memory): S = Q K^T (operands in shared memory, accumulator in tensor memory), P = 2^(cS - reference) by one thread a row,
-// written over S in 16 bits, O += P V with P read from tensor memory.  The two halves take turns: while one's softmax runs, the other's
-// products do.  Tensor memory: S and O of each half, 128 columns each; shared memory: Q (64 KB), two stages each of K and V (32 KB).
-// Roles: warps 0-3 and 4-7 the softmax of a half, 8 the products, 9-11 the copies.
+// 128 or 256 query rows a block against tiles of 128 keys, which come from HBM once for all of them.  Per job (a tile and 128 rows, the lanes
+// of tensor memory): S = Q K^T (operands in shared memory, accumulator in tensor memory), P = 2^(cS - reference) by a thread a row, written
+// over S in 16 bits, O += P V with P read from tensor memory.  Two halves with an S and an O of their own take turns, so that one's softmax
+// runs beside the other's products: with more than 128 rows each has 128 of them and all tiles, with fewer both have the same rows and
+// every other tile, and are joined at the end.  Tensor memory: S and O of each half, 128 columns each; shared memory: Q (64 KB), two stages
+// each of K and V (32 KB).  Roles: warps 0-3 and 4-7 the softmax of a half, 8 the products, 9-11 the copies.
 // At 256 rows of 128 a tile is 16.8 MFLOP, 2048 cycles of the tensor pipe, and 32768 exponentials, 2048 cycles of the special function
 // units: the two bound it alike, HBM (64 KB a tile) does below about 250 rows.
-constexpr int kTcTile = 128, kTcThreads = 384, kTcProducers = 3;
-constexpr int kTcWaitCap = 1 << 20;
+// A row's weights in a tile may sum to kTcMost before the reference follows (a maximum per tile costs a fifth of the softmax; the sum is there
+// anyway); a reference is set kTcBias below the maximum.  bf16 has fp32's range; fp16 ends at 65504 and keeps all its digits down to 2^-14.
+template <typename T> constexpr float kTcMost = 65536.f;
+template <> constexpr float kTcMost<__half> = 60000.f;
+template <typename T> constexpr float kTcBias = 0.f;
+template <> constexpr float kTcBias<__half> = 6.f;
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 ra, rb, rd;\nmov.b64 ra, {%2, %3};\nmov.b64 rb, {%4, %5};\nadd.rn.f32x2 rd, ra, rb;\nmov.b64 {%0, %1}, rd;\n}\n"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+constexpr int kTcTile = 128, kTcThreads = 384, kTcProducers = 3, kTcMma = 8, kTcCopy = 9;        // (warps)
+constexpr int kTcWaitCap = 1 << 20, kTcPolyEvery = 4;
 
 __device__ __forceinline__ uint32_t tc_idesc(bool bf16, bool negate, bool v_major, int n) {
     // fp32 accumulator; A and B f16 (0) or bf16 (1); A negated; B with N (1) or K (0) contiguous; N / 8; M = 128
     const uint32_t type = bf16 ? 1u : 0u;
     return 1u << 4 | type << 7 | type << 10 | (negate ? 1u : 0u) << 13 | (v_major ? 1u : 0u) << 16 | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
 }
-// Rows of 128 bytes, 128-byte swizzle: `lead` is the distance of 64-element blocks along a contiguous N, 8 rows are 1024 bytes.
-__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lead) {
-    return (uint64_t)(addr >> 4 & 0x3fffu) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+// Descriptors of operands in shared memory: rows of 128 bytes, 128-byte swizzle, 8 rows 1024 bytes; `lead` is the distance of 64-element
+// blocks along a contiguous N.  The address is in the low word, so that a step along the operand is one addition.
+__device__ __forceinline__ uint32_t tc_desc(uint32_t addr, uint32_t lead) { return addr >> 4 | (lead >> 4) << 16; }
+constexpr uint32_t kTcDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 da, db;\nsetp.ne.b32 p, %4, 0;\nmov.b64 da, {%1, %5};\nmov.b64 db, {%2, %5};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(kTcDescHigh) : "memory");
 }
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-                 "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 db;\nsetp.ne.b32 p, 1, 0;\nmov.b64 db, {%2, %4};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(kTcDescHigh) : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, 1, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc) : "memory");
+// One lane of the warp, always the same (and the compiler knows that it is one: the operands of its products are uniform).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t x;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(x));
+    return x != 0;
+}
+// 2^t on the FMA pipes, two at a time, t at most 2^7: t = n + f with n the nearest integer (it appears in the low bits of t + 1.5 * 2^23), 2^f
+// by a polynomial of degree 5 (fitted to the smallest largest relative error over [-1/2, 1/2], 2.3e-7 in fp32), n added to the exponent.
+// What is below -126 comes out as 2^-126; NaN and infinity as something that is not small.
+__device__ __forceinline__ float2 exp2_poly(float2 t) {
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(t.x));
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(t.y));
+    const float2 big = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f);
+    const float2 r = fadd2(t, big), n = fadd2(r, minus), f = ffma2(n, make_float2(-1.f, -1.f), t);
+    float2 y = ffma2(make_float2(0.0013276470126584172f, 0.0013276470126584172f), f, make_float2(0.009675540961325169f, 0.009675540961325169f));
+    y = ffma2(y, f, make_float2(0.05550713092088699f, 0.05550713092088699f));
+    y = ffma2(y, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
+    y = ffma2(y, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
+    y = ffma2(y, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(r.x) << 23)), __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(r.y) << 23)));
 }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
@@ -904,14 +939,17 @@ __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sy
 #define TC_R8(x, i) "=r"((x)[i]), "=r"((x)[i + 1]), "=r"((x)[i + 2]), "=r"((x)[i + 3]), "=r"((x)[i + 4]), "=r"((x)[i + 5]), "=r"((x)[i + 6]), "=r"((x)[i + 7])
 #define TC_U8(x, i) "+r"((x)[i]), "+r"((x)[i + 1]), "+r"((x)[i + 2]), "+r"((x)[i + 3]), "+r"((x)[i + 4]), "+r"((x)[i + 5]), "+r"((x)[i + 6]), "+r"((x)[i + 7])
 #define TC_W8(x, i) "r"((x)[i]), "r"((x)[i + 1]), "r"((x)[i + 2]), "r"((x)[i + 3]), "r"((x)[i + 4]), "r"((x)[i + 5]), "r"((x)[i + 6]), "r"((x)[i + 7])
-// 32 columns of this warp's 32 lanes, a lane a thread; not to be read before tc_wait_ld
-__device__ __forceinline__ void tc_ld32(uint32_t (&x)[32], uint32_t addr) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
-                 "%29,%30,%31}, [%32];\n"
-                 : TC_R8(x, 0), TC_R8(x, 8), TC_R8(x, 16), TC_R8(x, 24) : "r"(addr) : "memory");
+// 16 columns of this warp's 32 lanes, a lane a thread; not to be read before tc_wait_ld
+__device__ __forceinline__ void tc_ld16(uint32_t (&x)[16], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+                 : TC_R8(x, 0), TC_R8(x, 8) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void tc_wait_ld(uint32_t (&x)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;\n" : TC_U8(x, 0), TC_U8(x, 8), TC_U8(x, 16), TC_U8(x, 24)::"memory");
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&x)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : TC_U8(x, 0), TC_U8(x, 8)::"memory"); }
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* x) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr), TC_W8(x, 0), TC_W8(x, 8) : "memory");
+}
+__device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t* x) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(addr), TC_W8(x, 0) : "memory");
 }
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* x) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
@@ -924,7 +962,7 @@ template <int DK, int DV> struct TcShape {
     static constexpr int kst = kTcTile * DK * 2, vst = kTcTile * DV * 2, qhalf = 128 * DK * 2;
     static constexpr int stages = DK + DV > 192 ? 2 : 3;
     static constexpr int q = 0, k = 2 * qhalf, v = k + stages * kst, end = v + stages * vst;
-    static constexpr int bars = end, valid = bars + 256, spoilt = valid + 4 * 16, slot = spoilt + 8 * 16, total = slot + 16 + 1024;
+    static constexpr int bars = end, valid = bars + 256, spoilt = valid + 4 * 16, slot = spoilt + 8 * 16, swap = slot + 16, total = swap + 2 * 256 * 4 + 1024;
 };
 // mbarriers
 enum { kQFull = 0, kQEmpty, kSFull, kPReady = kSFull + 2, kOFull = kPReady + 2, kKFull = kOFull + 2, kKEmpty = kKFull + 3, kVFull = kKEmpty + 3, kVEmpty = kVFull + 3, kTcBars = kVEmpty + 3 };
@@ -959,7 +997,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
     if (tid == 0 && !p.by_unit) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
     if (!find_part<kTcThreads>(p, at, line, x0, x1)) return;
     const int n_tiles = (int)(x1 - x0);
-    if (w == 8) {
+    if (w == kTcMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
         tc_fence_before();
@@ -973,7 +1011,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
     };
     auto two_halves = [&](const Place& pl) { return p.N * p.G - (pl.unit - head_of(p, pl.unit) * p.row_tiles) * p.rows > 128 && p.rows > 128; };
 
-    if (w >= 9) {
+    if (w >= kTcCopy) {
         // ---- copies
         constexpr int KL = DK / 8, VL = DV / 8;
         const uint32_t base = smem_u32(sm);
@@ -981,181 +1019,193 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
         int done = 0;
         // where lane's piece of row r goes within a 128-row operand: 64 columns to a block of 128-byte rows, 16-byte pieces swizzled by the row
         auto place_of = [&](int r, int c) { return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
+        // This warp's slices of sixteen keys of a tile, w - 9, w - 6 and w - 3.  Sixteen cached tokens of one page are a box of the tensor maps
+        // (page >= 0, from token in of the page); of others (a sequence's end, drafts, small pages) lane x (and x + 16) knows the rows of key x.
+        struct Rows {
+            const char *k[3], *v[3];
+            uint32_t m[3];
+            int page[3], in[3];
+            bool any;
+        };
+        Rows ahead;
+        auto look = [&](Rows& r, const Place& pl, int j, int) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const int sl = w - kTcCopy + i * kTcProducers, pos = (pl.tile + j) * kTcTile + sl * 16;
+                r.page[i] = -1;
+                r.in[i] = 0;
+                if (p.boxes && sl < 8 && pl.tile + j < pl.tiles - p.draft_tiles && pos + 16 <= pl.len) {
+                    const int no = (int)p.page.div((uint32_t)pos);
+                    r.in[i] = pos - no * (int)p.page.d;
+                    r.page[i] = __ldg(p.table + (int64_t)pl.b * p.table_stride + no);
+                }
+            }
+        };
+        auto find_rows = [&](Rows& r, const Place& pl, int kv, int tile) {
+            r.any = false;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const int sl = w - kTcCopy + i * kTcProducers;
+                r.m[i] = 0;
+                if (r.page[i] >= 0 && r.page[i] < p.pages) { r.m[i] = 0xffffu; continue; }
+                r.page[i] = -1;
+                if (sl >= 8) continue;
+                const char *k = p.q, *v = p.q;
+                const bool on = key_row(p, Place{pl.b, pl.unit, tile, pl.tiles, pl.len}, kv, sl * 16 + (lane & 15), k, v, &bad);
+                r.k[i] = k; r.v[i] = v;
+                r.m[i] = __ballot_sync(0xffffffffu, on) & 0xffffu;
+                r.any = true;
+            }
+        };
+        // one operand of a tile; draft >= 0: values of drafts, noted in that line of `spoilt`
+        auto copy = [&](const CUtensorMap& map, int full, const Rows& rows, uint32_t dst, auto lanes_, int width, int kv, int draft) {
+            constexpr int lanes = decltype(lanes_)::value, per = 32 / lanes;
+            const bool values = &map == &maps.v;
+            uint32_t bytes = 0;
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const int sl = w - kTcCopy + i * kTcProducers;
+                if (rows.page[i] < 0) continue;
+                bytes += 16 * 16 * lanes;
+                if (elect_one())
+#pragma unroll
+                    for (int blk = 0; blk < lanes / 8; ++blk)
+                        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
+                                         dst + blk * (128 * 128) + sl * 2048), "l"(&map), "r"(blk * 64), "r"(rows.in[i]), "r"(kv), "r"(rows.page[i]),
+                                     "r"(smem_u32(bars + full)) : "memory");
+            }
+            if (rows.any) {
+                const int c = lane % lanes;
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    const int sl = w - kTcCopy + i * kTcProducers;
+                    if (sl >= 8 || rows.page[i] >= 0) continue;
+#pragma unroll 4
+                    for (int r = 0; r < 16; r += per) {
+                        const int x = r + lane / lanes;
+                        const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(values ? rows.v[i] : rows.k[i]), x));
+                        const bool on = (rows.m[i] >> x & 1) && c * 8 < width;
+                        cp_async16_or_zero(dst + place_of(sl * 16 + x, c), on ? src + c * 16 : p.q, on);
+                    }
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                if (draft >= 0)
+#pragma unroll 1
+                    for (int sl = w - kTcCopy; sl < 8; sl += kTcProducers)
+#pragma unroll 1
+                        for (int r = 0; r < 16; r += per) {
+                            const int x = sl * 16 + r + lane / lanes;
+                            if (take_out<T>(dst + place_of(x, c))) atomicOr(&spoilt[draft * 4 + (x >> 5)], 1u << (x & 31));
+                        }
+                fence_proxy_async();
+                __syncwarp();
+            }
+            if (lane == 0) mbar_arrive_expect_tx(bars + full, bytes);
+        };
         while (done < n_tiles) {
             const int piece = min(n_tiles - done, at.tiles - at.tile), cached = at.tiles - p.draft_tiles, kv = head_of(p, at.unit);
             { bool b = false; draft_length(p, at.b, &b); bad |= b; }
             wait(kQEmpty, (unit_no & 1) ^ 1);
             const int halves = two_halves(at) ? 2 : 1;
 #pragma unroll 1
-            for (int r0 = (w - 9) * (32 / KL); r0 < halves * 128; r0 += kTcProducers * (32 / KL)) {
+            for (int r0 = (w - kTcCopy) * (32 / KL); r0 < halves * 128; r0 += kTcProducers * (32 / KL)) {
                 const int r = r0 + lane / KL, c = lane % KL;
                 int n, h;
                 const bool on = row_of(p, at.unit, r, n, h) && c * 8 < p.K;
                 cp_async16_or_zero(base + S::q + (r >> 7) * S::qhalf + place_of(r & 127, c), on ? p.q + at.b * p.q_b + n * p.q_n + h * p.q_h + c * 16 : p.q, on);
             }
             cp_async_commit();
-            for (int j = 0; j < piece; ++j, ++g) {
-                const int tile = at.tile + j, st = g % ST;
-                const uint32_t ph = (uint32_t)(g / ST) & 1u;
-                // This warp's slices of sixteen keys, w - 9, w - 6, w - 3.  Sixteen cached tokens of one page are a box of the tensor maps; of
-                // others (a sequence's end, drafts, small pages) lane x (and x + 16) knows the row of key x.
-                const char *kr[3], *vr[3];
-                uint32_t m[3];
-                int page[3], in[3];
-                bool rows = false;
-#pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    const int sl = w - 9 + i * kTcProducers, pos = tile * kTcTile + sl * 16;
-                    page[i] = -1;
-                    m[i] = 0;
-                    if (p.boxes && sl < 8 && tile < cached && pos + 16 <= at.len) {
-                        const int no = (int)p.page.div((uint32_t)pos);
-                        in[i] = pos - no * (int)p.page.d;
-                        page[i] = __ldg(p.table + (int64_t)at.b * p.table_stride + no);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    const int sl = w - 9 + i * kTcProducers;
-                    kr[i] = vr[i] = p.q;
-                    if (page[i] >= 0 && page[i] < p.pages) { m[i] = 0xffffu; continue; }
-                    page[i] = -1;
-                    if (sl >= 8) continue;
-                    const char *k = p.q, *v = p.q;
-                    const bool on = key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, sl * 16 + (lane & 15), k, v, &bad);
-                    kr[i] = k; vr[i] = v;
-                    m[i] = __ballot_sync(0xffffffffu, on) & 0xffffu;
-                    rows = true;
-                }
-                auto copy = [&](const CUtensorMap& map, int full, int empty, const char* const (&row)[3], uint32_t dst, int lanes, int width, bool values) {
-                    wait(empty, ph ^ 1);
-                    uint32_t bytes = 0;
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) {
-                        const int sl = w - 9 + i * kTcProducers;
-                        if (page[i] < 0) continue;
-                        bytes += 16 * 16 * lanes;
-                        if (lane == 0)
-                            for (int blk = 0; blk < lanes / 8; ++blk)
-                                asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
-                                                 dst + blk * (128 * 128) + sl * 2048), "l"(&map), "r"(blk * 64), "r"(in[i]), "r"(kv), "r"(page[i]),
-                                             "r"(smem_u32(bars + full)) : "memory");
-                    }
-                    if (rows) {
-                        const int per = 32 / lanes, c = lane % lanes;
+            // Keys run one tile ahead of values: their stage is free as soon as the scores are there.
+            Rows now, next;
+            look(now, at, 0, piece);
+            find_rows(now, at, kv, at.tile);
+            for (int j = -1; j < piece; ++j) {
+                if (j + 1 < piece) {
+                    if (j >= 0) next = ahead;
+                    Rows& r = j >= 0 ? next : now;
+                    if (j >= 0) find_rows(r, at, kv, at.tile + j + 1);
+                    if (j + 2 < piece) look(ahead, at, j + 2, piece);
+                    const int t = g + j + 1, st = t % ST;
+                    wait(kKEmpty + st, ((uint32_t)(t / ST) & 1u) ^ 1u);
+                    // (the words of the tile four before are no longer read: the products after it are done, or this stage would not be empty)
+                    if (lane == 0)
 #pragma unroll
                         for (int i = 0; i < 3; ++i) {
-                            const int sl = w - 9 + i * kTcProducers;
-                            if (sl >= 8 || page[i] >= 0) continue;
-#pragma unroll 2
-                            for (int r = 0; r < 16; r += per) {
-                                const int x = r + lane / lanes;
-                                const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row[i]), x));
-                                const bool on = (m[i] >> x & 1) && c * 8 < width;
-                                cp_async16_or_zero(dst + place_of(sl * 16 + x, c), on ? src + c * 16 : p.q, on);
-                            }
+                            const int sl = w - kTcCopy + i * kTcProducers;
+                            if (sl < 8) reinterpret_cast<uint16_t*>(valid + (t & 3) * 4)[sl] = (uint16_t)r.m[i];
                         }
-                        cp_async_commit();
+                    copy(maps.k, kKFull + st, r, base + S::k + st * S::kst, std::integral_constant<int, KL>{}, p.K, kv, -1);
+                    if (j < 0) {
                         cp_async_wait<0>();
-                        if (values && tile >= cached)
-#pragma unroll 1
-                            for (int sl = w - 9; sl < 8; sl += kTcProducers)
-#pragma unroll 1
-                                for (int r = 0; r < 16; r += per) {
-                                    const int x = sl * 16 + r + lane / lanes;
-                                    if (take_out<T>(dst + place_of(x, c))) atomicOr(&spoilt[(g & 7) * 4 + (x >> 5)], 1u << (x & 31));
-                                }
                         fence_proxy_async();
                         __syncwarp();
+                        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bars + kQFull)) : "memory");
                     }
-                    if (lane == 0) mbar_arrive_expect_tx(bars + full, bytes);
-                };
-                // (the words of the tile four before are no longer read: its products are done, or this stage would not be empty)
-                wait(kKEmpty + st, ph ^ 1);
-                if (lane == 0)
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) {
-                        const int sl = w - 9 + i * kTcProducers;
-                        if (sl < 8) reinterpret_cast<uint16_t*>(valid + (g & 3) * 4)[sl] = (uint16_t)m[i];
-                    }
-                copy(maps.k, kKFull + st, kKEmpty + st, kr, base + S::k + st * S::kst, KL, p.K, false);
-                if (j == 0) {
-                    cp_async_wait<0>();
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bars + kQFull)) : "memory");
                 }
-                wait(kVEmpty + st, ph ^ 1);
-                if (w == 9 && lane < 4) spoilt[((g - ST) & 7) * 4 + lane] = 0;
-                copy(maps.v, kVFull + st, kVEmpty + st, vr, base + S::v + st * S::vst, VL, p.V, true);
+                if (j >= 0) {
+                    const int t = g + j, st = t % ST;
+                    wait(kVEmpty + st, ((uint32_t)(t / ST) & 1u) ^ 1u);
+                    if (w == kTcCopy && lane < 4) spoilt[((t - ST) & 7) * 4 + lane] = 0;
+                    copy(maps.v, kVFull + st, now, base + S::v + st * S::vst, std::integral_constant<int, VL>{}, p.V, kv, at.tile + j >= cached ? t & 7 : -1);
+                    now = next;
+                }
             }
+            g += piece;
             done += piece;
             ++unit_no;
             at.tile += piece - 1;
             at.next(p);
         }
-    } else if (w == 8) {
+    } else if (w == kTcMma) {
         // ---- products
-        if (lane == 0) {
+        if (elect_one()) {
             const uint32_t base = smem_u32(sm), iqk = tc_idesc(BF, p.neg, false, kTcTile), ipv = tc_idesc(BF, false, true, DV);
-            auto qk = [&](int half, int st) {
-                const uint32_t a = base + S::q + half * S::qhalf, b = base + S::k + st * S::kst;
+            auto qk = [&](int half, int rows, int st) {
+                const uint32_t a = tc_desc(base + S::q + rows * S::qhalf, 16), b = tc_desc(base + S::k + st * S::kst, 16);
 #pragma unroll
                 for (int ks = 0; ks < DK / 16; ++ks) {
-                    const uint32_t off = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
-                    tc_mma_ss(tmem + half * 128, tc_desc(a + off, 16), tc_desc(b + off, 16), iqk, ks > 0);
+                    const uint32_t off = ((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4;
+                    tc_mma_ss(tmem + half * 128, a + off, b + off, iqk, ks > 0);
                 }
             };
             auto pv = [&](int half, int st) {
-                const uint32_t b = base + S::v + st * S::vst;
+                const uint32_t b = tc_desc(base + S::v + st * S::vst, 128 * 128);
 #pragma unroll
-                for (int ks = 0; ks < kTcTile / 16; ++ks) tc_mma_ts(tmem + 256 + half * 128, tmem + half * 128 + ks * 8, tc_desc(b + ks * 2048, 128 * 128), ipv);
+                for (int ks = 0; ks < kTcTile / 16; ++ks) tc_mma_ts(tmem + 256 + half * 128, tmem + half * 128 + ks * 8, b + ks * (2048 >> 4), ipv);
             };
             int g = 0, unit_no = 0, done = 0;
-            uint32_t pa = 0, pb = 0;                      // tiles whose P a half has had
+            uint32_t had[2] = {0, 0};                     // jobs whose P a half has had
             while (done < n_tiles) {
                 const int piece = min(n_tiles - done, at.tiles - at.tile);
-                const bool two = two_halves(at);
+                // job i: half i & 1, tile i / 2 of the unit or (few rows) tile i
+                const int two = two_halves(at) ? 1 : 0, jobs = piece << two;
+                auto scores = [&](int i) {
+                    const int t = g + (i >> two), st = t % ST;
+                    if (!two || !(i & 1)) {
+                        wait(kKFull + st, (uint32_t)(t / ST) & 1u);
+                        tc_fence_after();
+                    }
+                    qk(i & 1, two ? i & 1 : 0, st);
+                    tc_commit(bars + kSFull + (i & 1));
+                    if (!two || (i & 1)) tc_commit(bars + kKEmpty + st);
+                };
                 wait(kQFull, unit_no & 1);
-                wait(kKFull + g % ST, (uint32_t)(g / ST) & 1u);
-                tc_fence_after();
-                qk(0, g % ST);
-                tc_commit(bars + kSFull);
-                if (two) {
-                    qk(1, g % ST);
-                    tc_commit(bars + kSFull + 1);
-                }
-                tc_commit(bars + kKEmpty + g % ST);
-                for (int j = 0; j < piece; ++j, ++g) {
-                    const int st = g % ST, nx = (g + 1) % ST;
-                    const bool more = j + 1 < piece;
-                    wait(kVFull + st, (uint32_t)(g / ST) & 1u);
-                    wait(kPReady, pa++ & 1u);
+                scores(0);
+                if (jobs > 1) scores(1);
+                for (int i = 0; i < jobs; ++i) {
+                    const int half = i & 1, t = g + (i >> two), st = t % ST;
+                    if (!two || !half) wait(kVFull + st, (uint32_t)(t / ST) & 1u);
+                    wait(kPReady + half, (half ? had[1]++ : had[0]++) & 1u);
                     tc_fence_after();
-                    pv(0, st);
-                    if (!more) tc_commit(bars + kOFull);
-                    if (more) {
-                        wait(kKFull + nx, (uint32_t)((g + 1) / ST) & 1u);
-                        tc_fence_after();
-                        qk(0, nx);
-                        tc_commit(bars + kSFull);
-                    }
-                    if (two) {
-                        wait(kPReady + 1, pb++ & 1u);
-                        tc_fence_after();
-                        pv(1, st);
-                        if (!more) tc_commit(bars + kOFull + 1);
-                    }
-                    tc_commit(bars + kVEmpty + st);
-                    if (more) {
-                        if (two) {
-                            qk(1, nx);
-                            tc_commit(bars + kSFull + 1);
-                        }
-                        tc_commit(bars + kKEmpty + nx);
-                    }
+                    pv(half, st);
+                    if (i + 2 >= jobs) tc_commit(bars + kOFull + half);
+                    if (!two || half) tc_commit(bars + kVEmpty + st);
+                    if (i + 2 < jobs) scores(i + 2);
                 }
                 tc_commit(bars + kQEmpty);
+                g += piece;
                 done += piece;
                 ++unit_no;
                 at.tile += piece - 1;
@@ -1166,161 +1216,207 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
         __syncwarp();
     } else {
         // ---- softmax: a thread a row
-        const int half = w >> 2, row = half * 128 + (w & 3) * 32 + lane;
+        const int half = w >> 2, lane_row = (w & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)(w & 3) << 21;   // lane 32 * (w & 3) of tensor memory
-        const uint32_t ts = tmem + lanes + half * 128, to = tmem + lanes + 256 + half * 128;
+        const uint32_t ts = tmem + lanes + half * 128, to = tmem + lanes + 256 + half * 128, to_other = tmem + lanes + 256 + (half ^ 1) * 128;
+        float2* swap = reinterpret_cast<float2*>(sm + S::swap);              // [half][row]: reference, mass
         int g = 0, done = 0;
-        uint32_t turns = 0, units_had = 0;
+        uint32_t turns = 0, ends[2] = {0, 0};             // jobs of this half; units that either half had jobs of
         bool first_piece = true;
         while (done < n_tiles) {
             const int piece = min(n_tiles - done, at.tiles - at.tile), cached = at.tiles - p.draft_tiles;
-            const bool whole = at.tile == 0 && piece == at.tiles;
+            const bool whole = at.tile == 0 && piece == at.tiles, two = two_halves(at);
             if (tid == 0 && at.tile == 0) leave_task(p, at, x0 + done, x0, blockIdx.x, line, whole);
-            if (half == 0 || two_halves(at)) {
-                int n, h;
-                const bool on = row_of(p, at.unit, row, n, h);
-                uint32_t x[2][32];
+            const int row = two ? half * 128 + lane_row : lane_row, jobs = two ? piece : (piece + 1 - half) >> 1;
+            int n, h;
+            const bool on = row_of(p, at.unit, row, n, h);
+            uint32_t x[2][16];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) x[0][i] = 0;
+            for (int i = 0; i < 16; ++i) x[0][i] = 0;
 #pragma unroll
-                for (int c = 0; c < DV / 32; ++c) tc_st32(to + c * 32, x[0]);
-                float ref = -INFINITY, mass = 0.f;
-                for (int j = 0; j < piece; ++j) {
-                    const int tile = at.tile + j, gg = g + j;
-                    const bool draft = tile >= cached;
-                    wait(kSFull + half, turns++ & 1u);
-                    tc_fence_after();
-                    uint32_t seen[4];
+            for (int c = 0; c < DV; c += 16) tc_st16(to + c, x[0]);
+            float ref = 0.f, mass = 0.f;
+            bool empty = true;                            // the row has had no key yet
+            for (int i = 0; i < jobs; ++i) {
+                const int j = two ? i : 2 * i + half, tile = at.tile + j, gg = g + j;
+                wait(kSFull + half, turns++ & 1u);
+                tc_fence_after();
+                tc_ld16(x[0], ts);
+                uint32_t seen[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) seen[i] = valid[(gg & 3) * 4 + i];
-                    if (draft) {
-                        const int tile0 = (tile - cached) * kTcTile;
-                        const uint64_t lo = on ? draft_mask(p, at.b, n, tile0, &bad) : 0ull, hi = on ? draft_mask(p, at.b, n, tile0 + 64, &bad) : 0ull;
-                        seen[0] &= (uint32_t)lo; seen[1] &= (uint32_t)(lo >> 32); seen[2] &= (uint32_t)hi; seen[3] &= (uint32_t)(hi >> 32);
-                        wait(kVFull + gg % ST, (uint32_t)(gg / ST) & 1u);
-                        uint32_t sp[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sp[i] = spoilt[(gg & 7) * 4 + i];
-                        if (sp[0] | sp[1] | sp[2] | sp[3]) {
-                            tc_wait_st();
-                            const char* v0 = p.v + at.b * p.v_b + head_of(p, at.unit) * p.v_h;
+                for (int c = 0; c < 4; ++c) seen[c] = valid[(gg & 3) * 4 + c];
+                if (tile >= cached) {
+                    const int tile0 = (tile - cached) * kTcTile;
+                    const uint64_t lo = on ? draft_mask(p, at.b, n, tile0, &bad) : 0ull, hi = on ? draft_mask(p, at.b, n, tile0 + 64, &bad) : 0ull;
+                    seen[0] &= (uint32_t)lo; seen[1] &= (uint32_t)(lo >> 32); seen[2] &= (uint32_t)hi; seen[3] &= (uint32_t)(hi >> 32);
+                    wait(kVFull + gg % ST, (uint32_t)(gg / ST) & 1u);
+                    const uint32_t* sp = spoilt + (gg & 7) * 4;
+                    if (sp[0] | sp[1] | sp[2] | sp[3]) {
+                        tc_wait_st();
+                        tc_wait_ld(x[0]);
+                        const char* v0 = p.v + at.b * p.v_b + head_of(p, at.unit) * p.v_h;
 #pragma unroll 1
-                            for (int key = 0; key < kTcTile; ++key) {
-                                const uint32_t word = key < 32 ? sp[0] : key < 64 ? sp[1] : key < 96 ? sp[2] : sp[3];
-                                if (!(word >> (key & 31) & 1)) continue;
-                                const uint32_t mine = key < 32 ? seen[0] : key < 64 ? seen[1] : key < 96 ? seen[2] : seen[3];
+                        for (int key = 0; key < kTcTile; ++key) {
+                            if (!(sp[key >> 5] >> (key & 31) & 1)) continue;
+                            const uint32_t mine = key < 32 ? seen[0] : key < 64 ? seen[1] : key < 96 ? seen[2] : seen[3];
 #pragma unroll 1
-                                for (int c = 0; c < DV; c += 32) {
-                                    tc_ld32(x[0], to + c);
-                                    tc_wait_ld(x[0]);
-                                    if (mine >> (key & 31) & 1)
-#pragma unroll
-                                        for (int i = 0; i < 32; ++i)
-                                            if (c + i < p.V) x[0][i] = __float_as_uint(put_back<T>(__uint_as_float(x[0][i]), v0 + (int64_t)(tile0 + key) * p.v_n, c + i));
-                                    tc_st32(to + c, x[0]);
-                                    tc_wait_st();
-                                }
-                            }
-                        }
-                    }
-                    const bool gaps = (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu;
-                    const bool masked = __any_sync(0xffffffffu, gaps);
-                    uint32_t pk[64];
-                    float top = -INFINITY, sum = 0.f;
-                    // One pass: P with the present reference, and the row's maximum; if that is further above the reference than P may grow,
-                    // (for the first tile always) the reference moves, the sums with it, and P is made again.
-                    bool again = j == 0;
-                    for (int pass = again ? 1 : 0;; ++pass) {
-                        const float base = ref == -INFINITY ? 0.f : -ref;
-                        sum = 0.f;
-                        const bool only_max = again && pass == 1;
-                        tc_ld32(x[0], ts);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t(&y)[32] = x[c & 1];
-                            tc_wait_ld(y);
-                            if (c < 3) tc_ld32(x[(c + 1) & 1], ts + (c + 1) * 32);
-                            if (masked)
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) y[i] = (seen[c] >> i & 1) ? y[i] : 0xff800000u;
-                            if (pass < 2) {
-                                float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-                                for (int i = 0; i < 32; i += 4) {
-                                    t0 = fmaxf(t0, fmaxf(__uint_as_float(y[i]), __uint_as_float(y[i + 1])));
-                                    t1 = fmaxf(t1, fmaxf(__uint_as_float(y[i + 2]), __uint_as_float(y[i + 3])));
-                                }
-                                top = fmaxf(top, fmaxf(t0, t1));
-                            }
-                            if (!only_max) {
-                                float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-                                for (int i = 0; i < 32; i += 2) {
-                                    const float e0 = ex2_approx(fmaf(__uint_as_float(y[i]), p.c, base)), e1 = ex2_approx(fmaf(__uint_as_float(y[i + 1]), p.c, base));
-                                    s0 += e0;
-                                    s1 += e1;
-                                    pk[c * 16 + (i >> 1)] = Frag<T>::pack(e0, e1);
-                                }
-                                sum += s0 + s1;
-                            }
-                        }
-                        if (pass >= 2) break;
-                        const float t = top * p.c;
-                        if (!only_max && !__any_sync(0xffffffffu, t > ref + (kLag<T> + kBias<T>))) break;
-                        const float now = fmaxf(ref, t - kBias<T>);
-                        const float keep = now == -INFINITY ? 1.f : ex2_approx(ref - now);
-                        ref = now;
-                        mass *= keep;
-                        if (j > 0) {
-#pragma unroll 1
-                            for (int c = 0; c < DV; c += 32) {
-                                tc_ld32(x[0], to + c);
+                            for (int c = 0; c < DV; c += 16) {
+                                tc_ld16(x[0], to + c);
                                 tc_wait_ld(x[0]);
+                                if (mine >> (key & 31) & 1)
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) x[0][i] = __float_as_uint(__uint_as_float(x[0][i]) * keep);
-                                tc_st32(to + c, x[0]);
+                                    for (int e = 0; e < 16; ++e)
+                                        if (c + e < p.V) x[0][e] = __float_as_uint(put_back<T>(__uint_as_float(x[0][e]), v0 + (int64_t)(tile0 + key) * p.v_n, c + e));
+                                tc_st16(to + c, x[0]);
+                                tc_wait_st();
                             }
                         }
-                        pass = 1;
+                        tc_ld16(x[0], ts);
                     }
-                    mass += sum;
+                }
+                uint32_t pk[64];
+                float2 sums[2];
+                sums[0] = sums[1] = make_float2(0.f, 0.f);
+                // P and its sum, of 16 scores; `mixed`: every kTcPolyEvery-th pair of exponentials on the FMA pipes
+                auto weigh = [&](const uint32_t (&y)[16], uint32_t* to_pk, auto mixed) {
+                    const float2 cc = make_float2(p.c, p.c), bb = make_float2(-ref, -ref);
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float2 t = ffma2(make_float2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), cc, bb);
+                        const float2 v = decltype(mixed)::value && (e >> 1) % kTcPolyEvery == kTcPolyEvery - 1 ? exp2_poly(t) : make_float2(ex2_approx(t.x), ex2_approx(t.y));
+                        sums[(e >> 1) & 1] = fadd2(sums[(e >> 1) & 1], v);
+                        to_pk[e >> 1] = Frag<T>::pack(v.x, v.y);
+                    }
+                };
+                bool anew = __any_sync(0xffffffffu, empty || (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu);
+                if (!anew) {
+                    // the reference stays, unless the weights get too large for the type: their sum tells (none is larger than it)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        tc_wait_ld(x[c & 1]);
+                        if (c < 7) tc_ld16(x[(c + 1) & 1], ts + (c + 1) * 16);
+                        weigh(x[c & 1], pk + c * 8, std::true_type{});
+                    }
+                    anew = __any_sync(0xffffffffu, !((sums[0].x + sums[0].y) + (sums[1].x + sums[1].y) <= kTcMost<T>));
+                } else {
+                    tc_wait_ld(x[0]);
+                }
+                if (anew) {
+                    // the row's maximum first; the sums follow the reference if it moves
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < 8; ++c) {
+                        tc_ld16(x[0], ts + c * 16);
+                        tc_wait_ld(x[0]);
+                        const uint32_t there = (c < 2 ? seen[0] : c < 4 ? seen[1] : c < 6 ? seen[2] : seen[3]) >> (c & 1) * 16;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) top = fmaxf(top, (there >> e & 1) ? __uint_as_float(x[0][e]) : -INFINITY);
+                    }
+                    // (a row that has had nothing yet keeps a reference of zero, which is worth nothing)
+                    const float want = top * p.c - kTcBias<T>, now = top == -INFINITY ? ref : empty ? want : fmaxf(ref, want);
+                    const float keep = empty ? 1.f : ex2_approx(ref - now);
+                    if (top != -INFINITY) empty = false;
+                    ref = now;
+                    mass *= keep;
+                    if (__any_sync(0xffffffffu, keep != 1.f)) {
+#pragma unroll 1
+                        for (int c = 0; c < DV; c += 16) {
+                            tc_ld16(x[0], to + c);
+                            tc_wait_ld(x[0]);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) x[0][e] = __float_as_uint(__uint_as_float(x[0][e]) * keep);
+                            tc_st16(to + c, x[0]);
+                        }
+                    }
+                    // (weights over the scores of sixteen keys take the place of eight: never of scores still to be read)
+                    sums[0] = sums[1] = make_float2(0.f, 0.f);
+#pragma unroll 1
+                    for (int c = 0; c < 8; ++c) {
+                        tc_ld16(x[0], ts + c * 16);
+                        tc_wait_ld(x[0]);
+                        const uint32_t there = (c < 2 ? seen[0] : c < 4 ? seen[1] : c < 6 ? seen[2] : seen[3]) >> (c & 1) * 16;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[0][e] = (there >> e & 1) ? x[0][e] : 0xff800000u;
+                        weigh(x[0], pk, std::false_type{});
+                        tc_st8(ts + c * 8, pk);
+                    }
+                } else {
                     tc_st32(ts, pk);
                     tc_st32(ts + 32, pk + 32);
-                    tc_wait_st();
-                    tc_fence_before();
-                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bars + kPReady + half)) : "memory");
                 }
-                wait(kOFull + half, units_had++ & 1u);
-                tc_fence_after();
-                const bool real = on && is_draft(p, at.b, n);
-                const float f = whole ? (real ? finish_scale(mass) : 0.f) : 1.f;
-                const int64_t at_out = ((int64_t)at.b * p.N + n) * p.H + h;
-                float* slot = p.part + (int64_t)(2 * blockIdx.x + (first_piece ? 0 : 1)) * p.rows * (p.V + 2);
+                mass += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+                tc_wait_st();
+                tc_fence_before();
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bars + kPReady + half)) : "memory");
+            }
+            // with both halves on the same rows: one reference, the other half's sums added, each half for half the columns
+            float f_own = 1.f, f_other = 0.f;
+            int c0 = 0, c1 = DV;
+            if (!two) {
+                swap[half * 128 + lane_row] = make_float2(empty ? -INFINITY : ref, mass);
+                tc_wait_st();                             // (a half without jobs: its zeros)
+                tc_fence_before();
+                asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");
+                const float2 other = swap[(half ^ 1) * 128 + lane_row];
+                const float own = empty ? -INFINITY : ref, t = fmaxf(own, other.x);
+                if (t != -INFINITY) {
+                    f_own = ex2_approx(own - t);
+                    f_other = ex2_approx(other.x - t);
+                    ref = t;
+                    empty = false;
+                }
+                mass = mass * f_own + other.y * f_other;
+                c0 = half * (DV / 2);
+                c1 = c0 + DV / 2;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const bool had_any = two || i == 0 || piece > 1;
+                if (had_any) {
+                    if (!two || i == half) wait(kOFull + i, ends[i] & 1u);
+                    ++ends[i];
+                }
+            }
+            tc_fence_after();
+            const bool real = on && is_draft(p, at.b, n), add = !two;
+            const float inv = whole ? (real ? finish_scale(mass) : 0.f) : 1.f;
+            const int64_t at_out = ((int64_t)at.b * p.N + n) * p.H + h;
+            float* slot = p.part + (int64_t)(2 * blockIdx.x + (first_piece ? 0 : 1)) * p.rows * (p.V + 2);
 #pragma unroll 1
-                for (int c = 0; c < DV; c += 32) {
-                    tc_ld32(x[0], to + c);
-                    tc_wait_ld(x[0]);
-                    if (!on) continue;
+            for (int c = c0; c < c1; c += 16) {
+                tc_ld16(x[0], to + c);
+                if (add) tc_ld16(x[1], to_other + c);
+                tc_wait_ld(x[0]);
+                tc_wait_ld(x[1]);
+                if (!on) continue;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        if (c + i >= p.V) break;
-                        float o[8];
+                for (int i = 0; i < 16; i += 8) {
+                    if (c + i >= p.V) break;
+                    float o[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(x[0][i + e]) * f;
-                        if (whole) {
-                            uint4 y = make_uint4(Frag<T>::pack(o[0], o[1]), Frag<T>::pack(o[2], o[3]), Frag<T>::pack(o[4], o[5]), Frag<T>::pack(o[6], o[7]));
-                            if (!real) y = make_uint4(0, 0, 0, 0);
-                            *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + at_out * p.V + c + i) = y;
-                        } else {
-                            *reinterpret_cast<float4*>(slot + row * p.V + c + i) = make_float4(o[0], o[1], o[2], o[3]);
-                            *reinterpret_cast<float4*>(slot + row * p.V + c + i + 4) = make_float4(o[4], o[5], o[6], o[7]);
-                        }
+                    for (int e = 0; e < 8; ++e) {
+                        o[e] = __uint_as_float(x[0][i + e]);
+                        if (add) o[e] = o[e] * f_own + __uint_as_float(x[1][i + e]) * f_other;
+                        o[e] *= inv;
+                    }
+                    if (whole) {
+                        uint4 y = make_uint4(Frag<T>::pack(o[0], o[1]), Frag<T>::pack(o[2], o[3]), Frag<T>::pack(o[4], o[5]), Frag<T>::pack(o[6], o[7]));
+                        if (!real) y = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + at_out * p.V + c + i) = y;
+                    } else {
+                        *reinterpret_cast<float4*>(slot + row * p.V + c + i) = make_float4(o[0], o[1], o[2], o[3]);
+                        *reinterpret_cast<float4*>(slot + row * p.V + c + i + 4) = make_float4(o[4], o[5], o[6], o[7]);
                     }
                 }
-                if (on) {
-                    if (!whole) *reinterpret_cast<float2*>(slot + p.rows * p.V + 2 * row) = make_float2(ref, mass);
-                    else if (p.lse) p.lse[at_out] = real ? finish_lse(ref, mass) : -INFINITY;
-                }
+            }
+            if (on && (two || half == 0)) {
+                if (!whole) *reinterpret_cast<float2*>(slot + p.rows * p.V + 2 * row) = make_float2(empty ? -INFINITY : ref, mass);
+                else if (p.lse) p.lse[at_out] = real ? finish_lse(ref, mass) : -INFINITY;
+            }
+            if (!two) {                                   // the other half has read this one's O, and this thread's words
+                tc_fence_before();
+                asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");
+                tc_fence_after();
             }
             g += piece;
             first_piece = false;
@@ -1331,7 +1427,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
         tc_fence_before();
     }
     __syncthreads();
-    if (w == 8) {
+    if (w == kTcMma) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
     }
