@@ -38,7 +38,7 @@ struct DraftParams {
     int32_t room;             // tokens that a row of the table can name
     int32_t grid, least, by_unit, team;                                    // parts at most; tiles of a part at least; how tasks are indexed, and joined
     int32_t variant;          // which kernel (choose)
-    int32_t boxes;            // tcgen05 kernel: pages of whole slices of sixteen tokens come by the tensor maps
+    int32_t boxes;            // tcgen05 kernel: what comes by tensor maps: 1 pages of whole slices of sixteen tokens, 2 q, 4 drafts
     int32_t neg;              // tensor-core kernels: the scale is negative, c its magnitude and q's signs are turned
     float c;                  // scale * log2 e
     FastDiv page, group, per_head;      // by the page size, by G, by row_tiles
@@ -956,16 +956,18 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* x) {
                  "%29,%30,%31,%32};\n" ::"r"(addr), TC_W8(x, 0), TC_W8(x, 8), TC_W8(x, 16), TC_W8(x, 24) : "memory");
 }
 
-struct TcMaps { CUtensorMap k, v; };       // the caches as [page][head][token][element], boxes of 16 tokens and 128 bytes
+// The caches as [page][head][token][element] and the drafts' k, v as [request][head][draft][element], boxes of 16 tokens and 128 bytes; q as
+// [request][draft][head][element], boxes of a group's heads of 128 / G drafts.
+struct TcMaps { CUtensorMap k, v, dk, dv, q; };
 
 template <int DK, int DV> struct TcShape {
     static constexpr int kst = kTcTile * DK * 2, vst = kTcTile * DV * 2, qhalf = 128 * DK * 2;
     static constexpr int stages = DK + DV > 192 ? 2 : 3;
     static constexpr int q = 0, k = 2 * qhalf, v = k + stages * kst, end = v + stages * vst;
-    static constexpr int bars = end, valid = bars + 256, spoilt = valid + 4 * 16, slot = spoilt + 8 * 16, swap = slot + 16, total = swap + 2 * 256 * 4 + 1024;
+    static constexpr int bars = end, valid = bars + 256, spoilt = valid + 8 * 16, slot = spoilt + 8 * 16, swap = slot + 16, total = swap + 2 * 256 * 4 + 1024;
 };
 // mbarriers
-enum { kQFull = 0, kQEmpty, kSFull, kPReady = kSFull + 2, kOFull = kPReady + 2, kKFull = kOFull + 2, kKEmpty = kKFull + 3, kVFull = kKEmpty + 3, kVEmpty = kVFull + 3, kTcBars = kVEmpty + 3 };
+enum { kQFull = 0, kQEmpty, kSFull, kPReady = kSFull + 2, kOFull = kPReady + 2, kKFull = kOFull + 2, kKEmpty = kKFull + 3, kVFull = kKEmpty + 3, kVEmpty = kVFull + 3, kRaw = kVEmpty + 3, kDone = kRaw + kTcProducers, kTcBars };
 static_assert(kTcBars * 8 <= 256, "");
 
 template <typename T, int DK, int DV>
@@ -976,7 +978,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
     extern __shared__ unsigned char sm_raw[];
     unsigned char* sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::bars);
-    uint32_t* valid = reinterpret_cast<uint32_t*>(sm + S::valid);            // [4][4]: which keys a tile has
+    uint32_t* valid = reinterpret_cast<uint32_t*>(sm + S::valid);            // [8][4]: which keys a tile has
     uint32_t* spoilt = reinterpret_cast<uint32_t*>(sm + S::spoilt);          // [8][4]: drafts with values that are not finite
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + S::slot);
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
@@ -984,9 +986,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
         mbar_init(bars + kQFull, kTcProducers); mbar_init(bars + kQEmpty, 1);
         for (int i = 0; i < 2; ++i) { mbar_init(bars + kSFull + i, 1); mbar_init(bars + kPReady + i, 128); mbar_init(bars + kOFull + i, 1); }
         for (int i = 0; i < ST; ++i) {
-            mbar_init(bars + kKFull + i, kTcProducers); mbar_init(bars + kKEmpty + i, 1);
-            mbar_init(bars + kVFull + i, kTcProducers); mbar_init(bars + kVEmpty + i, 1);
+            mbar_init(bars + kKFull + i, 1); mbar_init(bars + kKEmpty + i, 1);
+            mbar_init(bars + kVFull + i, 1); mbar_init(bars + kVEmpty + i, 1);
         }
+        for (int i = 0; i < kTcProducers; ++i) mbar_init(bars + kRaw + i, 1);
+        mbar_init(bars + kDone, 1);
         fence_barrier_init();
     }
     if (tid < 32) spoilt[tid] = 0;
@@ -1012,151 +1016,153 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
     auto two_halves = [&](const Place& pl) { return p.N * p.G - (pl.unit - head_of(p, pl.unit) * p.row_tiles) * p.rows > 128 && p.rows > 128; };
 
     if (w >= kTcCopy) {
-        // ---- copies
+        // ---- copies: a warp to a stage (a warp that came to a stage's next tile but one would take the phase before it for its own)
         constexpr int KL = DK / 8, VL = DV / 8;
         const uint32_t base = smem_u32(sm);
-        int g = 0, unit_no = 0;
-        int done = 0;
+        const int cw = w - kTcCopy;
+        int g = 0, unit_no = 0, done = 0;
+        uint32_t raws = 0;
+        int last = -1;
         // where lane's piece of row r goes within a 128-row operand: 64 columns to a block of 128-byte rows, 16-byte pieces swizzled by the row
         auto place_of = [&](int r, int c) { return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
-        // This warp's slices of sixteen keys of a tile, w - 9, w - 6 and w - 3.  Sixteen cached tokens of one page are a box of the tensor maps
-        // (page >= 0, from token in of the page); of others (a sequence's end, drafts, small pages) lane x (and x + 16) knows the rows of key x.
-        struct Rows {
-            const char *k[3], *v[3];
-            uint32_t m[3];
-            int page[3], in[3];
-            bool any;
-        };
-        Rows ahead;
-        auto look = [&](Rows& r, const Place& pl, int j, int) {
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                const int sl = w - kTcCopy + i * kTcProducers, pos = (pl.tile + j) * kTcTile + sl * 16;
-                r.page[i] = -1;
-                r.in[i] = 0;
-                if (p.boxes && sl < 8 && pl.tile + j < pl.tiles - p.draft_tiles && pos + 16 <= pl.len) {
-                    const int no = (int)p.page.div((uint32_t)pos);
-                    r.in[i] = pos - no * (int)p.page.d;
-                    r.page[i] = __ldg(p.table + (int64_t)pl.b * p.table_stride + no);
-                }
-            }
-        };
-        auto find_rows = [&](Rows& r, const Place& pl, int kv, int tile) {
-            r.any = false;
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                const int sl = w - kTcCopy + i * kTcProducers;
-                r.m[i] = 0;
-                if (r.page[i] >= 0 && r.page[i] < p.pages) { r.m[i] = 0xffffu; continue; }
-                r.page[i] = -1;
-                if (sl >= 8) continue;
-                const char *k = p.q, *v = p.q;
-                const bool on = key_row(p, Place{pl.b, pl.unit, tile, pl.tiles, pl.len}, kv, sl * 16 + (lane & 15), k, v, &bad);
-                r.k[i] = k; r.v[i] = v;
-                r.m[i] = __ballot_sync(0xffffffffu, on) & 0xffffu;
-                r.any = true;
-            }
-        };
-        // one operand of a tile; draft >= 0: values of drafts, noted in that line of `spoilt`
-        auto copy = [&](const CUtensorMap& map, int full, const Rows& rows, uint32_t dst, auto lanes_, int width, int kv, int draft) {
-            constexpr int lanes = decltype(lanes_)::value, per = 32 / lanes;
-            const bool values = &map == &maps.v;
-            uint32_t bytes = 0;
+        auto tell = [&](int bar, uint32_t bytes) { if (lane == 0) mbar_arrive_expect_tx(bars + bar, bytes); };
+        auto box = [&](const CUtensorMap& map, int blocks, int bar, uint32_t dst, int row, int head, int page) {
+            if (elect_one())
+                for (int blk = 0; blk < blocks; ++blk)
+                    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
+                                     dst + blk * (128 * 128)), "l"(&map), "r"(blk * 64), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bars + bar)) : "memory");
             __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                const int sl = w - kTcCopy + i * kTcProducers;
-                if (rows.page[i] < 0) continue;
-                bytes += 16 * 16 * lanes;
-                if (elect_one())
-#pragma unroll
-                    for (int blk = 0; blk < lanes / 8; ++blk)
-                        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
-                                         dst + blk * (128 * 128) + sl * 2048), "l"(&map), "r"(blk * 64), "r"(rows.in[i]), "r"(kv), "r"(rows.page[i]),
-                                     "r"(smem_u32(bars + full)) : "memory");
-            }
-            if (rows.any) {
-                const int c = lane % lanes;
-#pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    const int sl = w - kTcCopy + i * kTcProducers;
-                    if (sl >= 8 || rows.page[i] >= 0) continue;
-#pragma unroll 4
-                    for (int r = 0; r < 16; r += per) {
-                        const int x = r + lane / lanes;
-                        const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(values ? rows.v[i] : rows.k[i]), x));
-                        const bool on = (rows.m[i] >> x & 1) && c * 8 < width;
-                        cp_async16_or_zero(dst + place_of(sl * 16 + x, c), on ? src + c * 16 : p.q, on);
-                    }
-                }
-                cp_async_commit();
-                cp_async_wait<0>();
-                if (draft >= 0)
-#pragma unroll 1
-                    for (int sl = w - kTcCopy; sl < 8; sl += kTcProducers)
-#pragma unroll 1
-                        for (int r = 0; r < 16; r += per) {
-                            const int x = sl * 16 + r + lane / lanes;
-                            if (take_out<T>(dst + place_of(x, c))) atomicOr(&spoilt[draft * 4 + (x >> 5)], 1u << (x & 31));
-                        }
-                fence_proxy_async();
-                __syncwarp();
-            }
-            if (lane == 0) mbar_arrive_expect_tx(bars + full, bytes);
         };
         while (done < n_tiles) {
             const int piece = min(n_tiles - done, at.tiles - at.tile), cached = at.tiles - p.draft_tiles, kv = head_of(p, at.unit);
-            { bool b = false; draft_length(p, at.b, &b); bad |= b; }
+            if (cw == 0) { bool b = false; draft_length(p, at.b, &b); bad |= b; }
+            const int row0 = (at.unit - kv * p.row_tiles) * p.rows, halves = two_halves(at) ? 2 : 1;
             wait(kQEmpty, (unit_no & 1) ^ 1);
-            const int halves = two_halves(at) ? 2 : 1;
-#pragma unroll 1
-            for (int r0 = (w - kTcCopy) * (32 / KL); r0 < halves * 128; r0 += kTcProducers * (32 / KL)) {
-                const int r = r0 + lane / KL, c = lane % KL;
-                int n, h;
-                const bool on = row_of(p, at.unit, r, n, h) && c * 8 < p.K;
-                cp_async16_or_zero(base + S::q + (r >> 7) * S::qhalf + place_of(r & 127, c), on ? p.q + at.b * p.q_b + n * p.q_n + h * p.q_h + c * 16 : p.q, on);
+            if (p.boxes & 2) {                            // whole drafts to a half: a box of the heads of 128 / G drafts
+                if (cw == 0) {
+                    tell(kQFull, halves * S::qhalf);
+                    for (int i = 0; i < halves; ++i)
+                        box(maps.q, DK / 64, kQFull, base + S::q + i * S::qhalf, kv * p.G, (int)p.group.div((uint32_t)(row0 + i * 128)), at.b);
+                } else {
+                    tell(kQFull, 0);
+                }
+            } else {
+#pragma unroll 2
+                for (int r0 = cw * (32 / KL); r0 < halves * 128; r0 += kTcProducers * (32 / KL)) {
+                    const int r = r0 + lane / KL, c = lane % KL;
+                    int n, h;
+                    const bool on = row_of(p, at.unit, r, n, h) && c * 8 < p.K;
+                    if (r < halves * 128)
+                        cp_async16_or_zero(base + S::q + (r >> 7) * S::qhalf + place_of(r & 127, c), on ? p.q + at.b * p.q_b + n * p.q_n + h * p.q_h + c * 16 : p.q, on);
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                fence_proxy_async();
+                __syncwarp();
+                tell(kQFull, 0);
             }
-            cp_async_commit();
-            // Keys run one tile ahead of values: their stage is free as soon as the scores are there.
-            Rows now, next;
-            look(now, at, 0, piece);
-            find_rows(now, at, kv, at.tile);
-            for (int j = -1; j < piece; ++j) {
-                if (j + 1 < piece) {
-                    if (j >= 0) next = ahead;
-                    Rows& r = j >= 0 ? next : now;
-                    if (j >= 0) find_rows(r, at, kv, at.tile + j + 1);
-                    if (j + 2 < piece) look(ahead, at, j + 2, piece);
-                    const int t = g + j + 1, st = t % ST;
-                    wait(kKEmpty + st, ((uint32_t)(t / ST) & 1u) ^ 1u);
-                    // (the words of the tile four before are no longer read: the products after it are done, or this stage would not be empty)
-                    if (lane == 0)
+            int j = cw < ST ? (cw + ST - g % ST) % ST : piece;
+            int looked = -1, page = -1;                   // lane i < 8: the page of slice i of the next tile
+            auto look = [&](int tile) {
+                const int pos = tile * kTcTile + (lane & 7) * 16;
+                looked = tile;
+                page = tile < cached && pos < at.len ? __ldg(p.table + (int64_t)at.b * p.table_stride + p.page.div((uint32_t)pos)) : -1;
+            };
+            for (; j < piece; j += ST) {
+                const int t = g + j, tile = at.tile + j, st = t % ST;
+                const uint32_t ph = ((uint32_t)(t / ST) & 1u) ^ 1u;
+                const bool draft = tile >= cached;
+                const int n0 = (tile - cached) * kTcTile;
+                if (looked != tile) look(tile);
+                // Slices of sixteen keys that are one box of a tensor map: sixteen cached tokens of a page, or sixteen drafts.
+                const int pos = tile * kTcTile + (lane & 7) * 16, in = pos - (int)(p.page.div((uint32_t)pos) * p.page.d);
+                bool whole16;
+                if (!draft) {
+                    whole16 = (p.boxes & 1) && pos + 16 <= at.len && page >= 0 && page < p.pages;
+                } else {
+                    whole16 = (p.boxes & 4) && n0 + (lane & 7) * 16 + 16 <= p.N;
+                    if (whole16 && p.parents)
+                        for (int i = 0; i < 16; ++i) whole16 &= is_draft(p, at.b, n0 + (lane & 7) * 16 + i);
+                }
+                const uint32_t boxes = __ballot_sync(0xffffffffu, whole16) & 0xffu;
+                // others, row by row: which keys there are
+                uint32_t words[4];
 #pragma unroll
-                        for (int i = 0; i < 3; ++i) {
-                            const int sl = w - kTcCopy + i * kTcProducers;
-                            if (sl < 8) reinterpret_cast<uint16_t*>(valid + (t & 3) * 4)[sl] = (uint16_t)r.m[i];
+                for (int i = 0; i < 4; ++i) {
+                    words[i] = ((boxes >> (2 * i) & 1) ? 0xffffu : 0u) | ((boxes >> (2 * i + 1) & 1) ? 0xffff0000u : 0u);
+                    if (words[i] == 0xffffffffu) continue;
+                    const char *k = p.q, *v = p.q;
+                    words[i] = __ballot_sync(0xffffffffu, key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, i * 32 + lane, k, v, &bad));
+                }
+                // values: 1 where unread drafts may hold anything, and the tile has to be looked through
+                auto copy = [&](bool values) {
+                    const uint32_t dst = base + (values ? S::v + st * S::vst : S::k + st * S::kst);
+                    const int lanes = values ? VL : KL, full = (values ? kVFull : kKFull) + st, width = values ? p.V : p.K;
+                    const CUtensorMap& map = draft ? (values ? maps.dv : maps.dk) : (values ? maps.v : maps.k);
+                    // (a chain's drafts are read by all rows up to the first row's)
+                    const bool look_through = values && draft && (p.parents || n0 + kTcTile - 1 > (int)p.group.div((uint32_t)row0));
+                    const int bar = look_through ? kRaw + cw : full;
+                    const uint32_t bytes = (uint32_t)__popc(boxes) * 256u * lanes;
+                    if (look_through || boxes == 0xffu) tell(bar, bytes);
+#pragma unroll 1
+                    for (int sl = 0; sl < 8; ++sl) {
+                        const int pg = __shfl_sync(0xffffffffu, page, sl), i = __shfl_sync(0xffffffffu, in, sl);
+                        if (boxes >> sl & 1) box(map, lanes / 8, bar, dst + sl * 2048, draft ? n0 + sl * 16 : i, kv, draft ? at.b : pg);
+                    }
+                    if (boxes != 0xffu) {
+                        const int per = 32 / lanes, c = lane % lanes;
+#pragma unroll 1
+                        for (int q = 0; q < 4; ++q) {     // 32 keys, a lane each
+                            if ((boxes >> (2 * q) & 3u) == 3u) continue;
+                            const char *k = p.q, *v = p.q;
+                            bool dull = false;
+                            key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, q * 32 + lane, k, v, &dull);
+                            const unsigned long long own = reinterpret_cast<unsigned long long>(values ? v : k);
+#pragma unroll 4
+                            for (int r = 0; r < 32; r += per) {
+                                const int x = r + lane / lanes;
+                                const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, own, x));
+                                const bool on = (words[q] >> x & 1) && c * 8 < width;
+                                if (!(boxes >> (2 * q + (x >> 4)) & 1)) cp_async16_or_zero(dst + place_of(q * 32 + x, c), on ? src + c * 16 : p.q, on);
+                            }
                         }
-                    copy(maps.k, kKFull + st, r, base + S::k + st * S::kst, std::integral_constant<int, KL>{}, p.K, kv, -1);
-                    if (j < 0) {
+                        cp_async_commit();
                         cp_async_wait<0>();
+                    }
+                    if (look_through) {
+                        wait(bar, raws++ & 1u);
+                        __syncwarp();
+#pragma unroll 2
+                        for (int x = lane; x < kTcTile * lanes; x += 32)
+                            if (take_out<T>(dst + place_of(x / lanes, x % lanes))) atomicOr(&spoilt[(t & 7) * 4 + (x / lanes >> 5)], 1u << (x / lanes & 31));
+                    }
+                    if (look_through || boxes != 0xffu) {
                         fence_proxy_async();
                         __syncwarp();
-                        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bars + kQFull)) : "memory");
+                        tell(full, look_through ? 0 : bytes);
                     }
-                }
-                if (j >= 0) {
-                    const int t = g + j, st = t % ST;
-                    wait(kVEmpty + st, ((uint32_t)(t / ST) & 1u) ^ 1u);
-                    if (w == kTcCopy && lane < 4) spoilt[((t - ST) & 7) * 4 + lane] = 0;
-                    copy(maps.v, kVFull + st, now, base + S::v + st * S::vst, std::integral_constant<int, VL>{}, p.V, kv, at.tile + j >= cached ? t & 7 : -1);
-                    now = next;
-                }
+                };
+                wait(kKEmpty + st, ph);
+                if (lane == 0)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) valid[(t & 7) * 4 + i] = words[i];
+                copy(false);
+                wait(kVEmpty + st, ph);
+                if (lane < 4) spoilt[(t & 7) * 4 + lane] = 0;
+                __syncwarp();
+                copy(true);
+                if (j + ST < piece) look(tile + ST);
+                last = t;
             }
             g += piece;
             done += piece;
             ++unit_no;
             at.tile += piece - 1;
             at.next(p);
+        }
+        if (last >= 0) {                                  // whatever happened: nothing is in flight when the block ends
+            late |= !mbar_wait_bounded(bars + kKFull + last % ST, (uint32_t)(last / ST) & 1u, kTcWaitCap);
+            late |= !mbar_wait_bounded(bars + kVFull + last % ST, (uint32_t)(last / ST) & 1u, kTcWaitCap);
         }
     } else if (w == kTcMma) {
         // ---- products
@@ -1194,6 +1200,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 wait(kQFull, unit_no & 1);
                 scores(0);
                 if (jobs > 1) scores(1);
+                if (jobs <= 2) tc_commit(bars + kQEmpty);
                 for (int i = 0; i < jobs; ++i) {
                     const int half = i & 1, t = g + (i >> two), st = t % ST;
                     if (!two || !half) wait(kVFull + st, (uint32_t)(t / ST) & 1u);
@@ -1203,15 +1210,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                     if (i + 2 >= jobs) tc_commit(bars + kOFull + half);
                     if (!two || half) tc_commit(bars + kVEmpty + st);
                     if (i + 2 < jobs) scores(i + 2);
+                    if (i + 3 == jobs) tc_commit(bars + kQEmpty);
                 }
-                tc_commit(bars + kQEmpty);
                 g += piece;
                 done += piece;
                 ++unit_no;
                 at.tile += piece - 1;
                 at.next(p);
             }
-            wait(kQEmpty, (unit_no - 1) & 1);             // all products are done
+            tc_commit(bars + kDone);
+            late |= !mbar_wait_bounded(bars + kDone, 0, kTcWaitCap);          // all products are done
         }
         __syncwarp();
     } else {
@@ -1244,7 +1252,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 tc_ld16(x[0], ts);
                 uint32_t seen[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) seen[c] = valid[(gg & 3) * 4 + c];
+                for (int c = 0; c < 4; ++c) seen[c] = valid[(gg & 7) * 4 + c];
                 if (tile >= cached) {
                     const int tile0 = (tile - cached) * kTcTile;
                     const uint64_t lo = on ? draft_mask(p, at.b, n, tile0, &bad) : 0ull, hi = on ? draft_mask(p, at.b, n, tile0 + 64, &bad) : 0ull;
@@ -1440,77 +1448,98 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
 // ---- joining the parts -------------------------------------------------------------------------------------------------------
 
 // A task is the rows of a unit that several parts have left; by unit, or, where there are more units than parts, by the part that starts and
-// does not finish it.  A team of 1 to 8 warps joins a row (as many parts as a unit has on average, about four to a warp).
-constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
-template <typename T>
+// does not finish it.  A team of 1 to 8 warps joins a row (as many parts as a unit has on average, about four to a warp); a team of one
+// takes kJoinRows rows, whose loads it has in flight together.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinRows = 4;
+template <typename T, int R>
 __global__ void __launch_bounds__(kJoinThreads) draft_join_kernel(const __grid_constant__ DraftParams p) {
     __shared__ float red[kJoinWarps][256], wl[kJoinWarps];
     chain_enter();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, team = w / p.team, member = w - team * p.team;
     const int4 task = p.tasks[blockIdx.x];
     if (task.x < 0) return;
-    const int slots = task.w >> 1, r = blockIdx.y * (kJoinWarps / p.team) + team;
+    const int slots = task.w >> 1, r0 = (blockIdx.y * (kJoinWarps / p.team) + team) * R;
     const int64_t size = (int64_t)p.rows * (p.V + 2);
     const float* slot0 = p.part + 2 * (int64_t)task.z * size;
     const int64_t in_first = (task.w & 1) ? size : 0;
     auto slot_of = [&](int i) { return slot0 + (i == 0 ? in_first : 2 * i * size); };
-    int n = 0, h = 0;
-    const bool on = r < p.rows && row_of(p, task.y, r, n, h);
-    float top = -INFINITY, mass = 0.f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};      // columns lane*4 and lane*4 + 128
-    if (on) {
-        for (int i = lane; i < slots; i += 32) top = fmaxf(top, slot_of(i)[p.rows * p.V + 2 * r]);
-        top = warp_max(top);
-        const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-        for (int i = member; i < slots; i += p.team) {
-            const float* s = slot_of(i);
-            const float2 rm = *reinterpret_cast<const float2*>(s + p.rows * p.V + 2 * r);
-            float4 x[2];
+    float top[R], mass[R], o[R][8];                      // columns lane*4 and lane*4 + 128
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        top[k] = -INFINITY;
+        mass[k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[k][i] = 0.f;
+    }
+    // (rows behind the unit's last are whatever is there, and not written)
+    for (int i = lane; i < slots; i += 32)
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+            if (r0 + k < p.rows) top[k] = fmaxf(top[k], slot_of(i)[p.rows * p.V + 2 * (r0 + k)]);
+#pragma unroll
+    for (int k = 0; k < R; ++k) top[k] = warp_max(top[k]);
+#pragma unroll(R == 1 ? 4 : 2)
+    for (int i = member; i < slots; i += p.team) {
+        const float* s = slot_of(i);
+        float2 rm[R];
+        float4 x[R][2];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const int r = min(r0 + k, p.rows - 1);
+            rm[k] = *reinterpret_cast<const float2*>(s + p.rows * p.V + 2 * r);
 #pragma unroll
             for (int half = 0; half < 2; ++half)
-                x[half] = half * 128 + lane * 4 < p.V ? *reinterpret_cast<const float4*>(s + r * p.V + half * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float f = exp2f(rm.x - ref);
-            mass = fmaf(f, rm.y, mass);
+                x[k][half] = half * 128 + lane * 4 < p.V ? *reinterpret_cast<const float4*>(s + r * p.V + half * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const float f = exp2f(rm[k].x - (top[k] == -INFINITY ? 0.f : top[k]));
+            mass[k] = fmaf(f, rm[k].y, mass[k]);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                o[4 * half] = fmaf(f, x[half].x, o[4 * half]);
-                o[4 * half + 1] = fmaf(f, x[half].y, o[4 * half + 1]);
-                o[4 * half + 2] = fmaf(f, x[half].z, o[4 * half + 2]);
-                o[4 * half + 3] = fmaf(f, x[half].w, o[4 * half + 3]);
+                o[k][4 * half] = fmaf(f, x[k][half].x, o[k][4 * half]);
+                o[k][4 * half + 1] = fmaf(f, x[k][half].y, o[k][4 * half + 1]);
+                o[k][4 * half + 2] = fmaf(f, x[k][half].z, o[k][4 * half + 2]);
+                o[k][4 * half + 3] = fmaf(f, x[k][half].w, o[k][4 * half + 3]);
             }
         }
     }
-    if (p.team > 1) {
+    if (R == 1 && p.team > 1) {
 #pragma unroll
         for (int half = 0; half < 2; ++half)
-            if (half * 128 < p.V) *reinterpret_cast<float4*>(&red[w][half * 128 + lane * 4]) = make_float4(o[4 * half], o[4 * half + 1], o[4 * half + 2], o[4 * half + 3]);
-        if (lane == 0) wl[w] = mass;
+            if (half * 128 < p.V)
+                *reinterpret_cast<float4*>(&red[w][half * 128 + lane * 4]) = make_float4(o[0][4 * half], o[0][4 * half + 1], o[0][4 * half + 2], o[0][4 * half + 3]);
+        if (lane == 0) wl[w] = mass[0];
         __syncthreads();
         if (member > 0) return;
         for (int i = 1; i < p.team; ++i) {
-            mass += wl[w + i];
+            mass[0] += wl[w + i];
 #pragma unroll
             for (int half = 0; half < 2; ++half)
                 if (half * 128 < p.V) {
                     const float4 x = *reinterpret_cast<const float4*>(&red[w + i][half * 128 + lane * 4]);
-                    o[4 * half] += x.x; o[4 * half + 1] += x.y; o[4 * half + 2] += x.z; o[4 * half + 3] += x.w;
+                    o[0][4 * half] += x.x; o[0][4 * half + 1] += x.y; o[0][4 * half + 2] += x.z; o[0][4 * half + 3] += x.w;
                 }
         }
     }
-    if (!on) return;
-    const bool real = is_draft(p, task.x, n);
-    const int64_t row = ((int64_t)task.x * p.N + n) * p.H + h;
-    const float inv = finish_scale(mass);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const int col = (i >> 2) * 128 + lane * 4 + (i & 3);
-        if (col >= p.V) continue;
-        const float a = real ? o[i] * inv : 0.f, b = real ? o[i + 1] * inv : 0.f;
-        T* to = reinterpret_cast<T*>(p.out) + row * p.V + col;
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to) = make_float2(a, b);
-        else *reinterpret_cast<uint32_t*>(to) = Frag<T>::pack(a, b);
+    for (int k = 0; k < R; ++k) {
+        int n, h;
+        if (r0 + k >= p.rows || !row_of(p, task.y, r0 + k, n, h)) continue;
+        const bool real = is_draft(p, task.x, n);
+        const int64_t row = ((int64_t)task.x * p.N + n) * p.H + h;
+        const float inv = finish_scale(mass[k]);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const int col = (i >> 2) * 128 + lane * 4 + (i & 3);
+            if (col >= p.V) continue;
+            const float a = real ? o[k][i] * inv : 0.f, b = real ? o[k][i + 1] * inv : 0.f;
+            T* to = reinterpret_cast<T*>(p.out) + row * p.V + col;
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to) = make_float2(a, b);
+            else *reinterpret_cast<uint32_t*>(to) = Frag<T>::pack(a, b);
+        }
+        if (p.lse && lane == 0) p.lse[row] = real ? finish_lse(top[k], mass[k]) : -INFINITY;
     }
-    if (p.lse && lane == 0) p.lse[row] = real ? finish_lse(top, mass) : -INFINITY;
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------
@@ -1554,8 +1583,10 @@ static void choose(DraftParams& p, int dtype) {
     if (p.c < 1.1754944e-38f) p.c = 1.1754944e-38f;        // a scale of zero: scores of zero, but what is masked stays minus infinity
 }
 
-// The tensor map of a cache; false where its strides are none that a map can have (an expanded dimension), or the driver has no such call.
-static bool cache_map(CUtensorMap& map, const char* base, int width, int64_t row, int64_t head, int64_t page, const DraftParams& p, bool bf16) {
+// A tensor map over three dimensions of rows; false where the strides are none that a map can have (an expanded dimension), or the driver has
+// no such call.
+struct MapDim { int64_t size, stride; uint32_t box; };
+static bool row_map(CUtensorMap& map, const char* base, int width, const MapDim (&d)[3], bool bf16) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static const Encode encode = [] {
@@ -1567,14 +1598,29 @@ static bool cache_map(CUtensorMap& map, const char* base, int width, int64_t row
         }
         return reinterpret_cast<Encode>(f);
     }();
-    const cuuint64_t dims[4] = {(cuuint64_t)width, p.page.d, (cuuint64_t)p.Hkv, (cuuint64_t)p.pages};
-    // (the stride of a dimension of one element is never used, but has to be one)
-    const cuuint64_t strides[3] = {(cuuint64_t)(p.page.d > 1 ? row : 16), (cuuint64_t)(p.Hkv > 1 ? head : 16), (cuuint64_t)(p.pages > 1 ? page : 16)};
-    const cuuint32_t box[4] = {64, 16, 1, 1}, ones[4] = {1, 1, 1, 1};
-    for (const cuuint64_t x : strides) if (x == 0 || x >= (cuuint64_t(1) << 40)) return false;
+    cuuint64_t dims[4] = {(cuuint64_t)width, 0, 0, 0}, strides[3];
+    cuuint32_t box[4] = {64, 0, 0, 0};
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 3; ++i) {
+        dims[i + 1] = (cuuint64_t)d[i].size;
+        strides[i] = (cuuint64_t)(d[i].size > 1 ? d[i].stride : 16);       // (of one element it is never used, but has to be one)
+        box[i + 1] = d[i].box;
+        if (strides[i] == 0 || strides[i] >= (cuuint64_t(1) << 40) || dims[i + 1] > (cuuint64_t(1) << 32) || box[i + 1] > 256) return false;
+    }
     return encode && encode(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<char*>(base), dims, strides, box, ones,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+static int tc_maps(TcMaps& m, const DraftParams& p, bool bf16) {
+    int boxes = 0;
+    if (p.page.d % 16 == 0 && row_map(m.k, p.ck, p.K, {{(int64_t)p.page.d, p.ck_row, 16}, {p.Hkv, p.ck_h, 1}, {p.pages, p.ck_page, 1}}, bf16) &&
+        row_map(m.v, p.cv, p.V, {{(int64_t)p.page.d, p.cv_row, 16}, {p.Hkv, p.cv_h, 1}, {p.pages, p.cv_page, 1}}, bf16))
+        boxes |= 1;
+    if (128 % p.G == 0 && row_map(m.q, p.q, p.K, {{p.H, p.q_h, (uint32_t)p.G}, {p.N, p.q_n, (uint32_t)(128 / p.G)}, {p.B, p.q_b, 1}}, bf16)) boxes |= 2;
+    if (p.N >= 16 && row_map(m.dk, p.k, p.K, {{p.N, p.k_n, 16}, {p.Hkv, p.k_h, 1}, {p.B, p.k_b, 1}}, bf16) &&
+        row_map(m.dv, p.v, p.V, {{p.N, p.v_n, 16}, {p.Hkv, p.v_h, 1}, {p.B, p.v_b, 1}}, bf16))
+        boxes |= 4;
+    return boxes;
 }
 
 template <typename T, int DK, int DV, int RM>
@@ -1591,8 +1637,7 @@ static int launch_mma(const DraftParams& p, cudaStream_t st) {
         if (const cudaError_t e = limit.raise((const void*)draft_tc_kernel<T, DK, DV>, TcShape<DK, DV>::total)) return (int)e;
         TcMaps maps{};
         DraftParams q = p;
-        q.boxes = p.page.d % 16 == 0 && cache_map(maps.k, p.ck, p.K, p.ck_row, p.ck_h, p.ck_page, p, std::is_same<T, __nv_bfloat16>::value) &&
-                  cache_map(maps.v, p.cv, p.V, p.cv_row, p.cv_h, p.cv_page, p, std::is_same<T, __nv_bfloat16>::value);
+        q.boxes = tc_maps(maps, p, std::is_same<T, __nv_bfloat16>::value);
         return launch_chained(draft_tc_kernel<T, DK, DV>, dim3(p.grid), dim3(kTcThreads), TcShape<DK, DV>::total, st, q, maps);
     }
     return p.variant == kMma16 ? launch_mma<T, DK, DV, 1>(p, st) : launch_mma<T, DK, DV, 2>(p, st);
@@ -1621,9 +1666,11 @@ static int launch_draft(const DraftParams& p, cudaStream_t st) {
                        : (p.V <= 64 ? launch_mma<T, 128, 64>(p, st) : launch_mma<T, 128, 128>(p, st));
     }
     if (rc) return rc;
-    const int rows = p.N * p.G < p.rows ? p.N * p.G : p.rows, block = kJoinWarps / p.team;
+    const bool alone = p.team == 1;
+    const int rows = p.N * p.G < p.rows ? p.N * p.G : p.rows, block = kJoinWarps / p.team * (alone ? kJoinRows : 1);
     const dim3 grid(p.by_unit ? (unsigned)units_of(p) : (unsigned)p.grid, (rows + block - 1) / block);
-    return launch_chained(draft_join_kernel<T>, grid, dim3(kJoinThreads), 0, st, p);
+    return alone ? launch_chained(draft_join_kernel<T, kJoinRows>, grid, dim3(kJoinThreads), 0, st, p)
+                 : launch_chained(draft_join_kernel<T, 1>, grid, dim3(kJoinThreads), 0, st, p);
 }
 
 static int fill_draft(DraftParams& p, const HtreeCache* c, const HtreeDrafts* d) {
