@@ -39,6 +39,7 @@ struct DraftParams {
     int32_t grid, least, by_unit, team;                                    // parts at most; tiles of a part at least; how tasks are indexed, and joined
     int32_t variant;          // which kernel (choose)
     int32_t boxes;            // tcgen05 kernel: what comes by tensor maps: 1 pages of whole slices of sixteen tokens, 2 q, 4 drafts
+    int32_t box_rows;         // tokens of a box of a whole tile: as many as pages allow, up to the tile
     int32_t neg;              // tensor-core kernels: the scale is negative, c its magnitude and q's signs are turned
     float c;                  // scale * log2 e
     FastDiv page, group, per_head;      // by the page size, by G, by row_tiles
@@ -873,8 +874,8 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
 // of tensor memory): S = Q K^T (operands in shared memory, accumulator in tensor memory), P = 2^(cS - reference) by a thread a row, written
 // over S in 16 bits, O += P V with P read from tensor memory.  Two halves with an S and an O of their own take turns, so that one's softmax
 // runs beside the other's products: with more than 128 rows each has 128 of them and all tiles, with fewer both have the same rows and
-// every other tile, and are joined at the end.  Tensor memory: S and O of each half, 128 columns each; shared memory: Q (64 KB), two stages
-// each of K and V (32 KB).  Roles: warps 0-3 and 4-7 the softmax of a half, 8 the products, 9-11 the copies.
+// every other tile, and are joined at the end.  Tensor memory: S and O of each half, 128 columns each; shared memory: Q (64 KB), three
+// stages of K and two of V (32 KB).  Roles: warps 0-3 and 4-7 the softmax of a half, 8 the products, 9-11 the copies.
 // At 256 rows of 128 a tile is 16.8 MFLOP, 2048 cycles of the tensor pipe, and 32768 exponentials, 2048 cycles of the special function
 // units: the two bound it alike, HBM (64 KB a tile) does below about 250 rows.
 // A row's weights in a tile may sum to kTcMost before the reference follows (a maximum per tile costs a fifth of the softmax; the sum is there
@@ -958,13 +959,14 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* x) {
 
 // The caches as [page][head][token][element] and the drafts' k, v as [request][head][draft][element], boxes of 16 tokens and 128 bytes; q as
 // [request][draft][head][element], boxes of a group's heads of 128 / G drafts.
-struct TcMaps { CUtensorMap k, v, dk, dv, q; };
+struct TcMaps { CUtensorMap k, v, kb, vb, dk, dv, q; };      // kb, vb: boxes of box_rows tokens
 
 template <int DK, int DV> struct TcShape {
     static constexpr int kst = kTcTile * DK * 2, vst = kTcTile * DV * 2, qhalf = 128 * DK * 2;
-    static constexpr int stages = DK + DV > 192 ? 2 : 3;
-    static constexpr int q = 0, k = 2 * qhalf, v = k + stages * kst, end = v + stages * vst;
-    static constexpr int bars = end, valid = bars + 256, spoilt = valid + 8 * 16, slot = spoilt + 8 * 16, swap = slot + 16, total = swap + 2 * 256 * 4 + 1024;
+    static constexpr int vstages = DK + DV > 192 ? 2 : 3, kstages = 3;
+    static constexpr int q = 0, k = 2 * qhalf, v = k + kstages * kst, end = v + vstages * vst;
+    static constexpr int bars = end, valid = bars + 256, spoilt = valid + 8 * 16, slot = spoilt + 8 * 16, swap = slot + 16, total = swap + 128 * 8 + 1024;
+    static_assert(total + 128 <= 232448, "");
 };
 // mbarriers
 enum { kQFull = 0, kQEmpty, kSFull, kPReady = kSFull + 2, kOFull = kPReady + 2, kKFull = kOFull + 2, kKEmpty = kKFull + 3, kVFull = kKEmpty + 3, kVEmpty = kVFull + 3, kRaw = kVEmpty + 3, kDone = kRaw + kTcProducers, kTcBars };
@@ -973,7 +975,7 @@ static_assert(kTcBars * 8 <= 256, "");
 template <typename T, int DK, int DV>
 __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_constant__ DraftParams p, const __grid_constant__ TcMaps maps) {
     using S = TcShape<DK, DV>;
-    constexpr int ST = S::stages;
+    constexpr int KS = S::kstages, VS = S::vstages;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ unsigned char sm_raw[];
     unsigned char* sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
@@ -985,7 +987,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
     if (tid == 0) {
         mbar_init(bars + kQFull, kTcProducers); mbar_init(bars + kQEmpty, 1);
         for (int i = 0; i < 2; ++i) { mbar_init(bars + kSFull + i, 1); mbar_init(bars + kPReady + i, 128); mbar_init(bars + kOFull + i, 1); }
-        for (int i = 0; i < ST; ++i) {
+        for (int i = 0; i < 3; ++i) {
             mbar_init(bars + kKFull + i, 1); mbar_init(bars + kKEmpty + i, 1);
             mbar_init(bars + kVFull + i, 1); mbar_init(bars + kVEmpty + i, 1);
         }
@@ -1016,7 +1018,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
     auto two_halves = [&](const Place& pl) { return p.N * p.G - (pl.unit - head_of(p, pl.unit) * p.row_tiles) * p.rows > 128 && p.rows > 128; };
 
     if (w >= kTcCopy) {
-        // ---- copies: a warp to a stage (a warp that came to a stage's next tile but one would take the phase before it for its own)
+        // ---- copies.  (No warp may come to a stage's next tile but one before the next is done with: it would take the phase before for its own.)
         constexpr int KL = DK / 8, VL = DV / 8;
         const uint32_t base = smem_u32(sm);
         const int cw = w - kTcCopy;
@@ -1061,16 +1063,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 __syncwarp();
                 tell(kQFull, 0);
             }
-            int j = cw < ST ? (cw + ST - g % ST) % ST : piece;
+            // warp 0 the keys, in order; warps 1 and 2 the values of even and odd tiles
+            const bool values = cw > 0;
+            int j = values ? (cw - 1 + g) & 1 : 0;
+            const int jstep = values ? 2 : 1, lanes = values ? VL : KL, width = values ? p.V : p.K;
             int looked = -1, page = -1;                   // lane i < 8: the page of slice i of the next tile
             auto look = [&](int tile) {
                 const int pos = tile * kTcTile + (lane & 7) * 16;
                 looked = tile;
                 page = tile < cached && pos < at.len ? __ldg(p.table + (int64_t)at.b * p.table_stride + p.page.div((uint32_t)pos)) : -1;
             };
-            for (; j < piece; j += ST) {
-                const int t = g + j, tile = at.tile + j, st = t % ST;
-                const uint32_t ph = ((uint32_t)(t / ST) & 1u) ^ 1u;
+            for (; j < piece; j += jstep) {
+                const int t = g + j, tile = at.tile + j, st = values ? t % VS : t % KS, turn = values ? t / VS : t / KS;
+                const int full = (values ? kVFull : kKFull) + st, empty = (values ? kVEmpty : kKEmpty) + st;
+                const uint32_t dst = base + (values ? S::v + st * S::vst : S::k + st * S::kst);
                 const bool draft = tile >= cached;
                 const int n0 = (tile - cached) * kTcTile;
                 if (looked != tile) look(tile);
@@ -1086,72 +1092,73 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 }
                 const uint32_t boxes = __ballot_sync(0xffffffffu, whole16) & 0xffu;
                 // others, row by row: which keys there are
-                uint32_t words[4];
+                uint32_t words[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+                if (boxes != 0xffu) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    words[i] = ((boxes >> (2 * i) & 1) ? 0xffffu : 0u) | ((boxes >> (2 * i + 1) & 1) ? 0xffff0000u : 0u);
-                    if (words[i] == 0xffffffffu) continue;
-                    const char *k = p.q, *v = p.q;
-                    words[i] = __ballot_sync(0xffffffffu, key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, i * 32 + lane, k, v, &bad));
+                    for (int i = 0; i < 4; ++i) {
+                        const char *kk = p.q, *vv = p.q;
+                        words[i] = __ballot_sync(0xffffffffu, key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, i * 32 + lane, kk, vv, &bad));
+                    }
                 }
-                // values: 1 where unread drafts may hold anything, and the tile has to be looked through
-                auto copy = [&](bool values) {
-                    const uint32_t dst = base + (values ? S::v + st * S::vst : S::k + st * S::kst);
-                    const int lanes = values ? VL : KL, full = (values ? kVFull : kKFull) + st, width = values ? p.V : p.K;
+                wait(empty, ((uint32_t)turn & 1u) ^ 1u);
+                if (lane < 4) {
+                    if (values) spoilt[(t & 7) * 4 + lane] = 0;
+                    else valid[(t & 7) * 4 + lane] = lane == 0 ? words[0] : lane == 1 ? words[1] : lane == 2 ? words[2] : words[3];
+                }
+                __syncwarp();
+                // (a chain's drafts are read by all rows up to the first row's; others may hold anything, and are looked through)
+                const bool look_through = values && draft && (p.parents || n0 + kTcTile - 1 > (int)p.group.div((uint32_t)row0));
+                const int bar = look_through ? kRaw + cw : full;
+                const uint32_t bytes = (uint32_t)__popc(boxes) * 256u * lanes;
+                if (look_through || boxes == 0xffu) tell(bar, bytes);
+                if (boxes == 0xffu && !draft && p.box_rows > 16) {
+#pragma unroll 1
+                    for (int r = 0; r < kTcTile; r += p.box_rows) {
+                        const int pg = __shfl_sync(0xffffffffu, page, r >> 4), i = __shfl_sync(0xffffffffu, in, r >> 4);
+                        box(values ? maps.vb : maps.kb, lanes / 8, bar, dst + r * 128, i, kv, pg);
+                    }
+                } else {
                     const CUtensorMap& map = draft ? (values ? maps.dv : maps.dk) : (values ? maps.v : maps.k);
-                    // (a chain's drafts are read by all rows up to the first row's)
-                    const bool look_through = values && draft && (p.parents || n0 + kTcTile - 1 > (int)p.group.div((uint32_t)row0));
-                    const int bar = look_through ? kRaw + cw : full;
-                    const uint32_t bytes = (uint32_t)__popc(boxes) * 256u * lanes;
-                    if (look_through || boxes == 0xffu) tell(bar, bytes);
 #pragma unroll 1
                     for (int sl = 0; sl < 8; ++sl) {
                         const int pg = __shfl_sync(0xffffffffu, page, sl), i = __shfl_sync(0xffffffffu, in, sl);
                         if (boxes >> sl & 1) box(map, lanes / 8, bar, dst + sl * 2048, draft ? n0 + sl * 16 : i, kv, draft ? at.b : pg);
                     }
-                    if (boxes != 0xffu) {
-                        const int per = 32 / lanes, c = lane % lanes;
+                }
+                if (boxes != 0xffu) {
+                    const int per = 32 / lanes, c = lane % lanes;
 #pragma unroll 1
-                        for (int q = 0; q < 4; ++q) {     // 32 keys, a lane each
-                            if ((boxes >> (2 * q) & 3u) == 3u) continue;
-                            const char *k = p.q, *v = p.q;
-                            bool dull = false;
-                            key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, q * 32 + lane, k, v, &dull);
-                            const unsigned long long own = reinterpret_cast<unsigned long long>(values ? v : k);
+                    for (int q = 0; q < 4; ++q) {         // 32 keys, a lane each
+                        if ((boxes >> (2 * q) & 3u) == 3u) continue;
+                        const uint32_t word = q == 0 ? words[0] : q == 1 ? words[1] : q == 2 ? words[2] : words[3];
+                        const char *kk = p.q, *vv = p.q;
+                        bool dull = false;
+                        key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, q * 32 + lane, kk, vv, &dull);
+                        const unsigned long long own = reinterpret_cast<unsigned long long>(values ? vv : kk);
 #pragma unroll 4
-                            for (int r = 0; r < 32; r += per) {
-                                const int x = r + lane / lanes;
-                                const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, own, x));
-                                const bool on = (words[q] >> x & 1) && c * 8 < width;
-                                if (!(boxes >> (2 * q + (x >> 4)) & 1)) cp_async16_or_zero(dst + place_of(q * 32 + x, c), on ? src + c * 16 : p.q, on);
-                            }
+                        for (int r = 0; r < 32; r += per) {
+                            const int x = r + lane / lanes;
+                            const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, own, x));
+                            const bool on = (word >> x & 1) && c * 8 < width;
+                            if (!(boxes >> (2 * q + (x >> 4)) & 1)) cp_async16_or_zero(dst + place_of(q * 32 + x, c), on ? src + c * 16 : p.q, on);
                         }
-                        cp_async_commit();
-                        cp_async_wait<0>();
                     }
-                    if (look_through) {
-                        wait(bar, raws++ & 1u);
-                        __syncwarp();
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                }
+                if (look_through) {
+                    wait(bar, raws++ & 1u);
+                    __syncwarp();
 #pragma unroll 2
-                        for (int x = lane; x < kTcTile * lanes; x += 32)
-                            if (take_out<T>(dst + place_of(x / lanes, x % lanes))) atomicOr(&spoilt[(t & 7) * 4 + (x / lanes >> 5)], 1u << (x / lanes & 31));
-                    }
-                    if (look_through || boxes != 0xffu) {
-                        fence_proxy_async();
-                        __syncwarp();
-                        tell(full, look_through ? 0 : bytes);
-                    }
-                };
-                wait(kKEmpty + st, ph);
-                if (lane == 0)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) valid[(t & 7) * 4 + i] = words[i];
-                copy(false);
-                wait(kVEmpty + st, ph);
-                if (lane < 4) spoilt[(t & 7) * 4 + lane] = 0;
-                __syncwarp();
-                copy(true);
-                if (j + ST < piece) look(tile + ST);
+                    for (int x = lane; x < kTcTile * lanes; x += 32)
+                        if (take_out<T>(dst + place_of(x / lanes, x % lanes))) atomicOr(&spoilt[(t & 7) * 4 + (x / lanes >> 5)], 1u << (x / lanes & 31));
+                }
+                if (look_through || boxes != 0xffu) {
+                    fence_proxy_async();
+                    __syncwarp();
+                    tell(full, look_through ? 0 : bytes);
+                }
+                if (j + jstep < piece) look(tile + jstep);
                 last = t;
             }
             g += piece;
@@ -1161,8 +1168,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
             at.next(p);
         }
         if (last >= 0) {                                  // whatever happened: nothing is in flight when the block ends
-            late |= !mbar_wait_bounded(bars + kKFull + last % ST, (uint32_t)(last / ST) & 1u, kTcWaitCap);
-            late |= !mbar_wait_bounded(bars + kVFull + last % ST, (uint32_t)(last / ST) & 1u, kTcWaitCap);
+            if (cw > 0) late |= !mbar_wait_bounded(bars + kVFull + last % VS, (uint32_t)(last / VS) & 1u, kTcWaitCap);
+            else late |= !mbar_wait_bounded(bars + kKFull + last % KS, (uint32_t)(last / KS) & 1u, kTcWaitCap);
         }
     } else if (w == kTcMma) {
         // ---- products
@@ -1188,9 +1195,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 // job i: half i & 1, tile i / 2 of the unit or (few rows) tile i
                 const int two = two_halves(at) ? 1 : 0, jobs = piece << two;
                 auto scores = [&](int i) {
-                    const int t = g + (i >> two), st = t % ST;
+                    const int t = g + (i >> two), st = t % KS;
                     if (!two || !(i & 1)) {
-                        wait(kKFull + st, (uint32_t)(t / ST) & 1u);
+                        wait(kKFull + st, (uint32_t)(t / KS) & 1u);
                         tc_fence_after();
                     }
                     qk(i & 1, two ? i & 1 : 0, st);
@@ -1202,8 +1209,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 if (jobs > 1) scores(1);
                 if (jobs <= 2) tc_commit(bars + kQEmpty);
                 for (int i = 0; i < jobs; ++i) {
-                    const int half = i & 1, t = g + (i >> two), st = t % ST;
-                    if (!two || !half) wait(kVFull + st, (uint32_t)(t / ST) & 1u);
+                    const int half = i & 1, t = g + (i >> two), st = t % VS;
+                    if (!two || !half) wait(kVFull + st, (uint32_t)(t / VS) & 1u);
                     wait(kPReady + half, (half ? had[1]++ : had[0]++) & 1u);
                     tc_fence_after();
                     pv(half, st);
@@ -1227,7 +1234,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
         const int half = w >> 2, lane_row = (w & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)(w & 3) << 21;   // lane 32 * (w & 3) of tensor memory
         const uint32_t ts = tmem + lanes + half * 128, to = tmem + lanes + 256 + half * 128, to_other = tmem + lanes + 256 + (half ^ 1) * 128;
-        float2* swap = reinterpret_cast<float2*>(sm + S::swap);              // [half][row]: reference, mass
+        float2* swap = reinterpret_cast<float2*>(sm + S::swap) + lane_row;   // reference and mass of a row, of one half at a time
         int g = 0, done = 0;
         uint32_t turns = 0, ends[2] = {0, 0};             // jobs of this half; units that either half had jobs of
         bool first_piece = true;
@@ -1257,7 +1264,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                     const int tile0 = (tile - cached) * kTcTile;
                     const uint64_t lo = on ? draft_mask(p, at.b, n, tile0, &bad) : 0ull, hi = on ? draft_mask(p, at.b, n, tile0 + 64, &bad) : 0ull;
                     seen[0] &= (uint32_t)lo; seen[1] &= (uint32_t)(lo >> 32); seen[2] &= (uint32_t)hi; seen[3] &= (uint32_t)(hi >> 32);
-                    wait(kVFull + gg % ST, (uint32_t)(gg / ST) & 1u);
+                    wait(kVFull + gg % VS, (uint32_t)(gg / VS) & 1u);
                     const uint32_t* sp = spoilt + (gg & 7) * 4;
                     if (sp[0] | sp[1] | sp[2] | sp[3]) {
                         tc_wait_st();
@@ -1361,11 +1368,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
             float f_own = 1.f, f_other = 0.f;
             int c0 = 0, c1 = DV;
             if (!two) {
-                swap[half * 128 + lane_row] = make_float2(empty ? -INFINITY : ref, mass);
                 tc_wait_st();                             // (a half without jobs: its zeros)
                 tc_fence_before();
+                float2 other;
+                const float2 mine = make_float2(empty ? -INFINITY : ref, mass);
+                if (half == 0) *swap = mine;
                 asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");
-                const float2 other = swap[(half ^ 1) * 128 + lane_row];
+                if (half == 1) { other = *swap; *swap = mine; }
+                asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");
+                if (half == 0) other = *swap;
                 const float own = empty ? -INFINITY : ref, t = fmaxf(own, other.x);
                 if (t != -INFINITY) {
                     f_own = ex2_approx(own - t);
@@ -1448,98 +1459,98 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
 // ---- joining the parts -------------------------------------------------------------------------------------------------------
 
 // A task is the rows of a unit that several parts have left; by unit, or, where there are more units than parts, by the part that starts and
-// does not finish it.  A team of 1 to 8 warps joins a row (as many parts as a unit has on average, about four to a warp); a team of one
-// takes kJoinRows rows, whose loads it has in flight together.
-constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinRows = 4;
-template <typename T, int R>
+// does not finish it.  A team of 1 to 8 warps joins a row (as many parts as a unit has on average, about four to a warp), four parts in
+// flight at a time.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+template <typename T, bool Wide>
 __global__ void __launch_bounds__(kJoinThreads) draft_join_kernel(const __grid_constant__ DraftParams p) {
-    __shared__ float red[kJoinWarps][256], wl[kJoinWarps];
+    constexpr int C = Wide ? 2 : 1;                      // columns lane*4 (and + 128)
+    __shared__ float4 red[kJoinWarps][C][32];
+    __shared__ float2 stat[kJoinWarps];
     chain_enter();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, team = w / p.team, member = w - team * p.team;
     const int4 task = p.tasks[blockIdx.x];
     if (task.x < 0) return;
-    const int slots = task.w >> 1, r0 = (blockIdx.y * (kJoinWarps / p.team) + team) * R;
+    const int slots = task.w >> 1, r = blockIdx.y * (kJoinWarps / p.team) + team;
     const int64_t size = (int64_t)p.rows * (p.V + 2);
-    const float* slot0 = p.part + 2 * (int64_t)task.z * size;
-    const int64_t in_first = (task.w & 1) ? size : 0;
-    auto slot_of = [&](int i) { return slot0 + (i == 0 ? in_first : 2 * i * size); };
-    float top[R], mass[R], o[R][8];                      // columns lane*4 and lane*4 + 128
+    int n = 0, h = 0;
+    const bool on = r < p.rows && row_of(p, task.y, r, n, h);
+    const bool real = on && is_draft(p, task.x, n);
+    float top = -INFINITY, mass = 0.f;
+    float4 o[C];
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-        top[k] = -INFINITY;
-        mass[k] = 0.f;
+    for (int c = 0; c < C; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on) {
+        const float* slot0 = p.part + 2 * (int64_t)task.z * size;
+        for (int i0 = member; i0 < slots; i0 += 4 * p.team) {
+            float2 rm[4];
+            float4 x[4][C];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[k][i] = 0.f;
-    }
-    // (rows behind the unit's last are whatever is there, and not written)
-    for (int i = lane; i < slots; i += 32)
+            for (int u = 0; u < 4; ++u) {
+                const int i = i0 + u * p.team;
+                rm[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int k = 0; k < R; ++k)
-            if (r0 + k < p.rows) top[k] = fmaxf(top[k], slot_of(i)[p.rows * p.V + 2 * (r0 + k)]);
+                for (int c = 0; c < C; ++c) x[u][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < slots) {
+                    const float* s = slot0 + (i > 0 ? 2 * i * size : (task.w & 1) ? size : 0);
+                    rm[u] = *reinterpret_cast<const float2*>(s + p.rows * p.V + 2 * r);
 #pragma unroll
-    for (int k = 0; k < R; ++k) top[k] = warp_max(top[k]);
-#pragma unroll(R == 1 ? 4 : 2)
-    for (int i = member; i < slots; i += p.team) {
-        const float* s = slot_of(i);
-        float2 rm[R];
-        float4 x[R][2];
+                    for (int c = 0; c < C; ++c)
+                        if (c * 128 + lane * 4 < p.V) x[u][c] = *reinterpret_cast<const float4*>(s + r * p.V + c * 128 + lane * 4);
+                }
+            }
+            const float now = fmaxf(fmaxf(top, fmaxf(rm[0].x, rm[1].x)), fmaxf(rm[2].x, rm[3].x)), ref = now == -INFINITY ? 0.f : now;
+            const float keep = exp2f(top - ref);
+            top = now;
+            mass *= keep;
 #pragma unroll
-        for (int k = 0; k < R; ++k) {
-            const int r = min(r0 + k, p.rows - 1);
-            rm[k] = *reinterpret_cast<const float2*>(s + p.rows * p.V + 2 * r);
+            for (int c = 0; c < C; ++c) o[c] = make_float4(o[c].x * keep, o[c].y * keep, o[c].z * keep, o[c].w * keep);
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-                x[k][half] = half * 128 + lane * 4 < p.V ? *reinterpret_cast<const float4*>(s + r * p.V + half * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+            for (int u = 0; u < 4; ++u) {
+                const float f = exp2f(rm[u].x - ref);
+                mass = fmaf(f, rm[u].y, mass);
 #pragma unroll
-        for (int k = 0; k < R; ++k) {
-            const float f = exp2f(rm[k].x - (top[k] == -INFINITY ? 0.f : top[k]));
-            mass[k] = fmaf(f, rm[k].y, mass[k]);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                o[k][4 * half] = fmaf(f, x[k][half].x, o[k][4 * half]);
-                o[k][4 * half + 1] = fmaf(f, x[k][half].y, o[k][4 * half + 1]);
-                o[k][4 * half + 2] = fmaf(f, x[k][half].z, o[k][4 * half + 2]);
-                o[k][4 * half + 3] = fmaf(f, x[k][half].w, o[k][4 * half + 3]);
+                for (int c = 0; c < C; ++c)
+                    o[c] = make_float4(fmaf(f, x[u][c].x, o[c].x), fmaf(f, x[u][c].y, o[c].y), fmaf(f, x[u][c].z, o[c].z), fmaf(f, x[u][c].w, o[c].w));
             }
         }
     }
-    if (R == 1 && p.team > 1) {
+    if (p.team > 1) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-            if (half * 128 < p.V)
-                *reinterpret_cast<float4*>(&red[w][half * 128 + lane * 4]) = make_float4(o[0][4 * half], o[0][4 * half + 1], o[0][4 * half + 2], o[0][4 * half + 3]);
-        if (lane == 0) wl[w] = mass[0];
+        for (int c = 0; c < C; ++c) red[w][c][lane] = o[c];
+        if (lane == 0) stat[w] = make_float2(top, mass);
         __syncthreads();
         if (member > 0) return;
-        for (int i = 1; i < p.team; ++i) {
-            mass[0] += wl[w + i];
+        float now = top;
+        for (int i = 1; i < p.team; ++i) now = fmaxf(now, stat[w + i].x);
+        const float ref = now == -INFINITY ? 0.f : now;
+        mass = 0.f;
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-                if (half * 128 < p.V) {
-                    const float4 x = *reinterpret_cast<const float4*>(&red[w + i][half * 128 + lane * 4]);
-                    o[0][4 * half] += x.x; o[0][4 * half + 1] += x.y; o[0][4 * half + 2] += x.z; o[0][4 * half + 3] += x.w;
-                }
+        for (int c = 0; c < C; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < p.team; ++i) {
+            const float f = exp2f(stat[w + i].x - ref);
+            mass = fmaf(f, stat[w + i].y, mass);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float4 x = red[w + i][c][lane];
+                o[c] = make_float4(fmaf(f, x.x, o[c].x), fmaf(f, x.y, o[c].y), fmaf(f, x.z, o[c].z), fmaf(f, x.w, o[c].w));
+            }
         }
+        top = now;
     }
+    if (!on) return;
+    const int64_t row = ((int64_t)task.x * p.N + n) * p.H + h;
+    const float inv = real ? finish_scale(mass) : 0.f;
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-        int n, h;
-        if (r0 + k >= p.rows || !row_of(p, task.y, r0 + k, n, h)) continue;
-        const bool real = is_draft(p, task.x, n);
-        const int64_t row = ((int64_t)task.x * p.N + n) * p.H + h;
-        const float inv = finish_scale(mass[k]);
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            const int col = (i >> 2) * 128 + lane * 4 + (i & 3);
-            if (col >= p.V) continue;
-            const float a = real ? o[k][i] * inv : 0.f, b = real ? o[k][i + 1] * inv : 0.f;
-            T* to = reinterpret_cast<T*>(p.out) + row * p.V + col;
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to) = make_float2(a, b);
-            else *reinterpret_cast<uint32_t*>(to) = Frag<T>::pack(a, b);
-        }
-        if (p.lse && lane == 0) p.lse[row] = real ? finish_lse(top[k], mass[k]) : -INFINITY;
+    for (int c = 0; c < C; ++c) {
+        const int col = c * 128 + lane * 4;
+        if (col >= p.V) continue;
+        T* to = reinterpret_cast<T*>(p.out) + row * p.V + col;
+        const float4 y = real ? make_float4(o[c].x * inv, o[c].y * inv, o[c].z * inv, o[c].w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(to) = y;
+        else *reinterpret_cast<uint2*>(to) = make_uint2(Frag<T>::pack(y.x, y.y), Frag<T>::pack(y.z, y.w));
     }
+    if (p.lse && lane == 0) p.lse[row] = real ? finish_lse(top, mass) : -INFINITY;
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------
@@ -1611,11 +1622,15 @@ static bool row_map(CUtensorMap& map, const char* base, int width, const MapDim 
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-static int tc_maps(TcMaps& m, const DraftParams& p, bool bf16) {
+static int tc_maps(TcMaps& m, DraftParams& p, bool bf16) {
     int boxes = 0;
-    if (p.page.d % 16 == 0 && row_map(m.k, p.ck, p.K, {{(int64_t)p.page.d, p.ck_row, 16}, {p.Hkv, p.ck_h, 1}, {p.pages, p.ck_page, 1}}, bf16) &&
-        row_map(m.v, p.cv, p.V, {{(int64_t)p.page.d, p.cv_row, 16}, {p.Hkv, p.cv_h, 1}, {p.pages, p.cv_page, 1}}, bf16))
-        boxes |= 1;
+    auto caches = [&](CUtensorMap& k, CUtensorMap& v, uint32_t rows) {
+        return row_map(k, p.ck, p.K, {{(int64_t)p.page.d, p.ck_row, rows}, {p.Hkv, p.ck_h, 1}, {p.pages, p.ck_page, 1}}, bf16) &&
+               row_map(v, p.cv, p.V, {{(int64_t)p.page.d, p.cv_row, rows}, {p.Hkv, p.cv_h, 1}, {p.pages, p.cv_page, 1}}, bf16);
+    };
+    p.box_rows = p.page.d % 128 == 0 ? 128 : p.page.d % 64 == 0 ? 64 : p.page.d % 32 == 0 ? 32 : 16;
+    if (p.page.d % 16 == 0 && caches(m.k, m.v, 16)) boxes |= 1;
+    if (p.box_rows > 16 && !caches(m.kb, m.vb, (uint32_t)p.box_rows)) p.box_rows = 16;
     if (128 % p.G == 0 && row_map(m.q, p.q, p.K, {{p.H, p.q_h, (uint32_t)p.G}, {p.N, p.q_n, (uint32_t)(128 / p.G)}, {p.B, p.q_b, 1}}, bf16)) boxes |= 2;
     if (p.N >= 16 && row_map(m.dk, p.k, p.K, {{p.N, p.k_n, 16}, {p.Hkv, p.k_h, 1}, {p.B, p.k_b, 1}}, bf16) &&
         row_map(m.dv, p.v, p.V, {{p.N, p.v_n, 16}, {p.Hkv, p.v_h, 1}, {p.B, p.v_b, 1}}, bf16))
@@ -1637,7 +1652,7 @@ static int launch_mma(const DraftParams& p, cudaStream_t st) {
         if (const cudaError_t e = limit.raise((const void*)draft_tc_kernel<T, DK, DV>, TcShape<DK, DV>::total)) return (int)e;
         TcMaps maps{};
         DraftParams q = p;
-        q.boxes = tc_maps(maps, p, std::is_same<T, __nv_bfloat16>::value);
+        q.boxes = tc_maps(maps, q, std::is_same<T, __nv_bfloat16>::value);
         return launch_chained(draft_tc_kernel<T, DK, DV>, dim3(p.grid), dim3(kTcThreads), TcShape<DK, DV>::total, st, q, maps);
     }
     return p.variant == kMma16 ? launch_mma<T, DK, DV, 1>(p, st) : launch_mma<T, DK, DV, 2>(p, st);
@@ -1666,11 +1681,10 @@ static int launch_draft(const DraftParams& p, cudaStream_t st) {
                        : (p.V <= 64 ? launch_mma<T, 128, 64>(p, st) : launch_mma<T, 128, 128>(p, st));
     }
     if (rc) return rc;
-    const bool alone = p.team == 1;
-    const int rows = p.N * p.G < p.rows ? p.N * p.G : p.rows, block = kJoinWarps / p.team * (alone ? kJoinRows : 1);
+    const int rows = p.N * p.G < p.rows ? p.N * p.G : p.rows, block = kJoinWarps / p.team;
     const dim3 grid(p.by_unit ? (unsigned)units_of(p) : (unsigned)p.grid, (rows + block - 1) / block);
-    return alone ? launch_chained(draft_join_kernel<T, kJoinRows>, grid, dim3(kJoinThreads), 0, st, p)
-                 : launch_chained(draft_join_kernel<T, 1>, grid, dim3(kJoinThreads), 0, st, p);
+    return p.V > 128 ? launch_chained(draft_join_kernel<T, true>, grid, dim3(kJoinThreads), 0, st, p)
+                     : launch_chained(draft_join_kernel<T, false>, grid, dim3(kJoinThreads), 0, st, p);
 }
 
 static int fill_draft(DraftParams& p, const HtreeCache* c, const HtreeDrafts* d) {
