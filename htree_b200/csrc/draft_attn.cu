@@ -1028,12 +1028,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
         // where lane's piece of row r goes within a 128-row operand: 64 columns to a block of 128-byte rows, 16-byte pieces swizzled by the row
         auto place_of = [&](int r, int c) { return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
         auto tell = [&](int bar, uint32_t bytes) { if (lane == 0) mbar_arrive_expect_tx(bars + bar, bytes); };
+        // `blocks` boxes of 64 columns; by one lane
         auto box = [&](const CUtensorMap& map, int blocks, int bar, uint32_t dst, int row, int head, int page) {
-            if (elect_one())
-                for (int blk = 0; blk < blocks; ++blk)
-                    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
-                                     dst + blk * (128 * 128)), "l"(&map), "r"(blk * 64), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bars + bar)) : "memory");
-            __syncwarp();
+            for (int blk = 0; blk < blocks; ++blk)
+                asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
+                                 dst + blk * (128 * 128)), "l"(&map), "r"(blk * 64), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bars + bar)) : "memory");
+        };
+        auto copy_rows = [&](auto lanes_, uint32_t dst, const unsigned long long (&rows)[4], const uint32_t (&words)[4], uint32_t boxes, int width) {
+            constexpr int lanes = decltype(lanes_)::value, per = 32 / lanes;             // lanes of a row, rows at a time
+            const int c = lane % lanes, mine = lane / lanes;
+            const bool col = c * 8 < width;
+            const uint32_t to = dst + (c >> 3) * (128 * 128) + mine * 128, piece = (uint32_t)((c & 7) ^ mine);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if ((boxes >> (2 * q) & 3u) == 3u) continue;
+#pragma unroll
+                for (int r = 0; r < 32; r += per) {
+                    if (boxes >> (2 * q + (r >> 4)) & 1u) continue;
+                    const unsigned long long src = __shfl_sync(0xffffffffu, rows[q], r + mine);
+                    const bool on = (words[q] >> (r + mine) & 1u) && col;
+                    cp_async16_or_zero(to + (q * 32 + r) * 128 + ((piece ^ (r & 7)) << 4), on ? reinterpret_cast<const char*>(src) + c * 16 : p.q, on);
+                }
+            }
         };
         while (done < n_tiles) {
             const int piece = min(n_tiles - done, at.tiles - at.tile), cached = at.tiles - p.draft_tiles, kv = head_of(p, at.unit);
@@ -1043,7 +1059,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
             if (p.boxes & 2) {                            // whole drafts to a half: a box of the heads of 128 / G drafts
                 if (cw == 0) {
                     tell(kQFull, halves * S::qhalf);
-                    for (int i = 0; i < halves; ++i)
+                    __syncwarp();
+                    if (elect_one()) for (int i = 0; i < halves; ++i)
                         box(maps.q, DK / 64, kQFull, base + S::q + i * S::qhalf, kv * p.G, (int)p.group.div((uint32_t)(row0 + i * 128)), at.b);
                 } else {
                     tell(kQFull, 0);
@@ -1067,6 +1084,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
             const bool values = cw > 0;
             int j = values ? (cw - 1 + g) & 1 : 0;
             const int jstep = values ? 2 : 1, lanes = values ? VL : KL, width = values ? p.V : p.K;
+            int late_bar = -1;
+            uint32_t late_bytes = 0;
             int looked = -1, page = -1;                   // lane i < 8: the page of slice i of the next tile
             auto look = [&](int tile) {
                 const int pos = tile * kTcTile + (lane & 7) * 16;
@@ -1091,13 +1110,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                         for (int i = 0; i < 16; ++i) whole16 &= is_draft(p, at.b, n0 + (lane & 7) * 16 + i);
                 }
                 const uint32_t boxes = __ballot_sync(0xffffffffu, whole16) & 0xffu;
-                // others, row by row: which keys there are
+                // others, row by row: which keys there are, and where (lane x the key x of each 32)
                 uint32_t words[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+                unsigned long long rows[4];
                 if (boxes != 0xffu) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const char *kk = p.q, *vv = p.q;
                         words[i] = __ballot_sync(0xffffffffu, key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, i * 32 + lane, kk, vv, &bad));
+                        rows[i] = reinterpret_cast<unsigned long long>(values ? vv : kk);
                     }
                 }
                 wait(empty, ((uint32_t)turn & 1u) ^ 1u);
@@ -1111,40 +1132,44 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 const int bar = look_through ? kRaw + cw : full;
                 const uint32_t bytes = (uint32_t)__popc(boxes) * 256u * lanes;
                 if (look_through || boxes == 0xffu) tell(bar, bytes);
-                if (boxes == 0xffu && !draft && p.box_rows > 16) {
-#pragma unroll 1
-                    for (int r = 0; r < kTcTile; r += p.box_rows) {
-                        const int pg = __shfl_sync(0xffffffffu, page, r >> 4), i = __shfl_sync(0xffffffffu, in, r >> 4);
-                        box(values ? maps.vb : maps.kb, lanes / 8, bar, dst + r * 128, i, kv, pg);
-                    }
-                } else {
-                    const CUtensorMap& map = draft ? (values ? maps.dv : maps.dk) : (values ? maps.v : maps.k);
-#pragma unroll 1
+                if (boxes) {
+                    int pages[8], ins[8];
+#pragma unroll
                     for (int sl = 0; sl < 8; ++sl) {
-                        const int pg = __shfl_sync(0xffffffffu, page, sl), i = __shfl_sync(0xffffffffu, in, sl);
-                        if (boxes >> sl & 1) box(map, lanes / 8, bar, dst + sl * 2048, draft ? n0 + sl * 16 : i, kv, draft ? at.b : pg);
+                        pages[sl] = __shfl_sync(0xffffffffu, page, sl);
+                        ins[sl] = __shfl_sync(0xffffffffu, in, sl);
                     }
-                }
-                if (boxes != 0xffu) {
-                    const int per = 32 / lanes, c = lane % lanes;
-#pragma unroll 1
-                    for (int q = 0; q < 4; ++q) {         // 32 keys, a lane each
-                        if ((boxes >> (2 * q) & 3u) == 3u) continue;
-                        const uint32_t word = q == 0 ? words[0] : q == 1 ? words[1] : q == 2 ? words[2] : words[3];
-                        const char *kk = p.q, *vv = p.q;
-                        bool dull = false;
-                        key_row(p, Place{at.b, at.unit, tile, at.tiles, at.len}, kv, q * 32 + lane, kk, vv, &dull);
-                        const unsigned long long own = reinterpret_cast<unsigned long long>(values ? vv : kk);
-#pragma unroll 4
-                        for (int r = 0; r < 32; r += per) {
-                            const int x = r + lane / lanes;
-                            const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, own, x));
-                            const bool on = (word >> x & 1) && c * 8 < width;
-                            if (!(boxes >> (2 * q + (x >> 4)) & 1)) cp_async16_or_zero(dst + place_of(q * 32 + x, c), on ? src + c * 16 : p.q, on);
+                    if (elect_one()) {
+                        if (draft) {
+#pragma unroll
+                            for (int sl = 0; sl < 8; ++sl)
+                                if (boxes >> sl & 1) box(values ? maps.dv : maps.dk, lanes / 8, bar, dst + sl * 2048, n0 + sl * 16, kv, at.b);
+                        } else if (boxes == 0xffu && p.box_rows > 16) {
+#pragma unroll
+                            for (int sl = 0; sl < 8; sl += 2)
+                                if (((sl * 16) & (p.box_rows - 1)) == 0) box(values ? maps.vb : maps.kb, lanes / 8, bar, dst + sl * 2048, ins[sl], kv, pages[sl]);
+                        } else {
+#pragma unroll
+                            for (int sl = 0; sl < 8; ++sl)
+                                if (boxes >> sl & 1) box(values ? maps.v : maps.k, lanes / 8, bar, dst + sl * 2048, ins[sl], kv, pages[sl]);
                         }
                     }
+                    __syncwarp();
+                }
+                if (boxes != 0xffu) {
+                    if (lanes == 16) copy_rows(std::integral_constant<int, 16>{}, dst, rows, words, boxes, width);
+                    else copy_rows(std::integral_constant<int, 8>{}, dst, rows, words, boxes, width);
                     cp_async_commit();
-                    cp_async_wait<0>();
+                    if (values) cp_async_wait<0>();
+                }
+                // Rows of keys are told one tile later, when they have had time to come (their stage's next use is two tiles away; that of
+                // values waits for them).
+                if (late_bar >= 0) {
+                    if (boxes != 0xffu) cp_async_wait<1>(); else cp_async_wait<0>();
+                    fence_proxy_async();
+                    __syncwarp();
+                    tell(late_bar, late_bytes);
+                    late_bar = -1;
                 }
                 if (look_through) {
                     wait(bar, raws++ & 1u);
@@ -1153,13 +1178,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                     for (int x = lane; x < kTcTile * lanes; x += 32)
                         if (take_out<T>(dst + place_of(x / lanes, x % lanes))) atomicOr(&spoilt[(t & 7) * 4 + (x / lanes >> 5)], 1u << (x / lanes & 31));
                 }
-                if (look_through || boxes != 0xffu) {
+                if (!values && boxes != 0xffu) {
+                    late_bar = full;
+                    late_bytes = bytes;
+                } else if (look_through || boxes != 0xffu) {
                     fence_proxy_async();
                     __syncwarp();
                     tell(full, look_through ? 0 : bytes);
                 }
                 if (j + jstep < piece) look(tile + jstep);
                 last = t;
+            }
+            if (late_bar >= 0) {
+                cp_async_wait<0>();
+                fence_proxy_async();
+                __syncwarp();
+                tell(late_bar, late_bytes);
             }
             g += piece;
             done += piece;
@@ -1578,7 +1612,9 @@ static void fit(DraftParams& p, int rows, int tile, int blocks, int least) {
 static int64_t part_bytes(const DraftParams& p) { return (int64_t)p.grid * 2 * p.rows * (p.V + 2) * 4; }
 static int64_t workspace_of(const DraftParams& p) { return part_bytes(p) + p.grid * 16; }           // tasks: per unit or per part, never more than parts
 
-// Which kernel: 16-bit rows of up to 128 go to the tensor cores.
+// Which kernel: 16-bit rows of up to 128 go to the tensor cores, by mma.sync up to 32 query rows, up to 16 with rows of more than 64 (where
+// a warp of 32 has spills).  Measured, 8 requests of 16384, 4 heads of 128: 32 rows 84 us on mma.sync and 70 on tcgen05, 16 rows 63 and
+// 70; 8 heads of 64: 32 rows 78 and 97; 8 requests of 1000, 4 heads of 128: 32 rows 25 and 27, 16 rows 20 and 27.
 enum { kGeneric = 0, kMma16, kMma32, kTc };
 static void choose(DraftParams& p, int dtype) {
     const int sms = sm_count() > 0 ? sm_count() : 148, rows = p.N * p.G;
@@ -1587,7 +1623,7 @@ static void choose(DraftParams& p, int dtype) {
         fit(p, kGenRows, kTile, sms * (generic_smem(p) <= 110 * 1024 ? 2 : 1), 1);
         return;
     }
-    p.variant = rows <= 16 ? kMma16 : rows <= 32 ? kMma32 : kTc;
+    p.variant = rows <= 16 ? kMma16 : rows <= 32 && p.K <= 64 && p.V <= 64 ? kMma32 : kTc;
     if (p.variant == kTc) fit(p, rows <= 128 ? 128 : 256, kTcTile, sms, 1);
     else fit(p, rows <= 16 ? 16 : 32, kSlice, sms, rows <= 16 ? 12 : 8);
     if (p.c < 0.f) { p.neg = 1; p.c = -p.c; }
@@ -1655,7 +1691,9 @@ static int launch_mma(const DraftParams& p, cudaStream_t st) {
         q.boxes = tc_maps(maps, q, std::is_same<T, __nv_bfloat16>::value);
         return launch_chained(draft_tc_kernel<T, DK, DV>, dim3(p.grid), dim3(kTcThreads), TcShape<DK, DV>::total, st, q, maps);
     }
-    return p.variant == kMma16 ? launch_mma<T, DK, DV, 1>(p, st) : launch_mma<T, DK, DV, 2>(p, st);
+    if constexpr (DK == 64 && DV == 64)
+        if (p.variant == kMma32) return launch_mma<T, DK, DV, 2>(p, st);
+    return launch_mma<T, DK, DV, 1>(p, st);
 }
 
 template <typename T>
