@@ -463,28 +463,31 @@ __device__ __forceinline__ float put_back(float o, const char* v, int col) {
     return fabsf(x) <= 3.4028234e38f ? o : o + x;
 }
 
-template <int DK, int DV, int RM> struct MmaShape {
-    static constexpr int warps = RM == 1 ? 12 : 8, threads = warps * 32, rows = RM * 16;
-    static constexpr int krow = DK * 2 + 16, vrow = DV * 2 + 16;             // 16 bytes more than a row: eight rows meet in no bank
+template <typename T, int DK, int DV, int R> struct SliceShape {          // R query rows
+    static constexpr bool f32 = sizeof(T) == 4;
+    static constexpr int warps = R == 32 ? 8 : f32 && DK + DV > 192 ? 6 : f32 && DK + DV > 128 ? 8 : 12, threads = warps * 32, rows = R;
+    static constexpr int krow = DK * (int)sizeof(T) + 16, vrow = DV * (int)sizeof(T) + 16;             // 16 bytes more than a row: eight rows meet in no bank
     static constexpr int stage = kSlice * (krow + vrow);
     // columns of a joining round: what fits into the stage that the unit's last tile has left
     static constexpr int cols = DV == 128 && rows * 132 * 4 <= stage ? 128 : rows * 68 * 4 <= stage ? 64 : 32, jrow = cols + 4;
     static_assert(rows * jrow * 4 <= stage, "");
-    static constexpr int fixed = 2 * warps * rows * 4 + 2 * rows * 4 + rows * krow;
+    static constexpr int weights = f32 ? warps * rows * kSlice * 4 : 0;
+    static constexpr int fixed = 2 * warps * rows * 4 + (rows + 16) * 4 + rows * krow + weights;
     static constexpr int fit = (232448 - 512 - fixed) / (warps * stage);
     static constexpr int stages = fit > 4 ? 4 : fit;
     static_assert(stages >= 2, "");
-    static constexpr int wm = 0, wl = wm + warps * rows * 4, sums = wl + warps * rows * 4, q = sums + 2 * rows * 4, ring = (q + rows * krow + 127) / 128 * 128,
-                         total = ring + warps * stages * stage;
+    static constexpr int wm = 0, wl = wm + warps * rows * 4, sums = wl + warps * rows * 4, q = sums + (rows + 16) * 4, p = q + rows * krow,
+                         ring = (p + weights + 127) / 128 * 128, total = ring + warps * stages * stage;
 };
 
 // The code of a part runs few times over (a handful of tiles, one or two joins), and instructions that run for the first time come at 8 to
 // 10 cycles each: one loop, in which fetching, computing and joining stand once each, nothing unrolled that need not be.  (Unrolled, with
 // the prologue and every refill inlined, a call of 1024 cached tokens took 38,000 cycles, 26,000 of them outside the tiles.)
-template <typename T, int DK, int DV, int RM>
-__global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_kernel(const __grid_constant__ DraftParams p) {
-    using S = MmaShape<DK, DV, RM>;
-    constexpr int NT = S::threads, NW = S::warps, ST = S::stages, ROWS = S::rows;
+template <typename T, int DK, int DV, int ROWS>
+__global__ void __launch_bounds__(SliceShape<T, DK, DV, ROWS>::threads, 1) draft_slice_kernel(const __grid_constant__ DraftParams p) {
+    using S = SliceShape<T, DK, DV, ROWS>;
+    constexpr bool F32 = S::f32;
+    constexpr int NT = S::threads, NW = S::warps, ST = S::stages, RM = F32 ? 1 : ROWS / 16, E = 16 / (int)sizeof(T);       // E: elements of 16 bytes
     extern __shared__ __align__(128) unsigned char sm[];
     float* wm = reinterpret_cast<float*>(sm + S::wm);
     float* wl = reinterpret_cast<float*>(sm + S::wl);
@@ -511,11 +514,11 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
     // The rows of q of a unit, to shared memory.
     auto fetch_q = [&](const Place& pl) {
 #pragma unroll 1
-        for (int i = tid; i < ROWS * (DK / 8); i += NT) {
-            const int r = i / (DK / 8), c = i % (DK / 8);
+        for (int i = tid; i < ROWS * (DK / E); i += NT) {
+            const int r = i / (DK / E), c = i % (DK / E);
             int n, h;
             const bool on = row_of(p, pl.unit, r, n, h);
-            if (c * 8 < p.K) cp_async16_or_zero(q_u + r * S::krow + c * 16, on ? p.q + pl.b * p.q_b + n * p.q_n + h * p.q_h + c * 16 : p.q, on);
+            if (c * E < p.K) cp_async16_or_zero(q_u + r * S::krow + c * 16, on ? p.q + pl.b * p.q_b + n * p.q_n + h * p.q_h + c * 16 : p.q, on);
         }
     };
     fetch_q(at);
@@ -527,13 +530,15 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
         const int pos = pl.tile * kSlice + (lane & 15);
         return pl.tile < pl.tiles - p.draft_tiles && pos < pl.len ? __ldg(p.table + (int64_t)pl.b * p.table_stride + p.page.div((uint32_t)pos)) : -1;
     };
-    constexpr int KL = DK / 8, VL = DV / 8;              // lanes of a row
+    constexpr int KL = DK / E, VL = DV / E;              // lanes of a row
     const uint32_t kdst = ring_u + lane / KL * S::krow + lane % KL * 16, vdst = ring_u + kSlice * S::krow + lane / VL * S::vrow + lane % VL * 16;
-    const bool kcol = lane % KL * 8 < p.K, vcol = lane % VL * 8 < p.V;
+    const bool kcol = lane % KL * E < p.K, vcol = lane % VL * E < p.V;
     const int64_t kstep = p.ck_row * (32 / KL), vstep = p.cv_row * (32 / VL);
     uint64_t keys_of = 0;                  // which keys a stage has: 16 bits each
 
-    float o[RM][DV / 8][4], ref[RM][2], mass[RM][2];
+    // 16 bits: fragments of RM x 16 rows, this thread's rows g and g + 8 of each; fp32: all rows' columns CW * lane .., and this lane's keys' mass
+    constexpr int CW = DV / 32;
+    float o[RM][DV / 8][4], ref[RM][2], mass[RM][2], fo[F32 ? ROWS : 1][CW], fref[F32 ? ROWS : 1], fmass[F32 ? ROWS : 1];
     uint32_t qf[RM][DK / 16][4];
     int piece = 0, first = 0, end = 0;     // tiles first .. end of the part: the share of the present unit
     int had = -1;                          // the stage of this warp's last tile of the unit, or -1: it had none
@@ -546,15 +551,25 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
             if (piece > 0) {
                 // the block's warps, those that had a tile of the unit: one reference, the sums added, through the stages that they have left
                 if (had >= 0) {
+                    if constexpr (F32) {
 #pragma unroll
-                    for (int m = 0; m < RM; ++m)
+                        for (int r = 0; r < ROWS; ++r) {
+                            float x = fmass[r];
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            float x = mass[m][half];
-                            x += __shfl_xor_sync(0xffffffffu, x, 1);
-                            x += __shfl_xor_sync(0xffffffffu, x, 2);
-                            if (r4 == 0) { wm[w * ROWS + m * 16 + half * 8 + g] = ref[m][half]; wl[w * ROWS + m * 16 + half * 8 + g] = x; }
+                            for (int d = 8; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+                            if (lane == r) { wm[w * ROWS + r] = fref[r]; wl[w * ROWS + r] = x; }
                         }
+                    } else {
+#pragma unroll
+                        for (int m = 0; m < RM; ++m)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                float x = mass[m][half];
+                                x += __shfl_xor_sync(0xffffffffu, x, 1);
+                                x += __shfl_xor_sync(0xffffffffu, x, 2);
+                                if (r4 == 0) { wm[w * ROWS + m * 16 + half * 8 + g] = ref[m][half]; wl[w * ROWS + m * 16 + half * 8 + g] = x; }
+                            }
+                    }
                     if (lane == 0) stage_of[w] = had;
                 }
                 __syncthreads();
@@ -583,18 +598,33 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
                     scale_of[lane] = f;
                 }
                 float f[RM][2];
+                if constexpr (F32) {
 #pragma unroll
-                for (int m = 0; m < RM; ++m)
+                    for (int r = 0; r < ROWS; ++r) {
+                        const float j = __shfl_sync(0xffffffffu, joint, r), y = j == -INFINITY ? 1.f : ex2_approx(fref[r] - j);
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float j = __shfl_sync(0xffffffffu, joint, m * 16 + half * 8 + g);
-                        f[m][half] = j == -INFINITY ? 1.f : ex2_approx(ref[m][half] - j);
+                        for (int i = 0; i < CW; ++i) fo[r][i] *= y;
                     }
+                } else {
+#pragma unroll
+                    for (int m = 0; m < RM; ++m)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const float j = __shfl_sync(0xffffffffu, joint, m * 16 + half * 8 + g);
+                            f[m][half] = j == -INFINITY ? 1.f : ex2_approx(ref[m][half] - j);
+                        }
+                }
 #pragma unroll
                 for (int c = 0; c < DV / S::cols; ++c) {
                     if (c > 0) __syncthreads();
                     if (had >= 0) {
                         float* own = reinterpret_cast<float*>(ring + had * S::stage);
+                        if constexpr (F32) {
+#pragma unroll
+                            for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+                                for (int i = 0; i < CW; ++i) own[r * S::jrow + lane * CW + i] = fo[r][i];
+                        } else
 #pragma unroll
                         for (int m = 0; m < RM; ++m)
 #pragma unroll
@@ -618,9 +648,14 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
                             }
                             if (whole) {
                                 const float z = scale_of[row];
-                                uint2 v = make_uint2(Frag<T>::pack(sum.x * z, sum.y * z), Frag<T>::pack(sum.z * z, sum.w * z));
-                                if (z < 0.f) v = make_uint2(0u, 0u);
-                                *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + (((int64_t)at.b * p.N + n) * p.H + h) * p.V + col) = v;
+                                T* to = reinterpret_cast<T*>(p.out) + (((int64_t)at.b * p.N + n) * p.H + h) * p.V + col;
+                                if constexpr (F32) {
+                                    *reinterpret_cast<float4*>(to) = z < 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * z, sum.y * z, sum.z * z, sum.w * z);
+                                } else {
+                                    uint2 v = make_uint2(Frag<T>::pack(sum.x * z, sum.y * z), Frag<T>::pack(sum.z * z, sum.w * z));
+                                    if (z < 0.f) v = make_uint2(0u, 0u);
+                                    *reinterpret_cast<uint2*>(to) = v;
+                                }
                             } else {
                                 *reinterpret_cast<float4*>(slot + row * p.V + col) = sum;
                             }
@@ -653,6 +688,15 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
             piece = min(n_tiles - first, at.tiles - at.tile);
             end = first + piece;
             had = -1;
+            if constexpr (F32) {
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    fref[r] = -INFINITY;
+                    fmass[r] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < CW; ++i) fo[r][i] = 0.f;
+                }
+            } else {
 #pragma unroll
             for (int m = 0; m < RM; ++m) {
                 ref[m][0] = ref[m][1] = -INFINITY;
@@ -672,6 +716,7 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
                     for (int ks = 0; ks < DK / 16; ++ks)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) qf[m][ks][e] ^= 0x80008000u;
+            }
         }
 
         // fetch tile k of this warp
@@ -752,6 +797,81 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
         __syncwarp();
         const uint32_t kbase = ring_u + cur * S::stage, vbase = kbase + kSlice * S::krow;
         const uint32_t keys = (uint32_t)(keys_of >> (16 * cur)) & 0xffffu;
+        if constexpr (F32) {
+            // Lane x has key x & 15, and of every row half the elements.
+            const int key = lane & 15;
+            float s[ROWS];
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) s[r] = 0.f;
+            const float* kk = reinterpret_cast<const float*>(sm + (kbase - smem_u32(sm)) + key * S::krow) + (lane >> 4) * (DK / 2);
+            const float* qq = reinterpret_cast<const float*>(sm + S::q) + (lane >> 4) * (DK / 2);
+#pragma unroll 4
+            for (int d = 0; d < DK / 2; d += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(kk + d);
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    const float4 y = *reinterpret_cast<const float4*>(qq + r * (S::krow / 4) + d);
+                    s[r] = fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, fmaf(x.x, y.x, s[r]))));
+                }
+            }
+            uint32_t own = keys;                          // which keys row `lane` reads
+            if (draft) {
+                int n, h;
+                own = lane < ROWS && row_of(p, at.unit, lane, n, h) ? keys & (uint32_t)draft_mask(p, at.b, n, (tile - cached) * kSlice, &bad) : 0u;
+            }
+            bool above = false;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                s[r] += __shfl_xor_sync(0xffffffffu, s[r], 16);
+                const uint32_t seen = draft ? __shfl_sync(0xffffffffu, own, r) : keys;
+                s[r] = (seen >> key & 1) ? s[r] * p.c : -INFINITY;
+                above |= s[r] > fref[r] + kLag<T>;
+            }
+            if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    float x = s[r];
+#pragma unroll
+                    for (int d = 8; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                    const float now = fmaxf(fref[r], x), keep = now == -INFINITY ? 1.f : ex2_approx(fref[r] - now);
+                    fref[r] = now;
+                    fmass[r] *= keep;
+#pragma unroll
+                    for (int i = 0; i < CW; ++i) fo[r][i] *= keep;
+                }
+            }
+            float* pw = reinterpret_cast<float*>(sm + S::p) + w * ROWS * kSlice;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const float e = ex2_approx(s[r] - (fref[r] == -INFINITY ? 0.f : fref[r]));
+                fmass[r] += e;
+                if (lane < 16) pw[r * kSlice + lane] = e;
+            }
+            __syncwarp();
+            const float* vv = reinterpret_cast<const float*>(sm + (vbase - smem_u32(sm))) + lane * CW;
+#pragma unroll
+            for (int j = 0; j < kSlice; j += 4) {
+                float x[4][CW];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (CW == 4) *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(vv + (j + i) * (S::vrow / 4));
+                    else *reinterpret_cast<float2*>(x[i]) = *reinterpret_cast<const float2*>(vv + (j + i) * (S::vrow / 4));
+                }
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    const float4 y = *reinterpret_cast<const float4*>(pw + r * kSlice + j);
+                    const float ys[4] = {y.x, y.y, y.z, y.w};
+                    const uint32_t seen = draft ? __shfl_sync(0xffffffffu, own, r) >> j : 0xfu;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (!(seen >> i & 1)) continue;       // a draft's values, whatever they are, stay with those that read it
+#pragma unroll
+                        for (int c = 0; c < CW; ++c) fo[r][c] = fmaf(ys[i], x[i][c], fo[r][c]);
+                    }
+                }
+            }
+            __syncwarp();
+        } else {
         uint32_t spoilt = 0;
         if (draft) {
 #pragma unroll 1
@@ -865,6 +985,7 @@ __global__ void __launch_bounds__(MmaShape<DK, DV, RM>::threads, 1) draft_mma_ke
                             if ((seen[m][e >> 1] >> j & 1) && col < p.V) o[m][d][e] = put_back<T>(o[m][d][e], v, col);
                         }
             }
+        }
     }
 }
 
@@ -1615,15 +1736,20 @@ static int64_t workspace_of(const DraftParams& p) { return part_bytes(p) + p.gri
 // Which kernel: 16-bit rows of up to 128 go to the tensor cores, by mma.sync up to 32 query rows, up to 16 with rows of more than 64 (where
 // a warp of 32 has spills).  Measured, 8 requests of 16384, 4 heads of 128: 32 rows 84 us on mma.sync and 70 on tcgen05, 16 rows 63 and
 // 70; 8 heads of 64: 32 rows 78 and 97; 8 requests of 1000, 4 heads of 128: 32 rows 25 and 27, 16 rows 20 and 27.
-enum { kGeneric = 0, kMma16, kMma32, kTc };
+enum { kGeneric = 0, kSlice4, kSlice16, kSlice32, kTc };
 static void choose(DraftParams& p, int dtype) {
     const int sms = sm_count() > 0 ? sm_count() : 148, rows = p.N * p.G;
-    if (dtype == HTREE_F32 || p.K > 128 || p.V > 128) {
+    if (p.K > 128 || p.V > 128) {
         p.variant = kGeneric;
         fit(p, kGenRows, kTile, sms * (generic_smem(p) <= 110 * 1024 ? 2 : 1), 1);
         return;
     }
-    p.variant = rows <= 16 ? kMma16 : rows <= 32 && p.K <= 64 && p.V <= 64 ? kMma32 : kTc;
+    if (dtype == HTREE_F32) {
+        p.variant = rows <= 4 ? kSlice4 : kSlice16;
+        fit(p, rows <= 4 ? 4 : 16, kSlice, sms, p.K > 64 && p.V > 64 ? 6 : p.K > 64 || p.V > 64 ? 8 : 12);
+        return;
+    }
+    p.variant = rows <= 16 ? kSlice16 : rows <= 32 && p.K <= 64 && p.V <= 64 ? kSlice32 : kTc;
     if (p.variant == kTc) fit(p, rows <= 128 ? 128 : 256, kTcTile, sms, 1);
     else fit(p, rows <= 16 ? 16 : 32, kSlice, sms, rows <= 16 ? 12 : 8);
     if (p.c < 0.f) { p.neg = 1; p.c = -p.c; }
@@ -1674,15 +1800,18 @@ static int tc_maps(TcMaps& m, DraftParams& p, bool bf16) {
     return boxes;
 }
 
-template <typename T, int DK, int DV, int RM>
-static int launch_mma(const DraftParams& p, cudaStream_t st) {
+template <typename T, int DK, int DV, int ROWS>
+static int launch_slices(const DraftParams& p, cudaStream_t st) {
     static SmemLimit limit;
-    using S = MmaShape<DK, DV, RM>;
-    if (const cudaError_t e = limit.raise((const void*)draft_mma_kernel<T, DK, DV, RM>, S::total)) return (int)e;
-    return launch_chained(draft_mma_kernel<T, DK, DV, RM>, dim3(p.grid), dim3(S::threads), S::total, st, p);
+    using S = SliceShape<T, DK, DV, ROWS>;
+    if (const cudaError_t e = limit.raise((const void*)draft_slice_kernel<T, DK, DV, ROWS>, S::total)) return (int)e;
+    return launch_chained(draft_slice_kernel<T, DK, DV, ROWS>, dim3(p.grid), dim3(S::threads), S::total, st, p);
 }
 template <typename T, int DK, int DV>
-static int launch_mma(const DraftParams& p, cudaStream_t st) {
+static int launch_sized(const DraftParams& p, cudaStream_t st) {
+    if constexpr (sizeof(T) == 4) {
+        return p.variant == kSlice4 ? launch_slices<T, DK, DV, 4>(p, st) : launch_slices<T, DK, DV, 16>(p, st);
+    } else {
     if (p.variant == kTc) {
         static SmemLimit limit;
         if (const cudaError_t e = limit.raise((const void*)draft_tc_kernel<T, DK, DV>, TcShape<DK, DV>::total)) return (int)e;
@@ -1692,8 +1821,9 @@ static int launch_mma(const DraftParams& p, cudaStream_t st) {
         return launch_chained(draft_tc_kernel<T, DK, DV>, dim3(p.grid), dim3(kTcThreads), TcShape<DK, DV>::total, st, q, maps);
     }
     if constexpr (DK == 64 && DV == 64)
-        if (p.variant == kMma32) return launch_mma<T, DK, DV, 2>(p, st);
-    return launch_mma<T, DK, DV, 1>(p, st);
+        if (p.variant == kSlice32) return launch_slices<T, DK, DV, 32>(p, st);
+    return launch_slices<T, DK, DV, 16>(p, st);
+    }
 }
 
 template <typename T>
@@ -1710,14 +1840,9 @@ static int launch_generic(const DraftParams& p, cudaStream_t st) {
 
 template <typename T>
 static int launch_draft(const DraftParams& p, cudaStream_t st) {
-    int rc;
-    if constexpr (sizeof(T) == 4) {
-        rc = launch_generic<T>(p, st);
-    } else {
-        rc = p.variant == kGeneric ? launch_generic<T>(p, st)
-           : p.K <= 64 ? (p.V <= 64 ? launch_mma<T, 64, 64>(p, st) : launch_mma<T, 64, 128>(p, st))
-                       : (p.V <= 64 ? launch_mma<T, 128, 64>(p, st) : launch_mma<T, 128, 128>(p, st));
-    }
+    const int rc = p.variant == kGeneric ? launch_generic<T>(p, st)
+                 : p.K <= 64 ? (p.V <= 64 ? launch_sized<T, 64, 64>(p, st) : launch_sized<T, 64, 128>(p, st))
+                             : (p.V <= 64 ? launch_sized<T, 128, 64>(p, st) : launch_sized<T, 128, 128>(p, st));
     if (rc) return rc;
     const int rows = p.N * p.G < p.rows ? p.N * p.G : p.rows, block = kJoinWarps / p.team;
     const dim3 grid(p.by_unit ? (unsigned)units_of(p) : (unsigned)p.grid, (rows + block - 1) / block);
