@@ -36,6 +36,7 @@ struct DraftParams {
     int32_t B, N, H, Hkv, G, K, V, M, pages;
     int32_t rows, row_tiles, shift, draft_tiles;                           // rows of a row tile, log2 of the keys of a tile
     int32_t room;             // tokens that a row of the table can name
+    int32_t whole;            // short tables: parts of whole units, and nothing to join
     int32_t grid, least, by_unit, team;                                    // parts at most; tiles of a part at least; how tasks are indexed, and joined
     int32_t variant;          // which kernel (choose)
     int32_t boxes;            // tcgen05 kernel: what comes by tensor maps: 1 pages of whole slices of sixteen tokens, 2 q, 4 drafts
@@ -117,6 +118,21 @@ template <int NT>
 __device__ __forceinline__ bool find_part(const DraftParams& p, Place& at, Line& line, int64_t& x0, int64_t& x1) {
     __shared__ uint32_t scratch[NT / 32], found[2];
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, units = p.Hkv * p.row_tiles;
+    if (p.whole) {
+        const int64_t all = (int64_t)p.B * units, u0 = divide(blockIdx.x * all, p.grid), u1 = divide((blockIdx.x + 1) * all, p.grid);
+        if (u0 == u1) return false;
+        const int b0 = (int)divide(u0, units);
+        x0 = x1 = 0;
+        for (int64_t u = u0, b = b0; u < u1; ++b) {              // units of request b
+            const int64_t to = min((b + 1) * units, u1);
+            x1 += (to - u) * draft_tiles_of(p, (int)b);
+            u = to;
+        }
+        at.enter(p, b0);
+        at.unit = (int)(u0 - (int64_t)b0 * units);
+        at.tile = 0;
+        return true;
+    }
     const bool few = p.B <= 128;
     uint32_t mine, before;
     int b0;
@@ -161,6 +177,7 @@ __device__ __forceinline__ bool find_part(const DraftParams& p, Place& at, Line&
 // What there is to join of the unit that starts with tile u0 of the line, in part c: x = its request (-1: nothing), y = the unit of the
 // request, z = part c, w = 2 * parts + (another unit came before it in part c).
 __device__ __forceinline__ void leave_task(const DraftParams& p, const Place& at, int64_t u0, int64_t x0, int c, const Line& line, bool whole) {
+    if (p.whole) return;
     int4 t = make_int4(-1, 0, 0, 0);
     if (!whole) t = make_int4(at.b, at.unit, c, 2 * (line.part_of(u0 + at.tiles - 1) - c + 1) + (x0 < u0 ? 1 : 0));
     if (p.by_unit) p.tasks[(int64_t)at.b * p.Hkv * p.row_tiles + at.unit] = t;
@@ -261,7 +278,7 @@ __global__ void __launch_bounds__(kGenThreads) draft_generic_kernel(const __grid
     Place at;
     Line line;
     int64_t x0, x1;
-    if (tid == 0 && !p.by_unit) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (tid == 0 && !p.by_unit && !p.whole) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
     if (!find_part<kGenThreads>(p, at, line, x0, x1)) return;
     bool bad = false;
     { bool b = false; draft_length(p, at.b, &b); bad |= b; }
@@ -505,7 +522,7 @@ __global__ void __launch_bounds__(SliceShape<T, DK, DV, ROWS>::threads, 1) draft
     Place at;
     Line line;
     int64_t x0, x1;
-    if (tid == 0 && !p.by_unit) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (tid == 0 && !p.by_unit && !p.whole) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
     if (!find_part<NT>(p, at, line, x0, x1)) return;
     const int n_tiles = (int)(x1 - x0);
     bool bad = false;
@@ -1121,7 +1138,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
     Place at;
     Line line;
     int64_t x0, x1;
-    if (tid == 0 && !p.by_unit) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (tid == 0 && !p.by_unit && !p.whole) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
     if (!find_part<kTcThreads>(p, at, line, x0, x1)) return;
     const int n_tiles = (int)(x1 - x0);
     if (w == kTcMma) {
@@ -1726,12 +1743,17 @@ static void fit(DraftParams& p, int rows, int tile, int blocks, int least) {
     p.draft_tiles = (p.N + tile - 1) / tile;
     p.grid = blocks;
     p.least = least;
+    // With tables so short that a block is done with any unit in two rounds of its warps (tcgen05: in four tiles), parts are whole units, and
+    // the second kernel, 4 of 15 us of a small call, falls away.
+    const int most = ((p.room + tile - 1) >> p.shift) + p.draft_tiles;
+    p.whole = most <= (tile == kTcTile ? 4 : 2 * least);
+    if (p.whole && units_of(p) < p.grid) p.grid = (int32_t)units_of(p);
     p.by_unit = units_of(p) <= p.grid;
     const int64_t each = p.grid / units_of(p);         // parts of a unit
     p.team = each >= 16 ? 8 : each >= 8 ? 4 : each >= 4 ? 2 : 1;
 }
-static int64_t part_bytes(const DraftParams& p) { return (int64_t)p.grid * 2 * p.rows * (p.V + 2) * 4; }
-static int64_t workspace_of(const DraftParams& p) { return part_bytes(p) + p.grid * 16; }           // tasks: per unit or per part, never more than parts
+static int64_t part_bytes(const DraftParams& p) { return p.whole ? 0 : (int64_t)p.grid * 2 * p.rows * (p.V + 2) * 4; }
+static int64_t workspace_of(const DraftParams& p) { return p.whole ? 16 : part_bytes(p) + p.grid * 16; }           // tasks: per unit or per part, never more than parts
 
 // Which kernel: 16-bit rows of up to 128 go to the tensor cores, by mma.sync up to 32 query rows, up to 16 with rows of more than 64 (where
 // a warp of 32 has spills).  Measured, 8 requests of 16384, 4 heads of 128: 32 rows 84 us on mma.sync and 70 on tcgen05, 16 rows 63 and
@@ -1843,7 +1865,7 @@ static int launch_draft(const DraftParams& p, cudaStream_t st) {
     const int rc = p.variant == kGeneric ? launch_generic<T>(p, st)
                  : p.K <= 64 ? (p.V <= 64 ? launch_sized<T, 64, 64>(p, st) : launch_sized<T, 64, 128>(p, st))
                              : (p.V <= 64 ? launch_sized<T, 128, 64>(p, st) : launch_sized<T, 128, 128>(p, st));
-    if (rc) return rc;
+    if (rc || p.whole) return rc;
     const int rows = p.N * p.G < p.rows ? p.N * p.G : p.rows, block = kJoinWarps / p.team;
     const dim3 grid(p.by_unit ? (unsigned)units_of(p) : (unsigned)p.grid, (rows + block - 1) / block);
     return p.V > 128 ? launch_chained(draft_join_kernel<T, true>, grid, dim3(kJoinThreads), 0, st, p)
