@@ -1087,9 +1087,6 @@ __device__ __forceinline__ void tc_wait_ld(uint32_t (&x)[16]) { asm volatile("tc
 __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* x) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr), TC_W8(x, 0), TC_W8(x, 8) : "memory");
 }
-__device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t* x) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(addr), TC_W8(x, 0) : "memory");
-}
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* x) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
                  "%29,%30,%31,%32};\n" ::"r"(addr), TC_W8(x, 0), TC_W8(x, 8), TC_W8(x, 16), TC_W8(x, 24) : "memory");
@@ -1172,7 +1169,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
                                  dst + blk * (128 * 128)), "l"(&map), "r"(blk * 64), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bars + bar)) : "memory");
         };
-        auto copy_rows = [&](auto lanes_, uint32_t dst, const unsigned long long (&rows)[4], const uint32_t (&words)[4], uint32_t boxes, int width) {
+        // (rows of values that are not there become zero; rows of keys may hold anything, their scores are masked)
+        auto copy_rows = [&](auto lanes_, uint32_t dst, const unsigned long long (&rows)[4], const uint32_t (&words)[4], uint32_t boxes, int width, bool all_rows) {
             constexpr int lanes = decltype(lanes_)::value, per = 32 / lanes;             // lanes of a row, rows at a time
             const int c = lane % lanes, mine = lane / lanes;
             const bool col = c * 8 < width;
@@ -1185,6 +1183,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                     if (boxes >> (2 * q + (r >> 4)) & 1u) continue;
                     const unsigned long long src = __shfl_sync(0xffffffffu, rows[q], r + mine);
                     const bool on = (words[q] >> (r + mine) & 1u) && col;
+                    if (!all_rows && !(words[q] >> r & ((1u << per) - 1u))) continue;
                     cp_async16_or_zero(to + (q * 32 + r) * 128 + ((piece ^ (r & 7)) << 4), on ? reinterpret_cast<const char*>(src) + c * 16 : p.q, on);
                 }
             }
@@ -1295,8 +1294,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                     __syncwarp();
                 }
                 if (boxes != 0xffu) {
-                    if (lanes == 16) copy_rows(std::integral_constant<int, 16>{}, dst, rows, words, boxes, width);
-                    else copy_rows(std::integral_constant<int, 8>{}, dst, rows, words, boxes, width);
+                    if (lanes == 16) copy_rows(std::integral_constant<int, 16>{}, dst, rows, words, boxes, width, values);
+                    else copy_rows(std::integral_constant<int, 8>{}, dst, rows, words, boxes, width, values);
                     cp_async_commit();
                     if (values) cp_async_wait<0>();
                 }
@@ -1312,8 +1311,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 if (look_through) {
                     wait(bar, raws++ & 1u);
                     __syncwarp();
+                    const int rows_in = min(p.N - n0, kTcTile);
 #pragma unroll 2
-                    for (int x = lane; x < kTcTile * lanes; x += 32)
+                    for (int x = lane; x < rows_in * lanes; x += 32)
                         if (take_out<T>(dst + place_of(x / lanes, x % lanes))) atomicOr(&spoilt[(t & 7) * 4 + (x / lanes >> 5)], 1u << (x / lanes & 31));
                 }
                 if (!values && boxes != 0xffu) {
@@ -1436,30 +1436,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                     const int tile0 = (tile - cached) * kTcTile;
                     const uint64_t lo = on ? draft_mask(p, at.b, n, tile0, &bad) : 0ull, hi = on ? draft_mask(p, at.b, n, tile0 + 64, &bad) : 0ull;
                     seen[0] &= (uint32_t)lo; seen[1] &= (uint32_t)(lo >> 32); seen[2] &= (uint32_t)hi; seen[3] &= (uint32_t)(hi >> 32);
-                    wait(kVFull + gg % VS, (uint32_t)(gg / VS) & 1u);
-                    const uint32_t* sp = spoilt + (gg & 7) * 4;
-                    if (sp[0] | sp[1] | sp[2] | sp[3]) {
-                        tc_wait_st();
-                        tc_wait_ld(x[0]);
-                        const char* v0 = p.v + at.b * p.v_b + head_of(p, at.unit) * p.v_h;
-#pragma unroll 1
-                        for (int key = 0; key < kTcTile; ++key) {
-                            if (!(sp[key >> 5] >> (key & 31) & 1)) continue;
-                            const uint32_t mine = key < 32 ? seen[0] : key < 64 ? seen[1] : key < 96 ? seen[2] : seen[3];
-#pragma unroll 1
-                            for (int c = 0; c < DV; c += 16) {
-                                tc_ld16(x[0], to + c);
-                                tc_wait_ld(x[0]);
-                                if (mine >> (key & 31) & 1)
-#pragma unroll
-                                    for (int e = 0; e < 16; ++e)
-                                        if (c + e < p.V) x[0][e] = __float_as_uint(put_back<T>(__uint_as_float(x[0][e]), v0 + (int64_t)(tile0 + key) * p.v_n, c + e));
-                                tc_st16(to + c, x[0]);
-                                tc_wait_st();
-                            }
-                        }
-                        tc_ld16(x[0], ts);
-                    }
                 }
                 uint32_t pk[64];
                 float2 sums[2];
@@ -1492,12 +1468,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                     // the row's maximum first; the sums follow the reference if it moves
                     float top = -INFINITY;
 #pragma unroll 1
-                    for (int c = 0; c < 8; ++c) {
-                        tc_ld16(x[0], ts + c * 16);
+                    for (int c = 0; c < 4; ++c) {
+                        tc_ld16(x[0], ts + c * 32);
+                        tc_ld16(x[1], ts + c * 32 + 16);
                         tc_wait_ld(x[0]);
-                        const uint32_t there = (c < 2 ? seen[0] : c < 4 ? seen[1] : c < 6 ? seen[2] : seen[3]) >> (c & 1) * 16;
+                        tc_wait_ld(x[1]);
+                        const uint32_t there = c == 0 ? seen[0] : c == 1 ? seen[1] : c == 2 ? seen[2] : seen[3];
+                        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) top = fmaxf(top, (there >> e & 1) ? __uint_as_float(x[0][e]) : -INFINITY);
+                        for (int e = 0; e < 16; ++e) {
+                            t0 = fmaxf(t0, (there >> e & 1) ? __uint_as_float(x[0][e]) : -INFINITY);
+                            t1 = fmaxf(t1, (there >> (16 + e) & 1) ? __uint_as_float(x[1][e]) : -INFINITY);
+                        }
+                        top = fmaxf(top, fmaxf(t0, t1));
                     }
                     // (a row that has had nothing yet keeps a reference of zero, which is worth nothing)
                     const float want = top * p.c - kTcBias<T>, now = top == -INFINITY ? ref : empty ? want : fmaxf(ref, want);
@@ -1515,21 +1498,52 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                             tc_st16(to + c, x[0]);
                         }
                     }
-                    // (weights over the scores of sixteen keys take the place of eight: never of scores still to be read)
+                    // (weights over 32 scores take the place of sixteen: never of scores still to be read)
                     sums[0] = sums[1] = make_float2(0.f, 0.f);
 #pragma unroll 1
-                    for (int c = 0; c < 8; ++c) {
-                        tc_ld16(x[0], ts + c * 16);
+                    for (int c = 0; c < 4; ++c) {
+                        tc_ld16(x[0], ts + c * 32);
+                        tc_ld16(x[1], ts + c * 32 + 16);
                         tc_wait_ld(x[0]);
-                        const uint32_t there = (c < 2 ? seen[0] : c < 4 ? seen[1] : c < 6 ? seen[2] : seen[3]) >> (c & 1) * 16;
+                        tc_wait_ld(x[1]);
+                        const uint32_t there = c == 0 ? seen[0] : c == 1 ? seen[1] : c == 2 ? seen[2] : seen[3];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) x[0][e] = (there >> e & 1) ? x[0][e] : 0xff800000u;
-                        weigh(x[0], pk, std::false_type{});
-                        tc_st8(ts + c * 8, pk);
+                        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) x[i][e] = (there >> (16 * i + e) & 1) ? x[i][e] : 0xff800000u;
+                            weigh(x[i], pk + 8 * i, std::false_type{});
+                        }
+                        tc_st16(ts + c * 16, pk);
                     }
                 } else {
                     tc_st32(ts, pk);
                     tc_st32(ts + 32, pk + 32);
+                }
+                if (tile >= cached) {
+                    // values that are not finite, of drafts that this row reads
+                    const int tile0 = (tile - cached) * kTcTile;
+                    wait(kVFull + gg % VS, (uint32_t)(gg / VS) & 1u);
+                    const uint32_t* sp = spoilt + (gg & 7) * 4;
+                    if (sp[0] | sp[1] | sp[2] | sp[3]) {
+                        tc_wait_st();
+                        const char* v0 = p.v + at.b * p.v_b + head_of(p, at.unit) * p.v_h;
+#pragma unroll 1
+                        for (int key = 0; key < kTcTile; ++key) {
+                            if (!(sp[key >> 5] >> (key & 31) & 1)) continue;
+                            const uint32_t mine = key < 32 ? seen[0] : key < 64 ? seen[1] : key < 96 ? seen[2] : seen[3];
+#pragma unroll 1
+                            for (int c = 0; c < DV; c += 16) {
+                                tc_ld16(x[0], to + c);
+                                tc_wait_ld(x[0]);
+                                if (mine >> (key & 31) & 1)
+#pragma unroll
+                                    for (int e = 0; e < 16; ++e)
+                                        if (c + e < p.V) x[0][e] = __float_as_uint(put_back<T>(__uint_as_float(x[0][e]), v0 + (int64_t)(tile0 + key) * p.v_n, c + e));
+                                tc_st16(to + c, x[0]);
+                                tc_wait_st();
+                            }
+                        }
+                    }
                 }
                 mass += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
                 tc_wait_st();
@@ -1573,30 +1587,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
             const float inv = whole ? (real ? finish_scale(mass) : 0.f) : 1.f;
             const int64_t at_out = ((int64_t)at.b * p.N + n) * p.H + h;
             float* slot = p.part + (int64_t)(2 * blockIdx.x + (first_piece ? 0 : 1)) * p.rows * (p.V + 2);
+            auto write = [&](const float (&o)[8], int col) {
+                if (!on || col >= p.V) return;
+                if (whole) {
+                    uint4 y = make_uint4(Frag<T>::pack(o[0], o[1]), Frag<T>::pack(o[2], o[3]), Frag<T>::pack(o[4], o[5]), Frag<T>::pack(o[6], o[7]));
+                    if (!real) y = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + at_out * p.V + col) = y;
+                } else {
+                    *reinterpret_cast<float4*>(slot + row * p.V + col) = make_float4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<float4*>(slot + row * p.V + col + 4) = make_float4(o[4], o[5], o[6], o[7]);
+                }
+            };
+            f_own *= inv;
+            f_other *= inv;
 #pragma unroll 1
-            for (int c = c0; c < c1; c += 16) {
+            for (int c = c0; c < c1; c += add ? 16 : 32) {       // the sums of both halves, or 32 columns of this one's
                 tc_ld16(x[0], to + c);
-                if (add) tc_ld16(x[1], to_other + c);
+                tc_ld16(x[1], add ? to_other + c : to + c + 16);
                 tc_wait_ld(x[0]);
                 tc_wait_ld(x[1]);
-                if (!on) continue;
+                if (add) {
 #pragma unroll
-                for (int i = 0; i < 16; i += 8) {
-                    if (c + i >= p.V) break;
-                    float o[8];
+                    for (int i = 0; i < 16; i += 8) {
+                        float o[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        o[e] = __uint_as_float(x[0][i + e]);
-                        if (add) o[e] = o[e] * f_own + __uint_as_float(x[1][i + e]) * f_other;
-                        o[e] *= inv;
+                        for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(x[0][i + e]) * f_own + __uint_as_float(x[1][i + e]) * f_other;
+                        write(o, c + i);
                     }
-                    if (whole) {
-                        uint4 y = make_uint4(Frag<T>::pack(o[0], o[1]), Frag<T>::pack(o[2], o[3]), Frag<T>::pack(o[4], o[5]), Frag<T>::pack(o[6], o[7]));
-                        if (!real) y = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + at_out * p.V + c + i) = y;
-                    } else {
-                        *reinterpret_cast<float4*>(slot + row * p.V + c + i) = make_float4(o[0], o[1], o[2], o[3]);
-                        *reinterpret_cast<float4*>(slot + row * p.V + c + i + 4) = make_float4(o[4], o[5], o[6], o[7]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        float o[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(x[i >> 4][(i & 15) + e]) * f_own;
+                        write(o, c + i);
                     }
                 }
             }
