@@ -1150,6 +1150,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
     auto wait = [&](int bar, uint32_t parity) {
         if (!late && !mbar_wait_bounded(bars + bar, parity, kTcWaitCap)) late = true;      // (then nothing is waited for any more: wrong numbers, reported, no hang)
     };
+    // Tiles that have work: of a chain's drafts not those behind the row tile's last (they stand in the line all the same).
+    auto useful = [&](const Place& pl, int tiles) {
+        if (p.parents) return tiles;
+        const int rt = pl.unit - head_of(p, pl.unit) * p.row_tiles, last = min((int)p.group.div((uint32_t)(rt * p.rows + p.rows - 1)), p.N - 1);
+        return max(0, min(tiles, pl.tiles - p.draft_tiles + last / kTcTile + 1 - pl.tile));
+    };
     auto two_halves = [&](const Place& pl) { return p.N * p.G - (pl.unit - head_of(p, pl.unit) * p.row_tiles) * p.rows > 128 && p.rows > 128; };
 
     if (w >= kTcCopy) {
@@ -1189,8 +1195,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
             }
         };
         while (done < n_tiles) {
-            const int piece = min(n_tiles - done, at.tiles - at.tile), cached = at.tiles - p.draft_tiles, kv = head_of(p, at.unit);
+            const int share = min(n_tiles - done, at.tiles - at.tile), piece = useful(at, share), cached = at.tiles - p.draft_tiles, kv = head_of(p, at.unit);
             if (cw == 0) { bool b = false; draft_length(p, at.b, &b); bad |= b; }
+            if (piece == 0) {
+                done += share;
+                at.tile += share - 1;
+                at.next(p);
+                continue;
+            }
             const int row0 = (at.unit - kv * p.row_tiles) * p.rows, halves = two_halves(at) ? 2 : 1;
             wait(kQEmpty, (unit_no & 1) ^ 1);
             if (p.boxes & 2) {                            // whole drafts to a half: a box of the heads of 128 / G drafts
@@ -1334,9 +1346,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 tell(late_bar, late_bytes);
             }
             g += piece;
-            done += piece;
+            done += share;
             ++unit_no;
-            at.tile += piece - 1;
+            at.tile += share - 1;
             at.next(p);
         }
         if (last >= 0) {                                  // whatever happened: nothing is in flight when the block ends
@@ -1363,7 +1375,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
             int g = 0, unit_no = 0, done = 0;
             uint32_t had[2] = {0, 0};                     // jobs whose P a half has had
             while (done < n_tiles) {
-                const int piece = min(n_tiles - done, at.tiles - at.tile);
+                const int share = min(n_tiles - done, at.tiles - at.tile), piece = useful(at, share);
+                if (piece == 0) {
+                    done += share;
+                    at.tile += share - 1;
+                    at.next(p);
+                    continue;
+                }
                 // job i: half i & 1, tile i / 2 of the unit or (few rows) tile i
                 const int two = two_halves(at) ? 1 : 0, jobs = piece << two;
                 auto scores = [&](int i) {
@@ -1392,9 +1410,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                     if (i + 3 == jobs) tc_commit(bars + kQEmpty);
                 }
                 g += piece;
-                done += piece;
+                done += share;
                 ++unit_no;
-                at.tile += piece - 1;
+                at.tile += share - 1;
                 at.next(p);
             }
             tc_commit(bars + kDone);
@@ -1411,8 +1429,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
         uint32_t turns = 0, ends[2] = {0, 0};             // jobs of this half; units that either half had jobs of
         bool first_piece = true;
         while (done < n_tiles) {
-            const int piece = min(n_tiles - done, at.tiles - at.tile), cached = at.tiles - p.draft_tiles;
-            const bool whole = at.tile == 0 && piece == at.tiles, two = two_halves(at);
+            const int share = min(n_tiles - done, at.tiles - at.tile), piece = useful(at, share), cached = at.tiles - p.draft_tiles;
+            const bool whole = at.tile == 0 && share == at.tiles, two = two_halves(at);
             if (tid == 0 && at.tile == 0) leave_task(p, at, x0 + done, x0, blockIdx.x, line, whole);
             const int row = two ? half * 128 + lane_row : lane_row, jobs = two ? piece : (piece + 1 - half) >> 1;
             int n, h;
@@ -1576,12 +1594,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const bool had_any = two || i == 0 || piece > 1;
+                const bool had_any = piece > 0 && (two || i == 0 || piece > 1);
                 if (had_any) {
                     if (!two || i == half) wait(kOFull + i, ends[i] & 1u);
                     ++ends[i];
                 }
             }
+            if (piece == 0) tc_wait_st();
             tc_fence_after();
             const bool real = on && is_draft(p, at.b, n), add = !two;
             const float inv = whole ? (real ? finish_scale(mass) : 0.f) : 1.f;
@@ -1635,8 +1654,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
             }
             g += piece;
             first_piece = false;
-            done += piece;
-            at.tile += piece - 1;
+            done += share;
+            at.tile += share - 1;
             at.next(p);
         }
         tc_fence_before();

@@ -72,6 +72,14 @@ CASES = [
     (HF, 2, 4, 2, 32, 32, 256, [511, 512], True, 0), (HF, 9, 10, 2, 64, 128, 16, [65, 700], True, 0.2), (HF, 33, 12, 1, 128, 64, 5, [66], False, 0),
     (HF, 200, 3, 1, 64, 64, 16, [64, 190], True, 0.1), (HF, 1, 1, 1, 8, 8, 3, [5], False, 0), (BF, 4, 6, 2, 256, 192, 16, [140, 20], True, 0),
     (HF, 17, 40, 8, 80, 80, 16, [129, 64, 31], True, 0),
+    # 33 to 600 query rows: one and two halves of 128, ends inside a tile and inside a box of a page, several row tiles
+    (BF, 33, 1, 1, 64, 64, 16, [127, 128, 129], True, 0.1), (BF, 3, 16, 1, 128, 128, 128, [384, 385], True, 0), (HF, 5, 60, 2, 128, 64, 64, [200, 640, 0], True, 0.3),
+    (BF, 8, 32, 2, 64, 128, 32, [1000, 31], True, 0), (HF, 16, 32, 2, 96, 80, 48, [256, 100], True, 0), (BF, 43, 12, 2, 128, 128, 256, [700], False, 0),
+    (BF, 257, 4, 2, 128, 128, 16, [140, 3], False, 0), (HF, 600, 1, 1, 64, 64, 16, [0, 300], False, 0), (BF, 40, 16, 2, 128, 128, 7, [90], True, 0.2),
+    (BF, 144, 8, 1, 128, 128, 64, [128], True, 0.05), (HF, 20, 14, 2, 32, 96, 16, [333, 16], True, 0.9),
+    # fp32 with more than four rows of every width, and a 16-bit group that no box of heads fits
+    (FP, 4, 12, 1, 128, 128, 16, [70, 33], True, 0), (FP, 9, 4, 2, 64, 128, 5, [40], True, 0.2), (FP, 17, 8, 1, 64, 64, 16, [1000], False, 0),
+    (FP, 2, 2, 1, 96, 40, 16, [129, 0], True, 0), (BF, 30, 9, 3, 128, 128, 32, [260], True, 0.1),
 ]
 
 
@@ -84,7 +92,12 @@ def test_attention(dt, N, H, Hkv, K, V, page, lengths, is_tree, pad):
 @pytest.mark.parametrize("dt", [FP, BF, HF])
 def test_attention_of_many_splits_and_requests(dt):
     agrees(make(dt, 1, 4, 1, 64, 64, 16, [20000], seed=3))                                       # one unit over all blocks
-    agrees(make(dt, 2, 4, 2, 64, 64, 16, [(37 * i) % 300 for i in range(300)], seed=4), tree(300, 2))   # more requests than threads of a block
+    agrees(make(dt, 2, 4, 2, 64, 64, 16, [(37 * i) % 300 for i in range(300)], seed=4), tree(300, 2))   # more requests than threads of a warp
+    agrees(make(dt, 5, 8, 1, 64, 64, 16, [(91 * i) % 900 for i in range(150)], seed=5), tree(150, 5))
+    agrees(make(dt, 3, 40, 2, 128, 128, 16, [2500, 10, 1300], seed=6), tree(3, 3))
+    wide = make(dt, 3, 16, 2, 64, 64, 16, [100, 40], seed=7)                                     # a table of many more columns than are held
+    wide["block_table"] = torch.cat([wide["block_table"], torch.full((2, 1000), -1, dtype=torch.int32, device=DEV)], 1)
+    agrees(wide, tree(2, 3))
 
 
 @pytest.mark.parametrize("dt,scale", [(FP, 1.0), (BF, 2.0), (HF, -0.3), (BF, 0.0)])
