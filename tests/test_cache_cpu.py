@@ -51,7 +51,9 @@ def test_draft_attention_rejects_before_any_launch():
     assert _attend(_cache(K=264), _drafts()) == -8
     assert _attend(_cache(V=264), _drafts()) == -8
     assert _attend(_cache(), _drafts(N=1025, parents=P)) == -8
-    assert _attend(_cache(), _drafts(), ws_bytes=64) == -11
+    assert _attend(_cache(), _drafts(M=64, table_stride=64), ws_bytes=64) == -11      # (tables of a few hundred tokens need no more than a word)
+    need = _lib.lib().htree_b200_draft_workspace(ctypes.byref(_cache()), ctypes.byref(_drafts(M=64, table_stride=64)))
+    assert need > 64 and _attend(_cache(), _drafts(M=64, table_stride=64), ws_bytes=need - 1) == -11
     assert _lib.launch_count() == before
 
 
