@@ -239,193 +239,6 @@ __device__ __forceinline__ float finish_lse(float m, float mass) {
     return mass == 0.f ? -INFINITY : (m + log2f(mass)) * 0.69314718055994531f;
 }
 
-// ---- any type, any row width: fp32 arithmetic --------------------------------------------------------------------------------
-
-// 16 rows a block, four a warp; a warp's scores stay in it: lane x holds keys x and x + 32, and the columns 4x .. 4x + 3 (and + 128) of
-// the sums.
-constexpr int kGenRows = 16, kGenThreads = 128;
-
-template <typename T>
-__device__ __forceinline__ void load8(const char* src, float* dst) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
-        *reinterpret_cast<float4*>(dst) = a;
-        *reinterpret_cast<float4*>(dst + 4) = b;
-    } else {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(src));
-        const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = Frag<T>::unpack(u[i]);
-            dst[2 * i] = f.x;
-            dst[2 * i + 1] = f.y;
-        }
-    }
-}
-
-template <typename T, int VC>
-__global__ void __launch_bounds__(kGenThreads) draft_generic_kernel(const __grid_constant__ DraftParams p) {
-    extern __shared__ __align__(16) float smem[];
-    const int KS = p.K + 4, VS = VC * 128;
-    float* sk = smem;                               // [64][KS]: four floats on a row of eight threads meet in no bank
-    float* sv = sk + kTile * KS;                    // [64][VS], columns behind V zero
-    float* sq = sv + kTile * VS;                    // [16][K]
-    float* sp = sq + kGenRows * p.K;                // [16][64]
-    __shared__ uint64_t mask[kGenRows];
-    __shared__ uint8_t there[kTile];
-    chain_enter();
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-    Place at;
-    Line line;
-    int64_t x0, x1;
-    if (tid == 0 && !p.by_unit && !p.whole) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    if (!find_part<kGenThreads>(p, at, line, x0, x1)) return;
-    bool bad = false;
-    { bool b = false; draft_length(p, at.b, &b); bad |= b; }
-    float m[4], mass[4], o[4][4 * VC];
-    int first_tile = at.tile;                       // of the unit's part in this block
-    bool fresh = true, first_piece = true;
-    for (int64_t x = x0; x < x1; ++x) {
-        const int kv = head_of(p, at.unit);
-        if (fresh) {
-            first_tile = at.tile;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                m[r] = -INFINITY;
-                mass[r] = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4 * VC; ++i) o[r][i] = 0.f;
-            }
-            __syncthreads();
-            const int pieces = p.K / 8;
-            for (int i = tid; i < kGenRows * pieces; i += kGenThreads) {
-                const int r = i / pieces, c = i - r * pieces;
-                int n, h;
-                float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (row_of(p, at.unit, r, n, h)) load8<T>(p.q + at.b * p.q_b + n * p.q_n + h * p.q_h + c * 8 * (int)sizeof(T), f);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sq[r * p.K + c * 8 + e] = f[e];
-            }
-            fresh = false;
-        }
-        const bool draft = at.tile >= at.tiles - p.draft_tiles;
-        __syncthreads();
-        // two threads a key row
-        {
-            const int j = tid >> 1, half = tid & 1;
-            const char *k = nullptr, *v = nullptr;
-            const bool on = key_row(p, at, kv, j, k, v, &bad);
-            if (half == 0) there[j] = on;
-            for (int c = half; c < p.K / 8; c += 2) {
-                float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (on) load8<T>(k + c * 8 * (int)sizeof(T), f);
-                *reinterpret_cast<float4*>(sk + j * KS + c * 8) = make_float4(f[0], f[1], f[2], f[3]);
-                *reinterpret_cast<float4*>(sk + j * KS + c * 8 + 4) = make_float4(f[4], f[5], f[6], f[7]);
-            }
-            for (int c = half; c < VS / 8; c += 2) {
-                float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (on && c < p.V / 8) load8<T>(v + c * 8 * (int)sizeof(T), f);
-                *reinterpret_cast<float4*>(sv + j * VS + c * 8) = make_float4(f[0], f[1], f[2], f[3]);
-                *reinterpret_cast<float4*>(sv + j * VS + c * 8 + 4) = make_float4(f[4], f[5], f[6], f[7]);
-            }
-        }
-        if (draft && tid < kGenRows) {
-            int n, h;
-            mask[tid] = row_of(p, at.unit, tid, n, h) ? draft_mask(p, at.b, n, (at.tile - (at.tiles - p.draft_tiles)) * kTile, &bad) : 0ull;
-        }
-        __syncthreads();
-        float s[4][2];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[r][0] = s[r][1] = 0.f;
-        for (int d = 0; d < p.K; d += 4) {
-            const float4 a = *reinterpret_cast<const float4*>(sk + lane * KS + d), b = *reinterpret_cast<const float4*>(sk + (lane + 32) * KS + d);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float4 q = *reinterpret_cast<const float4*>(sq + (w * 4 + r) * p.K + d);
-                s[r][0] = fmaf(q.w, a.w, fmaf(q.z, a.z, fmaf(q.y, a.y, fmaf(q.x, a.x, s[r][0]))));
-                s[r][1] = fmaf(q.w, b.w, fmaf(q.z, b.z, fmaf(q.y, b.y, fmaf(q.x, b.x, s[r][1]))));
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint64_t seen = draft ? mask[w * 4 + r] : ~0ull;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int j = lane + 32 * i;
-                s[r][i] = there[j] && (seen >> j & 1) ? s[r][i] * p.c : -INFINITY;
-            }
-            const float top = fmaxf(m[r], warp_max(fmaxf(s[r][0], s[r][1]))), ref = top == -INFINITY ? 0.f : top;
-            const float keep = exp2f(m[r] - ref), e0 = exp2f(s[r][0] - ref), e1 = exp2f(s[r][1] - ref);
-            m[r] = top;
-            mass[r] = fmaf(mass[r], keep, e0 + e1);
-#pragma unroll
-            for (int i = 0; i < 4 * VC; ++i) o[r][i] *= keep;
-            sp[(w * 4 + r) * kTile + lane] = e0;
-            sp[(w * 4 + r) * kTile + lane + 32] = e1;
-        }
-        __syncwarp();
-        for (int j = 0; j < kTile; j += 4) {
-            float pr[4][4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) *reinterpret_cast<float4*>(pr[r]) = *reinterpret_cast<const float4*>(sp + (w * 4 + r) * kTile + j);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int c = 0; c < VC; ++c) {
-                    const float4 v = *reinterpret_cast<const float4*>(sv + (j + i) * VS + c * 128 + lane * 4);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if (draft && !(mask[w * 4 + r] >> (j + i) & 1)) continue;      // a draft's values, whatever they are, stay with those that read it
-                        o[r][4 * c] = fmaf(pr[r][i], v.x, o[r][4 * c]);
-                        o[r][4 * c + 1] = fmaf(pr[r][i], v.y, o[r][4 * c + 1]);
-                        o[r][4 * c + 2] = fmaf(pr[r][i], v.z, o[r][4 * c + 2]);
-                        o[r][4 * c + 3] = fmaf(pr[r][i], v.w, o[r][4 * c + 3]);
-                    }
-                }
-        }
-        __syncwarp();
-        const bool done = at.tile + 1 == at.tiles;
-        if (done || x + 1 == x1) {                  // the unit ends, or this block's part of it
-            const bool whole = done && first_tile == 0;
-            float* slot = p.part + (int64_t)(2 * blockIdx.x + (first_piece ? 0 : 1)) * kGenRows * (p.V + 2);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float sum = warp_sum(mass[r]);
-                int n, h;
-                if (!row_of(p, at.unit, w * 4 + r, n, h)) continue;
-                if (whole) {
-                    const bool real = is_draft(p, at.b, n);
-                    const float inv = real ? finish_scale(sum) : 0.f;
-                    const int64_t row = ((int64_t)at.b * p.N + n) * p.H + h;
-#pragma unroll
-                    for (int i = 0; i < 4 * VC; ++i) {
-                        const int c = (i / 4) * 128 + lane * 4 + (i & 3);
-                        if (c < p.V) reinterpret_cast<T*>(p.out)[row * p.V + c] = from_f<T>(real ? o[r][i] * inv : 0.f);
-                    }
-                    if (p.lse && lane == 0) p.lse[row] = real ? finish_lse(m[r], sum) : -INFINITY;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4 * VC; ++i) {
-                        const int c = (i / 4) * 128 + lane * 4 + (i & 3);
-                        if (c < p.V) slot[(w * 4 + r) * p.V + c] = o[r][i];
-                    }
-                    if (lane == 0) {
-                        slot[kGenRows * p.V + 2 * (w * 4 + r)] = m[r];
-                        slot[kGenRows * p.V + 2 * (w * 4 + r) + 1] = sum;
-                    }
-                }
-            }
-            if (tid == 0 && first_tile == 0) leave_task(p, at, x - at.tile, x0, blockIdx.x, line, whole);
-            first_piece = false;
-            fresh = true;
-        }
-        const int b = at.b;
-        at.next(p);
-        if (at.b != b) { bool d = false; draft_length(p, at.b, &d); bad |= d; }
-    }
-    if (bad && p.status) atomicOr(p.status, HTREE_STATUS_CACHE);
-}
-
 // ---- 16-bit types, up to 32 query rows: mma.sync ---------------------------------------------------------------------------------
 
 // HBM bounds these: the products only have to keep up.  A tile is 16 keys and belongs to one warp, with a softmax of its own (reference,
@@ -482,11 +295,12 @@ __device__ __forceinline__ float put_back(float o, const char* v, int col) {
 
 template <typename T, int DK, int DV, int R> struct SliceShape {          // R query rows
     static constexpr bool f32 = sizeof(T) == 4;
-    static constexpr int warps = R == 32 ? 8 : f32 && DK + DV > 192 ? 6 : f32 && DK + DV > 128 ? 8 : 12, threads = warps * 32, rows = R;
+    static constexpr int warps = DK + DV > 256 ? (f32 ? 3 : 6) : R == 32 ? 8 : f32 && DK + DV > 192 ? 6 : f32 && DK + DV > 128 ? 8 : 12;
+    static constexpr int threads = warps * 32, rows = R;
     static constexpr int krow = DK * (int)sizeof(T) + 16, vrow = DV * (int)sizeof(T) + 16;             // 16 bytes more than a row: eight rows meet in no bank
     static constexpr int stage = kSlice * (krow + vrow);
     // columns of a joining round: what fits into the stage that the unit's last tile has left
-    static constexpr int cols = DV == 128 && rows * 132 * 4 <= stage ? 128 : rows * 68 * 4 <= stage ? 64 : 32, jrow = cols + 4;
+    static constexpr int cols = f32 ? DV : DV == 128 && rows * 132 * 4 <= stage ? 128 : rows * 68 * 4 <= stage ? 64 : 32, jrow = cols + 4;
     static_assert(rows * jrow * 4 <= stage, "");
     static constexpr int weights = f32 ? warps * rows * kSlice * 4 : 0;
     static constexpr int fixed = 2 * warps * rows * 4 + (rows + 16) * 4 + rows * krow + weights;
@@ -547,9 +361,11 @@ __global__ void __launch_bounds__(SliceShape<T, DK, DV, ROWS>::threads, 1) draft
         const int pos = pl.tile * kSlice + (lane & 15);
         return pl.tile < pl.tiles - p.draft_tiles && pos < pl.len ? __ldg(p.table + (int64_t)pl.b * p.table_stride + p.page.div((uint32_t)pos)) : -1;
     };
-    constexpr int KL = DK / E, VL = DV / E;              // lanes of a row
+    constexpr int KP = DK > 32 * E ? DK / (32 * E) : 1, VP = DV > 32 * E ? DV / (32 * E) : 1;                 // pieces of a row of a lane,
+    constexpr int KL = DK / E / KP, VL = DV / E / VP;                                                         // 32 apart; lanes of a row
     const uint32_t kdst = ring_u + lane / KL * S::krow + lane % KL * 16, vdst = ring_u + kSlice * S::krow + lane / VL * S::vrow + lane % VL * 16;
-    const bool kcol = lane % KL * E < p.K, vcol = lane % VL * E < p.V;
+    auto kcol = [&](int h) { return (lane % KL + 32 * h) * E < p.K; };
+    auto vcol = [&](int h) { return (lane % VL + 32 * h) * E < p.V; };
     const int64_t kstep = p.ck_row * (32 / KL), vstep = p.cv_row * (32 / VL);
     uint64_t keys_of = 0;                  // which keys a stage has: 16 bits each
 
@@ -759,12 +575,20 @@ __global__ void __launch_bounds__(SliceShape<T, DK, DV, ROWS>::threads, 1) draft
                 // sixteen tokens of one page (the same one in every lane)
                 const char* ks = p.ck + page_of * p.ck_page + (in0 + lane / KL) * p.ck_row + kv * p.ck_h + lane % KL * 16;
                 const char* vs = p.cv + page_of * p.cv_page + (in0 + lane / VL) * p.cv_row + kv * p.cv_h + lane % VL * 16;
-                if (kcol)
 #pragma unroll
-                    for (int i = 0; i < kSlice * KL / 32; ++i, ks += kstep) cp_async16(kd + i * (32 / KL) * S::krow, ks);
-                if (vcol)
+                for (int h = 0; h < KP; ++h) {
+                    const char* src = ks + h * 512;
+                    if (kcol(h))
 #pragma unroll
-                    for (int i = 0; i < kSlice * VL / 32; ++i, vs += vstep) cp_async16(vd + i * (32 / VL) * S::vrow, vs);
+                        for (int i = 0; i < kSlice * KL / 32; ++i, src += kstep) cp_async16(kd + i * (32 / KL) * S::krow + h * 512, src);
+                }
+#pragma unroll
+                for (int h = 0; h < VP; ++h) {
+                    const char* src = vs + h * 512;
+                    if (vcol(h))
+#pragma unroll
+                        for (int i = 0; i < kSlice * VL / 32; ++i, src += vstep) cp_async16(vd + i * (32 / VL) * S::vrow + h * 512, src);
+                }
             } else {
                 const char *ks = p.q, *vs = p.q;         // (a row that is not there has no source)
                 bool on = false;
@@ -790,13 +614,17 @@ __global__ void __launch_bounds__(SliceShape<T, DK, DV, ROWS>::threads, 1) draft
                 for (int i = 0; i < kSlice * KL / 32; ++i) {
                     const int j = i * (32 / KL) + lane / KL;
                     const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ks), j));
-                    if (kcol) cp_async16_or_zero(kd + i * (32 / KL) * S::krow, (m >> j & 1) ? src + lane % KL * 16 : p.q, m >> j & 1);
+#pragma unroll
+                    for (int h = 0; h < KP; ++h)
+                        if (kcol(h)) cp_async16_or_zero(kd + i * (32 / KL) * S::krow + h * 512, (m >> j & 1) ? src + lane % KL * 16 + h * 512 : p.q, m >> j & 1);
                 }
 #pragma unroll 1
                 for (int i = 0; i < kSlice * VL / 32; ++i) {
                     const int j = i * (32 / VL) + lane / VL;
                     const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vs), j));
-                    if (vcol) cp_async16_or_zero(vd + i * (32 / VL) * S::vrow, (m >> j & 1) ? src + lane % VL * 16 : p.q, m >> j & 1);
+#pragma unroll
+                    for (int h = 0; h < VP; ++h)
+                        if (vcol(h)) cp_async16_or_zero(vd + i * (32 / VL) * S::vrow + h * 512, (m >> j & 1) ? src + lane % VL * 16 + h * 512 : p.q, m >> j & 1);
                 }
             }
             keys_of = (keys_of & ~(0xffffull << (16 * stage))) | (uint64_t)m << (16 * stage);
@@ -871,8 +699,10 @@ __global__ void __launch_bounds__(SliceShape<T, DK, DV, ROWS>::threads, 1) draft
                 float x[4][CW];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if constexpr (CW == 4) *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(vv + (j + i) * (S::vrow / 4));
-                    else *reinterpret_cast<float2*>(x[i]) = *reinterpret_cast<const float2*>(vv + (j + i) * (S::vrow / 4));
+                    if constexpr (CW >= 4) {
+#pragma unroll
+                        for (int c = 0; c < CW; c += 4) *reinterpret_cast<float4*>(x[i] + c) = *reinterpret_cast<const float4*>(vv + (j + i) * (S::vrow / 4) + c);
+                    } else *reinterpret_cast<float2*>(x[i]) = *reinterpret_cast<const float2*>(vv + (j + i) * (S::vrow / 4));
                 }
 #pragma unroll
                 for (int r = 0; r < ROWS; ++r) {
@@ -1004,6 +834,216 @@ __global__ void __launch_bounds__(SliceShape<T, DK, DV, ROWS>::threads, 1) draft
             }
         }
     }
+}
+
+// ---- fp32, more than 16 query rows: FFMA -------------------------------------------------------------------------------------
+
+// 64 query rows a block against tiles of 64 keys, four warps of 16 rows each.  A thread has 8 rows and, of the scores, the keys
+// kg, kg + 16, .. of the tile, of the sums the columns 4 cg .. 4 cg + 3 of every 64 (kg = cg = lane & 15): per 64 products it reads 4 to 6
+// times 16 bytes of shared memory, so that the FMA pipes bound it and not the reads.  A warp's weights stay in it.  The keys of the next tile come
+// by cp.async while the values are multiplied, the values while the scores are; pieces of 16 bytes are swizzled so that the lanes of a
+// read meet in no bank.
+constexpr int kFmaRows = 64, kFmaThreads = 128;
+template <int D> struct FmaShape {
+    static constexpr int q = 0, k = q + kFmaRows * D * 4, v = k + kTile * D * 4, p = v + kTile * D * 4, mask = p + kFmaRows * kTile * 4,
+                         there = mask + kFmaRows * 8, total = there + 16;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kFmaThreads, D > 128 ? 1 : 2) draft_fma_kernel(const __grid_constant__ DraftParams p) {
+    using S = FmaShape<D>;
+    constexpr int CJ = D / 64;                          // float4s of a thread's columns
+    extern __shared__ __align__(128) unsigned char sm[];
+    uint64_t* mask = reinterpret_cast<uint64_t*>(sm + S::mask);              // which drafts of the tile a row reads
+    uint16_t* there = reinterpret_cast<uint16_t*>(sm + S::there);            // [2][4]: which keys the tile has, this tile's and the next one's
+    const uint32_t base = smem_u32(sm);
+    chain_enter();
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rg = lane >> 4, kg = lane & 15;
+    Place at;
+    Line line;
+    int64_t x0, x1;
+    if (tid == 0 && !p.by_unit && !p.whole) p.tasks[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (!find_part<kFmaThreads>(p, at, line, x0, x1)) return;
+    bool bad = false;
+    { bool b = false; draft_length(p, at.b, &b); bad |= b; }
+    // Where the keys and values of a tile are: lane j (and j + 16) knows key 16 w + j.
+    const char *kp = nullptr, *vp = nullptr;
+    uint32_t has = 0;
+    auto look = [&](const Place& pl, int buf) {
+        kp = vp = p.q;
+        has = __ballot_sync(0xffffffffu, key_row(p, pl, head_of(p, pl.unit), w * 16 + kg, kp, vp, &bad)) & 0xffffu;
+        if (lane == 0) there[buf * 4 + w] = (uint16_t)has;
+    };
+    // ... and this warp's sixteen of them, to shared memory
+    auto copy = [&](const char* rows, uint32_t dst, int width, bool swizzled) {
+#pragma unroll 4
+        for (int j = 0; j < 16; ++j) {
+            const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(rows), j));
+            const bool on = has >> j & 1;
+            for (int c = lane; c * 4 < width; c += 32)
+                cp_async16_or_zero(dst + (w * 16 + j) * (D * 4) + (swizzled ? c ^ (j & 7) : c) * 16, on ? src + c * 16 : p.q, on);
+        }
+        cp_async_commit();
+    };
+    look(at, 0);
+    copy(kp, base + S::k, p.K, true);
+    float m[8], mass[8], o[8][CJ * 4];
+    int first_tile = at.tile;                           // of the unit's part in this block
+    bool fresh = true, first_piece = true;
+    int buf = 0;
+    const float* sq = reinterpret_cast<const float*>(sm + S::q) + (w * 16 + rg * 8) * D;
+    const float* sk = reinterpret_cast<const float*>(sm + S::k) + kg * D;
+    const float* sv = reinterpret_cast<const float*>(sm + S::v) + kg * 4;
+    float* sp = reinterpret_cast<float*>(sm + S::p) + w * (16 * kTile) + rg * 8;              // [key][16 rows]
+    for (int64_t x = x0; x < x1; ++x, buf ^= 1) {
+        if (fresh) {
+            fresh = false;
+            first_tile = at.tile;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                m[r] = -INFINITY;
+                mass[r] = 0.f;
+#pragma unroll
+                for (int i = 0; i < CJ * 4; ++i) o[r][i] = 0.f;
+            }
+#pragma unroll 1
+            for (int j = 0; j < 16; ++j) {
+                int n, h;
+                const bool on = row_of(p, at.unit, w * 16 + j, n, h);
+                for (int c = lane; c * 4 < p.K; c += 32)
+                    cp_async16_or_zero(base + S::q + (w * 16 + j) * (D * 4) + (c ^ (j >> 3)) * 16, on ? p.q + at.b * p.q_b + n * p.q_n + h * p.q_h + c * 16 : p.q, on);
+            }
+            cp_async_commit();
+        }
+        copy(vp, base + S::v, p.V, false);
+        const int cached = at.tiles - p.draft_tiles, tile0 = (at.tile - cached) * kTile;
+        const bool draft = tile0 >= 0;
+        bool idle = false;                              // a chain's drafts behind the rows of this tile
+        if (draft) {
+            int n, h;
+            if (tid < kFmaRows) mask[tid] = row_of(p, at.unit, tid, n, h) ? draft_mask(p, at.b, n, tile0, &bad) : 0ull;
+            (void)row_of(p, at.unit, kFmaRows - 1, n, h);
+            idle = !p.parents && tile0 > n;
+        }
+        cp_async_wait<1>();                             // the keys, and q
+        __syncthreads();
+        if (!idle) {
+            float s[8][4];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[r][j] = 0.f;
+#pragma unroll 2
+            for (int c = 0; c < p.K / 4; ++c) {
+                float4 a[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) a[j] = *reinterpret_cast<const float4*>(sk + j * 16 * D + (c ^ (kg & 7)) * 4);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const float4 y = *reinterpret_cast<const float4*>(sq + r * D + (c ^ rg) * 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[r][j] = fmaf(y.w, a[j].w, fmaf(y.z, a[j].z, fmaf(y.y, a[j].y, fmaf(y.x, a[j].x, s[r][j]))));
+                }
+            }
+            const uint64_t keys = *reinterpret_cast<const uint64_t*>(there + buf * 4);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const uint64_t seen = (draft ? keys & mask[w * 16 + rg * 8 + r] : keys) >> kg;
+                float top = m[r];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[r][j] = (seen >> (16 * j) & 1) ? s[r][j] * p.c : -INFINITY;
+                    top = fmaxf(top, s[r][j]);
+                }
+#pragma unroll
+                for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float ref = top == -INFINITY ? 0.f : top, keep = ex2_approx(m[r] - ref);
+                m[r] = top;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[r][j] = ex2_approx(s[r][j] - ref);
+                mass[r] = fmaf(mass[r], keep, (s[r][0] + s[r][1]) + (s[r][2] + s[r][3]));
+                if (keep != 1.f)
+#pragma unroll
+                    for (int i = 0; i < CJ * 4; ++i) o[r][i] *= keep;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int r = 0; r < 8; r += 4) *reinterpret_cast<float4*>(sp + (kg + 16 * j) * 16 + r) = make_float4(s[r][j], s[r + 1][j], s[r + 2][j], s[r + 3][j]);
+        }
+        __syncthreads();                                // all have read the keys
+        Place next = at;
+        if (x + 1 < x1) {
+            next.next(p);
+            if (next.b != at.b) { bool d = false; draft_length(p, next.b, &d); bad |= d; }
+            look(next, buf ^ 1);
+            copy(kp, base + S::k, p.K, true);
+        } else {
+            cp_async_commit();
+        }
+        cp_async_wait<1>();                             // the values
+        __syncthreads();
+        if (!idle) {
+            auto add = [&](auto some) {
+#pragma unroll 4
+                for (int key = 0; key < kTile; ++key) {
+                    float y[8];
+                    *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(sp + key * 16);
+                    *reinterpret_cast<float4*>(y + 4) = *reinterpret_cast<const float4*>(sp + key * 16 + 4);
+#pragma unroll
+                    for (int i = 0; i < CJ; ++i) {
+                        const float4 a = *reinterpret_cast<const float4*>(sv + key * D + i * 64);
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) {
+                            // (a draft's values, whatever they are, stay with those that read it)
+                            if (decltype(some)::value && !(mask[w * 16 + rg * 8 + r] >> key & 1)) continue;
+                            o[r][4 * i] = fmaf(y[r], a.x, o[r][4 * i]);
+                            o[r][4 * i + 1] = fmaf(y[r], a.y, o[r][4 * i + 1]);
+                            o[r][4 * i + 2] = fmaf(y[r], a.z, o[r][4 * i + 2]);
+                            o[r][4 * i + 3] = fmaf(y[r], a.w, o[r][4 * i + 3]);
+                        }
+                    }
+                }
+            };
+            if (draft) add(std::true_type{}); else add(std::false_type{});
+        }
+        const bool done = at.tile + 1 == at.tiles;
+        if (done || x + 1 == x1) {                      // the unit ends, or this block's part of it
+            const bool whole = done && first_tile == 0;
+            float* slot = p.part + (int64_t)(2 * blockIdx.x + (first_piece ? 0 : 1)) * kFmaRows * (p.V + 2);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                float sum = mass[r];
+#pragma unroll
+                for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                const int row = w * 16 + rg * 8 + r;
+                int n, h;
+                if (!row_of(p, at.unit, row, n, h)) continue;
+                const bool real = is_draft(p, at.b, n);
+                const float inv = whole ? (real ? finish_scale(sum) : 0.f) : 1.f;
+                const int64_t at_out = ((int64_t)at.b * p.N + n) * p.H + h;
+                float* to = whole ? reinterpret_cast<float*>(p.out) + at_out * p.V : slot + row * p.V;
+#pragma unroll
+                for (int i = 0; i < CJ; ++i) {
+                    const int col = i * 64 + kg * 4;
+                    if (col >= p.V) continue;
+                    float4 y = make_float4(o[r][4 * i] * inv, o[r][4 * i + 1] * inv, o[r][4 * i + 2] * inv, o[r][4 * i + 3] * inv);
+                    if (whole && !real) y = make_float4(0.f, 0.f, 0.f, 0.f);
+                    *reinterpret_cast<float4*>(to + col) = y;
+                }
+                if (kg == 0) {
+                    if (!whole) *reinterpret_cast<float2*>(slot + kFmaRows * p.V + 2 * row) = make_float2(m[r], sum);
+                    else if (p.lse) p.lse[at_out] = real ? finish_lse(m[r], sum) : -INFINITY;
+                }
+            }
+            if (tid == 0 && first_tile == 0) leave_task(p, at, x - at.tile, x0, blockIdx.x, line, whole);
+            first_piece = false;
+            fresh = true;
+        }
+        at = next;
+        __syncthreads();                                // the values and masks have been read
+    }
+    if (bad && p.status) atomicOr(p.status, HTREE_STATUS_CACHE);
 }
 
 // ---- 16-bit types, more than 32 query rows: tcgen05 -----------------------------------------------------------------------------------
@@ -1770,11 +1810,6 @@ __global__ void __launch_bounds__(kJoinThreads) draft_join_kernel(const __grid_c
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------
 
-static size_t generic_smem(const DraftParams& p) {
-    const int VS = p.V > 128 ? 256 : 128;
-    return ((size_t)kTile * (p.K + 4) + (size_t)kTile * VS + (size_t)kGenRows * p.K + (size_t)kGenRows * kTile) * 4;
-}
-
 static int64_t units_of(const DraftParams& p) { return (int64_t)p.B * p.Hkv * p.row_tiles; }
 
 // least: tiles that a part has at least (a block's warps, each of which takes one at a time).
@@ -1789,7 +1824,7 @@ static void fit(DraftParams& p, int rows, int tile, int blocks, int least) {
     // With tables so short that a block is done with any unit in two rounds of its warps (tcgen05: in four tiles), parts are whole units, and
     // the second kernel, 4 of 15 us of a small call, falls away.
     const int most = ((p.room + tile - 1) >> p.shift) + p.draft_tiles;
-    p.whole = most <= (tile == kTcTile ? 4 : 2 * least);
+    p.whole = most <= (tile == kSlice ? 2 * least : 4);
     if (p.whole && units_of(p) < p.grid) p.grid = (int32_t)units_of(p);
     p.by_unit = units_of(p) <= p.grid;
     const int64_t each = p.grid / units_of(p);         // parts of a unit
@@ -1801,22 +1836,19 @@ static int64_t workspace_of(const DraftParams& p) { return p.whole ? 16 : part_b
 // Which kernel: 16-bit rows of up to 128 go to the tensor cores, by mma.sync up to 32 query rows, up to 16 with rows of more than 64 (where
 // a warp of 32 has spills).  Measured, 8 requests of 16384, 4 heads of 128: 32 rows 84 us on mma.sync and 70 on tcgen05, 16 rows 63 and
 // 70; 8 heads of 64: 32 rows 78 and 97; 8 requests of 1000, 4 heads of 128: 32 rows 25 and 27, 16 rows 20 and 27.
-enum { kGeneric = 0, kSlice4, kSlice16, kSlice32, kTc };
+enum { kSlice4 = 0, kSlice16, kSlice32, kFma, kTc };
 static void choose(DraftParams& p, int dtype) {
     const int sms = sm_count() > 0 ? sm_count() : 148, rows = p.N * p.G;
-    if (p.K > 128 || p.V > 128) {
-        p.variant = kGeneric;
-        fit(p, kGenRows, kTile, sms * (generic_smem(p) <= 110 * 1024 ? 2 : 1), 1);
-        return;
-    }
+    const bool wide = p.K > 128 || p.V > 128;
     if (dtype == HTREE_F32) {
-        p.variant = rows <= 4 ? kSlice4 : kSlice16;
-        fit(p, rows <= 4 ? 4 : 16, kSlice, sms, p.K > 64 && p.V > 64 ? 6 : p.K > 64 || p.V > 64 ? 8 : 12);
+        p.variant = rows <= 4 ? kSlice4 : rows <= 16 ? kSlice16 : kFma;
+        if (p.variant == kFma) fit(p, kFmaRows, kTile, wide ? sms : 2 * sms, 1);
+        else fit(p, rows <= 4 ? 4 : 16, kSlice, sms, wide ? 3 : p.K > 64 && p.V > 64 ? 6 : p.K > 64 || p.V > 64 ? 8 : 12);
         return;
     }
-    p.variant = rows <= 16 ? kSlice16 : rows <= 32 && p.K <= 64 && p.V <= 64 ? kSlice32 : kTc;
+    p.variant = wide || rows <= 16 ? kSlice16 : rows <= 32 && p.K <= 64 && p.V <= 64 ? kSlice32 : kTc;
     if (p.variant == kTc) fit(p, rows <= 128 ? 128 : 256, kTcTile, sms, 1);
-    else fit(p, rows <= 16 ? 16 : 32, kSlice, sms, rows <= 16 ? 12 : 8);
+    else fit(p, p.variant == kSlice16 ? 16 : 32, kSlice, sms, wide ? 6 : p.variant == kSlice16 ? 12 : 8);
     if (p.c < 0.f) { p.neg = 1; p.c = -p.c; }
     if (p.c < 1.1754944e-38f) p.c = 1.1754944e-38f;        // a scale of zero: scores of zero, but what is masked stays minus infinity
 }
@@ -1892,22 +1924,25 @@ static int launch_sized(const DraftParams& p, cudaStream_t st) {
 }
 
 template <typename T>
-static int launch_generic(const DraftParams& p, cudaStream_t st) {
-    static SmemLimit limit1, limit2;
-    const size_t smem = generic_smem(p);
-    if (p.V <= 128) {
-        if (const cudaError_t e = limit1.raise((const void*)draft_generic_kernel<T, 1>, smem)) return (int)e;
-        return launch_chained(draft_generic_kernel<T, 1>, dim3(p.grid), dim3(kGenThreads), smem, st, p);
-    }
-    if (const cudaError_t e = limit2.raise((const void*)draft_generic_kernel<T, 2>, smem)) return (int)e;
-    return launch_chained(draft_generic_kernel<T, 2>, dim3(p.grid), dim3(kGenThreads), smem, st, p);
+static int launch_wide(const DraftParams& p, cudaStream_t st) {
+    if constexpr (sizeof(T) == 4)
+        if (p.variant == kSlice4) return launch_slices<T, 256, 256, 4>(p, st);
+    return launch_slices<T, 256, 256, 16>(p, st);
+}
+template <int D>
+static int launch_fma(const DraftParams& p, cudaStream_t st) {
+    static SmemLimit limit;
+    if (const cudaError_t e = limit.raise((const void*)draft_fma_kernel<D>, FmaShape<D>::total)) return (int)e;
+    return launch_chained(draft_fma_kernel<D>, dim3(p.grid), dim3(kFmaThreads), FmaShape<D>::total, st, p);
 }
 
 template <typename T>
 static int launch_draft(const DraftParams& p, cudaStream_t st) {
-    const int rc = p.variant == kGeneric ? launch_generic<T>(p, st)
-                 : p.K <= 64 ? (p.V <= 64 ? launch_sized<T, 64, 64>(p, st) : launch_sized<T, 64, 128>(p, st))
-                             : (p.V <= 64 ? launch_sized<T, 128, 64>(p, st) : launch_sized<T, 128, 128>(p, st));
+    const bool k64 = p.K <= 64, v64 = p.V <= 64;
+    int rc;
+    if (p.variant == kFma) rc = k64 && v64 ? launch_fma<64>(p, st) : p.K <= 128 && p.V <= 128 ? launch_fma<128>(p, st) : launch_fma<256>(p, st);
+    else if (p.K > 128 || p.V > 128) rc = launch_wide<T>(p, st);
+    else rc = k64 ? (v64 ? launch_sized<T, 64, 64>(p, st) : launch_sized<T, 64, 128>(p, st)) : v64 ? launch_sized<T, 128, 64>(p, st) : launch_sized<T, 128, 128>(p, st);
     if (rc || p.whole) return rc;
     const int rows = p.N * p.G < p.rows ? p.N * p.G : p.rows, block = kJoinWarps / p.team;
     const dim3 grid(p.by_unit ? (unsigned)units_of(p) : (unsigned)p.grid, (rows + block - 1) / block);

@@ -80,6 +80,13 @@ CASES = [
     # fp32 with more than four rows of every width, and a 16-bit group that no box of heads fits
     (FP, 4, 12, 1, 128, 128, 16, [70, 33], True, 0), (FP, 9, 4, 2, 64, 128, 5, [40], True, 0.2), (FP, 17, 8, 1, 64, 64, 16, [1000], False, 0),
     (FP, 2, 2, 1, 96, 40, 16, [129, 0], True, 0), (BF, 30, 9, 3, 128, 128, 32, [260], True, 0.1),
+    # rows wider than 128, keys and values of different widths among them, in few and many parts
+    (BF, 1, 8, 1, 256, 256, 16, [3000, 17], False, 0), (HF, 1, 4, 2, 192, 128, 64, [640], False, 0), (BF, 7, 10, 2, 136, 256, 5, [300, 0], True, 0.2),
+    (HF, 40, 6, 2, 8, 248, 16, [77], True, 0.1), (FP, 1, 4, 1, 256, 256, 16, [2000, 3], False, 0), (FP, 2, 2, 1, 144, 8, 3, [250], True, 0),
+    (FP, 3, 10, 2, 200, 256, 16, [500], True, 0.2), (FP, 11, 2, 2, 16, 256, 1, [100, 40], False, 0), (FP, 40, 2, 1, 256, 192, 32, [333], True, 0.1),
+    # fp32 with more than sixteen rows: parts of one and of several row tiles of 64
+    (FP, 64, 1, 1, 128, 128, 64, [1000, 64], True, 0), (FP, 130, 2, 1, 64, 64, 16, [129, 0, 500], False, 0), (FP, 70, 3, 1, 96, 128, 7, [260], True, 0.3),
+    (FP, 20, 8, 2, 32, 24, 16, [63, 65], True, 0.5), (FP, 300, 4, 4, 128, 128, 16, [40], False, 0),
 ]
 
 
