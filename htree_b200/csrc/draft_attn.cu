@@ -193,22 +193,35 @@ __device__ __forceinline__ bool row_of(const DraftParams& p, int unit, int r, in
     return row < p.N * p.G;
 }
 
-// Which of the drafts tile0 .. tile0 + 63 draft n reads.
-__device__ __forceinline__ uint64_t draft_mask(const DraftParams& p, int b, int n, int tile0, bool* bad) {
+// Which of the drafts tile0 .. tile0 + 64 * W - 1 draft n reads.
+template <int W>
+__device__ __forceinline__ void draft_masks(const DraftParams& p, int b, int n, int tile0, uint64_t (&m)[W], bool* bad) {
     if (!p.parents) {                                        // a chain: n and all before it
-        const int upto = n - tile0;
-        return upto < 0 ? 0ull : upto >= 63 ? ~0ull : (2ull << upto) - 1ull;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const int upto = n - tile0 - 64 * i;
+            m[i] = upto < 0 ? 0ull : upto >= 63 ? ~0ull : (2ull << upto) - 1ull;
+        }
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < W; ++i) m[i] = 0;
     const int32_t* par = p.parents + (int64_t)b * p.N;
-    if (par[n] < -1) return 0ull;
-    uint64_t m = 0;
-    for (int i = n; i >= tile0;) {                           // parents come before their children: at most n steps
-        if (i < tile0 + 64) m |= 1ull << (i - tile0);
-        const int up = par[i];
-        if (up >= i) { *bad = true; break; }
+    int up = par[n];
+    if (up < -1) return;
+    for (int i = n; i >= tile0; up = par[i]) {               // parents come before their children: at most n steps
+        const uint64_t bit = 1ull << ((i - tile0) & 63);
+#pragma unroll
+        for (int j = 0; j < W; ++j) if ((i - tile0) >> 6 == j) m[j] |= bit;
+        if (up >= i) { *bad = true; return; }
         i = up;
+        if (i < tile0) return;
     }
-    return m;
+}
+__device__ __forceinline__ uint64_t draft_mask(const DraftParams& p, int b, int n, int tile0, bool* bad) {
+    uint64_t m[1];
+    draft_masks(p, b, n, tile0, m, bad);
+    return m[0];
 }
 __device__ __forceinline__ bool is_draft(const DraftParams& p, int b, int n) { return !p.parents || p.parents[(int64_t)b * p.N + n] >= -1; }
 
@@ -1492,8 +1505,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 for (int c = 0; c < 4; ++c) seen[c] = valid[(gg & 7) * 4 + c];
                 if (tile >= cached) {
                     const int tile0 = (tile - cached) * kTcTile;
-                    const uint64_t lo = on ? draft_mask(p, at.b, n, tile0, &bad) : 0ull, hi = on ? draft_mask(p, at.b, n, tile0 + 64, &bad) : 0ull;
-                    seen[0] &= (uint32_t)lo; seen[1] &= (uint32_t)(lo >> 32); seen[2] &= (uint32_t)hi; seen[3] &= (uint32_t)(hi >> 32);
+                    uint64_t own[2] = {0, 0};
+                    if (on) draft_masks(p, at.b, n, tile0, own, &bad);
+                    seen[0] &= (uint32_t)own[0]; seen[1] &= (uint32_t)(own[0] >> 32); seen[2] &= (uint32_t)own[1]; seen[3] &= (uint32_t)(own[1] >> 32);
                 }
                 uint32_t pk[64];
                 float2 sums[2];
