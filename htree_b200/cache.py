@@ -53,7 +53,8 @@ def cache_plan(lengths: torch.Tensor, counts: torch.Tensor, block_table: torch.T
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
                  index: Optional[torch.Tensor] = None) -> None:
     """Rows of k [B, N, H_kv, K] and v [B, N, H_kv, V] into their slots [B, n] (-1: not written): token i of request b, or token
-    index[b, i] (int32), e.g. the accepted drafts.  Slots of one call have to differ: of tokens that share one, any may be kept."""
+    index[b, i] (int32), e.g. the accepted drafts.  Slots of one call have to differ: of tokens that share one, any may be kept.  k and v
+    must not lie in the cache themselves."""
     _glue(k_cache).cache_append(k, v, k_cache, v_cache, slots, index, _status(k_cache.device))
 
 

@@ -94,6 +94,12 @@ void check_new(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cac
     TORCH_CHECK_VALUE(k.size(0) <= INT32_MAX && k.size(1) <= INT32_MAX, "too many tokens");
 }
 
+// What a call has written: saved for somebody's backward, it has changed since.
+void written(std::initializer_list<const at::Tensor*> ts) {
+    for (const at::Tensor* t : ts)
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 int32_t* status_of(const at::Tensor& status) { return status.data_ptr<int32_t>(); }
 
 std::tuple<at::Tensor, at::Tensor> cache_plan(const at::Tensor& lengths, const at::Tensor& counts, const at::Tensor& table, const at::Tensor& pool,
@@ -117,6 +123,7 @@ std::tuple<at::Tensor, at::Tensor> cache_plan(const at::Tensor& lengths, const a
                                 table.data_ptr<int32_t>(), table_stride(table), pool.data_ptr<int32_t>(), (int32_t)pool.size(0), top.data_ptr<int32_t>(),
                                 slots.data_ptr<int64_t>(), taken.data_ptr<int32_t>(), status_of(status), stream()),
           "cache_plan");
+    written({&lengths, &table, &pool, &top});
     return {slots, taken};
 }
 
@@ -145,6 +152,7 @@ void cache_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_
     check(htree_b200_cache_append(&cache, (int32_t)B, (int32_t)N, (int32_t)n, kk.data_ptr(), ks, vv.data_ptr(), vs, s.data_ptr<int64_t>(),
                                   idx.defined() ? idx.data_ptr<int32_t>() : nullptr, status_of(status), stream()),
           "cache_append");
+    written({&k_cache, &v_cache});
 }
 
 std::tuple<at::Tensor, at::Tensor> cache_gather(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& table, const at::Tensor& lengths,

@@ -364,6 +364,27 @@ def test_append_and_gather(dt, Hkv, K, V, page):
             assert torch.equal(a[i, :counts[i]], k[i, :counts[i]]) and torch.equal(b[i, :counts[i]], v[i, :counts[i]])
 
 
+def test_what_is_written_is_known_to_autograd():
+    """A tensor saved for a backward pass and written since is an error there, not a wrong gradient."""
+    import htree_b200 as ht
+    kc, vc = torch.ones(4, 8, 1, 16, device=DEV), torch.ones(4, 8, 1, 16, device=DEV)
+    k = torch.zeros(1, 1, 1, 16, device=DEV)
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    loss = (w * kc).sum()
+    ht.cache_append(k, k, kc, vc, torch.zeros(1, 1, dtype=torch.int64, device=DEV))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    lengths, table, pool, top = _ints([0]), _ints([[-1, -1]]), _ints([0, 1]), _ints([2])
+    before = [x._version for x in (lengths, table, pool, top)]
+    ht.cache_plan(lengths, _ints([3]), table, pool, top, 8, 3)
+    assert all(x._version > n for x, n in zip((lengths, table, pool, top), before))
+    with torch.inference_mode():
+        kc = torch.ones(4, 8, 1, 16, device=DEV)
+        ht.cache_append(k, k, kc, kc.clone(), torch.zeros(1, 1, dtype=torch.int64, device=DEV))
+    ht.cache_append(k, k, kc, torch.ones_like(kc), torch.ones(1, 1, dtype=torch.int64, device=DEV))
+    assert kc[0, :2].abs().sum() == 0
+
+
 def test_parts_join_by_their_lse():
     """Attention over two halves of 320 tokens (the last of each as the draft), joined by lse, is attention over the whole."""
     import htree_b200 as ht
