@@ -259,8 +259,9 @@ __device__ __forceinline__ float finish_lse(float m, float mass) {
 
 // ---- few query rows, and rows wider than 128: slices of keys ------------------------------------------------------------------
 
-// HBM bounds these (fp32 with 16 rows: the FMA pipes); the products only have to keep up: mma.sync in 16 bits, FFMA in fp32.  Measured, 32
-// requests of 16384, 8 heads of the cache, 4 query heads each: 128 wide in bf16 6.1 TB/s.  A tile is 16 keys and belongs to one warp, with a softmax of its own (reference,
+// HBM bounds these (fp32 with more than 4 rows: the FMA pipes, at 11 to 15 TFLOP/s); the products only have to keep up: mma.sync in 16
+// bits, FFMA in fp32.  Measured, 32 requests, 8 heads of the cache, 4 query heads each: 16384 tokens of 128 in 359 us in bf16 (6.0 TB/s)
+// and 762 in fp32 (5.6), of 64 in 213 and 413 (5.0 and 5.2), 8192 of 256 in 373 and 938 (5.8 and 4.6).  A tile is 16 keys and belongs to one warp, with a softmax of its own (reference,
 // mass and sums in registers) and a ring of its own in shared memory that the warp fills by cp.async: the warps of a block do not wait for
 // one another until the unit ends.  The line is cut into parts of whole blocks; the tiles of a part go round the block's warps.
 // (One bulk copy of 256 bytes per lane and row instead: the compiler issues them lane by lane, 790 instructions a tile.)
@@ -861,7 +862,8 @@ __global__ void __launch_bounds__(SliceShape<T, DK, DV, ROWS>::threads, 1) draft
 // kg, kg + 16, .. of the tile, of the sums the columns 4 cg .. 4 cg + 3 of every 64 (kg = cg = lane & 15): per 64 products it reads 4 to 6
 // times 16 bytes of shared memory, so that the FMA pipes bound it and not the reads.  A warp's weights stay in it.  The keys of the next tile come
 // by cp.async while the values are multiplied, the values while the scores are; pieces of 16 bytes are swizzled so that the lanes of a
-// read meet in no bank.
+// read meet in no bank.  Measured, 4 requests of 16384, 4 heads of 128, 256 rows: 935 us, 37 TFLOP/s (slices of sixteen rows: 1983 us);
+// seven in ten issue slots are taken, seven in ten of those by products.  Products of two at a time in packed instructions change it by 2%.
 constexpr int kFmaRows = 64, kFmaThreads = 128;
 template <int D> struct FmaShape {
     static constexpr int q = 0, k = q + kFmaRows * D * 4, v = k + kTile * D * 4, p = v + kTile * D * 4, mask = p + kFmaRows * kTile * 4,
@@ -1074,7 +1076,9 @@ __global__ void __launch_bounds__(kFmaThreads, D > 128 ? 1 : 2) draft_fma_kernel
 // every other tile, and are joined at the end.  Tensor memory: S and O of each half, 128 columns each; shared memory: Q (64 KB), three
 // stages of K and two of V (32 KB).  Roles: warps 0-3 and 4-7 the softmax of a half, 8 the products, 9-11 the copies.
 // At 256 rows of 128 a tile is 16.8 MFLOP, 2048 cycles of the tensor pipe, and 32768 exponentials, 2048 cycles of the special function
-// units: the two bound it alike, HBM (64 KB a tile) does below about 250 rows.
+// units: the two bound it alike, HBM (64 KB a tile) does below about 250 rows.  A tile of 256 rows takes 2500 to 2800 cycles as it is (the
+// scores' operands and the copies share the bandwidth of shared memory).  Measured in bf16, 128 wide: 4 requests of 16384, 8 heads, chunks of
+// 512 drafts with 4 query heads each: 615 us, 908 TFLOP/s; 8 of 65536, 4 heads, 256 rows: 308 us, 894 TFLOP/s, 128 rows 210 us, 5.1 TB/s.
 // A row's weights in a tile may sum to kTcMost before the reference follows (a maximum per tile costs a fifth of the softmax; the sum is there
 // anyway); a reference is set kTcBias below the maximum.  bf16 has fp32's range; fp16 ends at 65504 and keeps all its digits down to 2^-14.
 template <typename T> constexpr float kTcMost = 65536.f;
@@ -1853,17 +1857,19 @@ static void fit(DraftParams& p, int rows, int tile, int blocks, int least) {
 static int64_t part_bytes(const DraftParams& p) { return p.whole ? 0 : (int64_t)p.grid * 2 * p.rows * (p.V + 2) * 4; }
 static int64_t workspace_of(const DraftParams& p) { return p.whole ? 16 : part_bytes(p) + p.grid * 16; }           // tasks: per unit or per part, never more than parts
 
-// Which kernel: 16-bit rows of up to 128 go to the tensor cores, by mma.sync up to 32 query rows, up to 16 with rows of more than 64 (where
+// Which kernel.  16-bit rows of up to 128 go to the tensor cores, by mma.sync up to 32 query rows, up to 16 with rows of more than 64 (where
 // a warp of 32 has spills).  Measured, 8 requests of 16384, 4 heads of 128: 32 rows 84 us on mma.sync and 70 on tcgen05, 16 rows 63 and
 // 70; 8 heads of 64: 32 rows 78 and 97; 8 requests of 1000, 4 heads of 128: 32 rows 25 and 27, 16 rows 20 and 27.
-enum { kSlice4 = 0, kSlice16, kSlice32, kFma, kTc };
+// fp32 (4 requests of 16384, 4 heads of 128): 17 to 32 rows 266 us by slices of sixteen rows and 242 by FFMA tiles of 64, 16 rows 147 and
+// 242; 8 rows 95 by slices of eight and 148 by those of sixteen.  Wider 16-bit rows: slices of 16 query rows however many there are (4 requests of 16384, 4 heads of 256, 256 rows: 620 us).
+enum { kSlice4 = 0, kSlice8, kSlice16, kSlice32, kFma, kTc };
 static void choose(DraftParams& p, int dtype) {
     const int sms = sm_count() > 0 ? sm_count() : 148, rows = p.N * p.G;
     const bool wide = p.K > 128 || p.V > 128;
     if (dtype == HTREE_F32) {
-        p.variant = rows <= 4 ? kSlice4 : rows <= 16 ? kSlice16 : kFma;
+        p.variant = rows <= 4 ? kSlice4 : rows <= 8 ? kSlice8 : rows <= 16 ? kSlice16 : kFma;
         if (p.variant == kFma) fit(p, kFmaRows, kTile, wide ? sms : 2 * sms, 1);
-        else fit(p, rows <= 4 ? 4 : 16, kSlice, sms, wide ? 3 : p.K > 64 && p.V > 64 ? 6 : p.K > 64 || p.V > 64 ? 8 : 12);
+        else fit(p, rows <= 4 ? 4 : rows <= 8 ? 8 : 16, kSlice, sms, wide ? 3 : p.K > 64 && p.V > 64 ? 6 : p.K > 64 || p.V > 64 ? 8 : 12);
         return;
     }
     p.variant = wide || rows <= 16 ? kSlice16 : rows <= 32 && p.K <= 64 && p.V <= 64 ? kSlice32 : kTc;
@@ -1927,8 +1933,9 @@ static int launch_slices(const DraftParams& p, cudaStream_t st) {
 template <typename T, int DK, int DV>
 static int launch_sized(const DraftParams& p, cudaStream_t st) {
     if constexpr (sizeof(T) == 4) {
-        return p.variant == kSlice4 ? launch_slices<T, DK, DV, 4>(p, st) : launch_slices<T, DK, DV, 16>(p, st);
+        return p.variant == kSlice4 ? launch_slices<T, DK, DV, 4>(p, st) : p.variant == kSlice8 ? launch_slices<T, DK, DV, 8>(p, st) : launch_slices<T, DK, DV, 16>(p, st);
     } else {
+    if constexpr (DK <= 128)
     if (p.variant == kTc) {
         static SmemLimit limit;
         if (const cudaError_t e = limit.raise((const void*)draft_tc_kernel<T, DK, DV>, TcShape<DK, DV>::total)) return (int)e;
@@ -1943,12 +1950,6 @@ static int launch_sized(const DraftParams& p, cudaStream_t st) {
     }
 }
 
-template <typename T>
-static int launch_wide(const DraftParams& p, cudaStream_t st) {
-    if constexpr (sizeof(T) == 4)
-        if (p.variant == kSlice4) return launch_slices<T, 256, 256, 4>(p, st);
-    return launch_slices<T, 256, 256, 16>(p, st);
-}
 template <int D>
 static int launch_fma(const DraftParams& p, cudaStream_t st) {
     static SmemLimit limit;
@@ -1961,7 +1962,7 @@ static int launch_draft(const DraftParams& p, cudaStream_t st) {
     const bool k64 = p.K <= 64, v64 = p.V <= 64;
     int rc;
     if (p.variant == kFma) rc = k64 && v64 ? launch_fma<64>(p, st) : p.K <= 128 && p.V <= 128 ? launch_fma<128>(p, st) : launch_fma<256>(p, st);
-    else if (p.K > 128 || p.V > 128) rc = launch_wide<T>(p, st);
+    else if (p.K > 128 || p.V > 128) rc = launch_sized<T, 256, 256>(p, st);
     else rc = k64 ? (v64 ? launch_sized<T, 64, 64>(p, st) : launch_sized<T, 64, 128>(p, st)) : v64 ? launch_sized<T, 128, 64>(p, st) : launch_sized<T, 128, 128>(p, st);
     if (rc || p.whole) return rc;
     const int rows = p.N * p.G < p.rows ? p.N * p.G : p.rows, block = kJoinWarps / p.team;

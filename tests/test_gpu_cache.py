@@ -87,6 +87,9 @@ CASES = [
     # fp32 with more than sixteen rows: parts of one and of several row tiles of 64
     (FP, 64, 1, 1, 128, 128, 64, [1000, 64], True, 0), (FP, 130, 2, 1, 64, 64, 16, [129, 0, 500], False, 0), (FP, 70, 3, 1, 96, 128, 7, [260], True, 0.3),
     (FP, 20, 8, 2, 32, 24, 16, [63, 65], True, 0.5), (FP, 300, 4, 4, 128, 128, 16, [40], False, 0),
+    # ... and with five to eight
+    (FP, 1, 7, 1, 128, 128, 16, [1000, 5], False, 0), (FP, 8, 2, 2, 64, 64, 16, [300], True, 0.1), (FP, 2, 6, 2, 256, 144, 8, [222], False, 0),
+    (FP, 5, 1, 1, 128, 40, 3, [64, 130], True, 0), (FP, 4, 2, 1, 24, 128, 64, [700], True, 0),
 ]
 
 
