@@ -26,16 +26,19 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _status
+from .ops import _status, _status_words
 
 
-def _glue(t: torch.Tensor):
+def _calls(t: torch.Tensor):
+    """The C++ side of the calls, and the status word of the device (a call of a few microseconds: nothing is looked up twice)."""
     if not t.is_cuda:
         raise RuntimeError("htree_b200 runs on CUDA tensors only; there is no CPU implementation")
     g = _lib.glue()
     if not g:
         raise RuntimeError("the cache operators need the library that the torch glue is linked to: unset HTREE_B200_LIB")
-    return g
+    device = t.device
+    status = _status_words.get(device)
+    return g, _status(device) if status is None else status
 
 
 def cache_plan(lengths: torch.Tensor, counts: torch.Tensor, block_table: torch.Tensor, pool: torch.Tensor, top: torch.Tensor,
@@ -47,7 +50,8 @@ def cache_plan(lengths: torch.Tensor, counts: torch.Tensor, block_table: torch.T
     taken[b] is counts[b] where request b was served and 0 where it was not (no pages left, or, reported by check_status, more than n
     tokens or than its table row can name); slots[b, i] is the slot (page * page_size + place) of its i-th new token, -1 elsewhere.
     lengths, block_table, pool and top are updated in place."""
-    return _glue(block_table).cache_plan(lengths, counts, block_table, pool, top, page_size, n, _status(block_table.device))
+    g, status = _calls(block_table)
+    return g.cache_plan(lengths, counts, block_table, pool, top, page_size, n, status)
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
@@ -55,13 +59,15 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     """Rows of k [B, N, H_kv, K] and v [B, N, H_kv, V] into their slots [B, n] (-1: not written): token i of request b, or token
     index[b, i] (int32), e.g. the accepted drafts.  Slots of one call have to differ: of tokens that share one, any may be kept.  k and v
     must not lie in the cache themselves."""
-    _glue(k_cache).cache_append(k, v, k_cache, v_cache, slots, index, _status(k_cache.device))
+    g, status = _calls(k_cache)
+    g.cache_append(k, v, k_cache, v_cache, slots, index, status)
 
 
 def cache_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
                  T: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """The first T tokens of every request as contiguous (k [B, T, H_kv, K], v [B, T, H_kv, V]), zeros behind a request's end."""
-    return _glue(k_cache).cache_gather(k_cache, v_cache, block_table, lengths, T, _status(k_cache.device))
+    g, status = _calls(k_cache)
+    return g.cache_gather(k_cache, v_cache, block_table, lengths, T, status)
 
 
 def draft_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -77,7 +83,8 @@ def draft_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: 
     1024 drafts, chains of any length."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    out, lse = _glue(k_cache).draft_attention(q, k, v, k_cache, v_cache, block_table, lengths, parents, scale, return_lse, _status(k_cache.device))
+    g, status = _calls(k_cache)
+    out, lse = g.draft_attention(q, k, v, k_cache, v_cache, block_table, lengths, parents, scale, return_lse, status)
     return (out, lse) if return_lse else out
 
 

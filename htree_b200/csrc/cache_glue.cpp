@@ -1,6 +1,8 @@
 // The torch side of the paged cache's calls: argument checks, outputs, workspace and stream (a call of a few microseconds of kernel has no
 // time for the interpreter to do it).  Python (cache.py) documents them and keeps the status word.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -100,6 +102,9 @@ void written(std::initializer_list<const at::Tensor*> ts) {
         if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
+// A new tensor without a way through the dispatcher (which takes as long as the allocation).
+at::Tensor fresh(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) { return at::Tensor(at::detail::empty_cuda(size, type, like.device(), c10::nullopt)); }
+
 int32_t* status_of(const at::Tensor& status) { return status.data_ptr<int32_t>(); }
 
 std::tuple<at::Tensor, at::Tensor> cache_plan(const at::Tensor& lengths, const at::Tensor& counts, const at::Tensor& table, const at::Tensor& pool,
@@ -116,7 +121,7 @@ std::tuple<at::Tensor, at::Tensor> cache_plan(const at::Tensor& lengths, const a
     TORCH_CHECK_VALUE(n > 0 && n <= INT32_MAX, "n must be positive, not ", n);
     TORCH_CHECK_VALUE(B <= 65535 && table.size(1) <= INT32_MAX && pool.size(0) <= INT32_MAX, "at most 65535 requests");
     c10::cuda::CUDAGuard guard(table.device());
-    at::Tensor slots = at::empty({B, n}, table.options().dtype(at::kLong)), taken = at::empty({B}, table.options());
+    at::Tensor slots = fresh({B, n}, at::kLong, table), taken = fresh({B}, at::kInt, table);
     if (B == 0) return {slots, taken};
     const at::Tensor c = counts.contiguous();
     check(htree_b200_cache_plan((int32_t)B, (int32_t)table.size(1), (int32_t)page_size, (int32_t)n, lengths.data_ptr<int32_t>(), c.data_ptr<int32_t>(),
@@ -165,7 +170,8 @@ std::tuple<at::Tensor, at::Tensor> cache_gather(const at::Tensor& k_cache, const
     TORCH_CHECK_VALUE(table.device() == k_cache.device(), "block_table and the cache must be on one device");
     TORCH_CHECK_VALUE(T >= 0 && T <= INT32_MAX && B <= 65535 && table.size(1) <= INT32_MAX, "T must not be negative; at most 65535 requests");
     c10::cuda::CUDAGuard guard(k_cache.device());
-    at::Tensor k = at::empty({B, T, k_cache.size(2), k_cache.size(3)}, k_cache.options()), v = at::empty({B, T, k_cache.size(2), v_cache.size(3)}, v_cache.options());
+    at::Tensor k = fresh({B, T, k_cache.size(2), k_cache.size(3)}, k_cache.scalar_type(), k_cache);
+    at::Tensor v = fresh({B, T, k_cache.size(2), v_cache.size(3)}, k_cache.scalar_type(), k_cache);
     if (B == 0 || T == 0) return {k, v};
     check(htree_b200_cache_gather(&cache, (int32_t)B, (int32_t)table.size(1), (int32_t)T, table.data_ptr<int32_t>(), table_stride(table),
                                   lengths.data_ptr<int32_t>(), k.data_ptr(), v.data_ptr(), status_of(status), stream()),
@@ -196,9 +202,9 @@ std::tuple<at::Tensor, OptTensor> draft_attention(const at::Tensor& q, const at:
         par = parents->contiguous();
     }
     c10::cuda::CUDAGuard guard(k_cache.device());
-    at::Tensor out = at::empty({B, N, H, (int64_t)cache.V}, q.options().requires_grad(false));
+    at::Tensor out = fresh({B, N, H, (int64_t)cache.V}, q.scalar_type(), q);
     OptTensor lse;
-    if (want_lse) lse = at::empty({B, N, H}, q.options().dtype(at::kFloat).requires_grad(false));
+    if (want_lse) lse = fresh({B, N, H}, at::kFloat, q);
     if (B == 0 || N == 0) return {out, lse};
     HtreeDrafts d{};
     const at::Tensor qq = readable(q, d.q_stride), kk = readable(k, d.k_stride), vv = readable(v, d.v_stride);
@@ -210,8 +216,8 @@ std::tuple<at::Tensor, OptTensor> draft_attention(const at::Tensor& q, const at:
     d.scale = (float)scale;
     const int64_t bytes = htree_b200_draft_workspace(&cache, &d);
     if (bytes < 0) check(bytes, "draft_attention");
-    const at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte).requires_grad(false));
-    check(htree_b200_draft_attention(&cache, &d, ws.data_ptr(), bytes, status_of(status), stream()), "draft_attention");
+    const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)bytes);       // (of the current stream, as the tensors)
+    check(htree_b200_draft_attention(&cache, &d, ws.get(), bytes, status_of(status), stream()), "draft_attention");
     return {out, lse};
 }
 
