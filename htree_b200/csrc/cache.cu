@@ -31,7 +31,7 @@ struct PlanParams {
     FastDiv page;
 };
 
-constexpr int kPlanThreads = 512;
+constexpr int kPlanThreads = 1024;
 constexpr uint32_t kPlanMost = 0x7fffffffu;      // sums of pages stop here: no pool has as many
 
 __device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, kPlanMost); }
@@ -71,7 +71,9 @@ __device__ __forceinline__ int plan_length(const PlanParams& p, int len, bool* b
 // One cluster does the whole plan, so that the pages that ending rows give back can go to growing rows in the same call: every block
 // computes the two scans for itself (a few words a request), the blocks share the rows, and cluster barriers separate the pushes, the
 // pops and the slots.  `W` threads work on a row: a warp where there are many rows, all of them where there is one.  What bounds it is
-// latency: entries move eight at a time (one by one, 512 rows of 800 pages took 61 us; so 12).
+// latency: entries move eight at a time (one by one, 512 rows of 800 pages took 61 us; so 12), by sixteen blocks of 1024 threads (admitting,
+// extending and ending 512 requests of 16384 tokens in pages of 16: 38 us in three calls, by eight of 512 threads 50; 1024 requests of 2000 in
+// pages of one: 56 and 108).
 __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_constant__ PlanParams p) {
     __shared__ uint32_t scratch[kPlanThreads / 32];
     __shared__ uint32_t first[kPlanThreads];
@@ -201,6 +203,18 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
         if (bad) atomicOr(p.status, HTREE_STATUS_CACHE);
         if (refused) atomicOr(p.status, HTREE_STATUS_ROW);
     }
+}
+
+// Clusters of sixteen blocks have to be allowed, once per device.
+static bool sixteen_allowed() {
+    static std::atomic<int> have[64] = {};           // 1: allowed, 2: refused
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return false; }
+    if (dev < 64 && have[dev].load(std::memory_order_acquire)) return have[dev].load(std::memory_order_acquire) == 1;
+    const bool ok = cudaFuncSetAttribute((const void*)cache_plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+    if (!ok) cudaGetLastError();
+    if (dev < 64) have[dev].store(ok ? 1 : 2, std::memory_order_release);
+    return ok;
 }
 
 // The slot map of a plan with many new tokens, by the whole chip (8 bytes a token; the cluster alone would write it at a tenth of the
@@ -401,8 +415,10 @@ int htree_b200_cache_plan(int32_t B, int32_t M, int32_t page_size, int32_t n, in
     const int64_t entries = (int64_t)B * M, map = (int64_t)B * n, room = (int64_t)M * page_size, most = 0x7fffffff - (int64_t)page_size;
     p.room = (int32_t)(room < most ? room : most);
     p.slots_here = map <= 16384;
-    const int CL = entries <= 4096 ? 1 : 8;
-    const int rc = launch_clusters(cache_plan_kernel, CL, dim3(1), dim3(kPlanThreads), 0, (cudaStream_t)stream, p);
+    const int CL = entries <= 4096 ? 1 : sixteen_allowed() ? 16 : 8;
+    int rc = launch_chained_clusters(cache_plan_kernel, CL, dim3(CL), dim3(kPlanThreads), 0, (cudaStream_t)stream, p);
+    if (rc && CL == 16) rc = launch_chained_clusters(cache_plan_kernel, 8, dim3(8), dim3(kPlanThreads), 0, (cudaStream_t)stream, p);
+    if (rc && CL > 1) rc = launch_chained_clusters(cache_plan_kernel, 1, dim3(1), dim3(kPlanThreads), 0, (cudaStream_t)stream, p);
     if (rc || p.slots_here) return rc;
     const dim3 grid((unsigned)((n + 256 * (int64_t)kSlotsPerThread - 1) / (256 * kSlotsPerThread)), B);
     return n % 2 == 0 && cache_aligned(slots) ? launch_chained(cache_slots_kernel<true>, grid, dim3(256), 0, (cudaStream_t)stream, p)

@@ -282,7 +282,7 @@ def test_refusals():
             ht.cache_plan(*args)
 
 
-@pytest.mark.parametrize("B,M,page,n,pages", [(1, 4, 16, 20, 5), (7, 9, 4, 30, 40), (33, 40, 1, 25, 500), (700, 30, 16, 64, 9000), (3, 6000, 2, 11000, 9000),
+@pytest.mark.parametrize("B,M,page,n,pages", [(1, 4, 16, 20, 5), (7, 9, 4, 30, 40), (33, 40, 1, 25, 500), (700, 30, 16, 64, 9000), (1300, 9, 4, 12, 7000), (3, 6000, 2, 11000, 9000),
                                               (40, 700, 16, 3000, 9000)])
 def test_plan(B, M, page, n, pages):
     """Turns of a batch that grows, runs out of pages, ends and goes on."""
