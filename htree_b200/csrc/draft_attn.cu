@@ -212,15 +212,14 @@ __device__ __forceinline__ void draft_masks(const DraftParams& p, int b, int n, 
 #pragma unroll
     for (int i = 0; i < W; ++i) m[i] = 0;
     const int32_t* par = p.parents + (int64_t)b * p.N;
-    int up = par[n];
-    if (up < -1) return;
-    for (int i = n; i >= tile0; up = par[i]) {               // parents come before their children: at most n steps
+    for (int i = n; i >= tile0;) {                           // parents come before their children: at most n steps
+        const int up = par[i];
+        if (up < -1) return;                                 // no draft
         const uint64_t bit = 1ull << ((i - tile0) & 63);
 #pragma unroll
         for (int j = 0; j < W; ++j) if ((i - tile0) >> 6 == j) m[j] |= bit;
         if (up >= i) { *bad = true; return; }
         i = up;
-        if (i < tile0) return;
     }
 }
 __device__ __forceinline__ uint64_t draft_mask(const DraftParams& p, int b, int n, int tile0, bool* bad) {
@@ -1311,16 +1310,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 const bool draft = tile >= cached;
                 const int n0 = (tile - cached) * kTcTile;
                 if (looked != tile) look(tile);
-                // Slices of sixteen keys that are one box of a tensor map: sixteen cached tokens of a page, or sixteen drafts.
-                const int pos = tile * kTcTile + (lane & 7) * 16, in = pos - (int)(p.page.div((uint32_t)pos) * p.page.d);
-                bool whole16;
-                if (!draft) {
-                    whole16 = (p.boxes & 1) && pos + 16 <= at.len && page >= 0 && page < p.pages;
-                } else {
-                    whole16 = (p.boxes & 4) && n0 + (lane & 7) * 16 + 16 <= p.N;
-                    if (whole16 && p.parents)
-                        for (int i = 0; i < 16; ++i) whole16 &= is_draft(p, at.b, n0 + (lane & 7) * 16 + i);
-                }
+                // Slices of sixteen keys that are one box of a tensor map: sixteen cached tokens of a page, sixteen drafts (those that are none are
+                // read by no row, and their values looked through; behind the last a map gives zeros), or, of values, no token at all.
+                const int pos = tile * kTcTile + (lane & 7) * 16;
+                int in = pos - (int)(p.page.div((uint32_t)pos) * p.page.d);
+                const bool none = values && !draft && (p.boxes & 1) && pos >= at.len;
+                const uint32_t nothing = __ballot_sync(0xffffffffu, none) & 0xffu;
+                if (none) { page = 0; in = (int)p.page.d; }
+                const bool whole16 = draft ? (p.boxes & 4) != 0 : none || ((p.boxes & 1) && pos + 16 <= at.len && page >= 0 && page < p.pages);
                 const uint32_t boxes = __ballot_sync(0xffffffffu, whole16) & 0xffu;
                 // others, row by row: which keys there are, and where (lane x the key x of each 32)
                 uint32_t words[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
@@ -1356,7 +1353,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
 #pragma unroll
                             for (int sl = 0; sl < 8; ++sl)
                                 if (boxes >> sl & 1) box(values ? maps.dv : maps.dk, lanes / 8, bar, dst + sl * 2048, n0 + sl * 16, kv, at.b);
-                        } else if (boxes == 0xffu && p.box_rows > 16) {
+                        } else if (boxes == 0xffu && p.box_rows > 16 && !nothing) {
 #pragma unroll
                             for (int sl = 0; sl < 8; sl += 2)
                                 if (((sl * 16) & (p.box_rows - 1)) == 0) box(values ? maps.vb : maps.kb, lanes / 8, bar, dst + sl * 2048, ins[sl], kv, pages[sl]);
@@ -1375,7 +1372,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                     if (values) cp_async_wait<0>();
                 }
                 // Rows of keys are told one tile later, when they have had time to come (their stage's next use is two tiles away; that of
-                // values waits for them).
+                // values waits for them), while whole tiles of tokens follow.
                 if (late_bar >= 0) {
                     if (boxes != 0xffu) cp_async_wait<1>(); else cp_async_wait<0>();
                     fence_proxy_async();
@@ -1391,10 +1388,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                     for (int x = lane; x < rows_in * lanes; x += 32)
                         if (take_out<T>(dst + place_of(x / lanes, x % lanes))) atomicOr(&spoilt[(t & 7) * 4 + (x / lanes >> 5)], 1u << (x / lanes & 31));
                 }
-                if (!values && boxes != 0xffu) {
+                if (!values && boxes != 0xffu && j + 1 < piece && (tile + 2) * kTcTile <= at.len) {
                     late_bar = full;
                     late_bytes = bytes;
                 } else if (look_through || boxes != 0xffu) {
+                    if (!values) cp_async_wait<0>();
                     fence_proxy_async();
                     __syncwarp();
                     tell(full, look_through ? 0 : bytes);
@@ -1522,7 +1520,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 uint32_t pk[64];
                 float2 sums[2];
                 sums[0] = sums[1] = make_float2(0.f, 0.f);
-                // P and its sum, of 16 scores; `mixed`: every kTcPolyEvery-th pair of exponentials on the FMA pipes
+                // (A row whose scores are NaN, as those of padding may be, stays so and does not call for a new reference: that its neighbours'
+                // would move with.)  P and its sum, of 16 scores; `mixed`: every kTcPolyEvery-th pair of exponentials on the FMA pipes
                 auto weigh = [&](const uint32_t (&y)[16], uint32_t* to_pk, auto mixed) {
                     const float2 cc = make_float2(p.c, p.c), bb = make_float2(-ref, -ref);
 #pragma unroll
@@ -1533,7 +1532,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                         to_pk[e >> 1] = Frag<T>::pack(v.x, v.y);
                     }
                 };
-                bool anew = __any_sync(0xffffffffu, empty || (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu);
+                bool anew = __any_sync(0xffffffffu, (empty && mass == mass) || (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu);
                 if (!anew) {
                     // the reference stays, unless the weights get too large for the type: their sum tells (none is larger than it)
 #pragma unroll
@@ -1542,7 +1541,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                         if (c < 7) tc_ld16(x[(c + 1) & 1], ts + (c + 1) * 16);
                         weigh(x[c & 1], pk + c * 8, std::true_type{});
                     }
-                    anew = __any_sync(0xffffffffu, !((sums[0].x + sums[0].y) + (sums[1].x + sums[1].y) <= kTcMost<T>));
+                    anew = __any_sync(0xffffffffu, (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y) > kTcMost<T>);
                 } else {
                     tc_wait_ld(x[0]);
                 }
@@ -1917,7 +1916,7 @@ static int tc_maps(TcMaps& m, DraftParams& p, bool bf16) {
     if (p.page.d % 16 == 0 && caches(m.k, m.v, 16)) boxes |= 1;
     if (p.box_rows > 16 && !caches(m.kb, m.vb, (uint32_t)p.box_rows)) p.box_rows = 16;
     if (128 % p.G == 0 && row_map(m.q, p.q, p.K, {{p.H, p.q_h, (uint32_t)p.G}, {p.N, p.q_n, (uint32_t)(128 / p.G)}, {p.B, p.q_b, 1}}, bf16)) boxes |= 2;
-    if (p.N >= 16 && row_map(m.dk, p.k, p.K, {{p.N, p.k_n, 16}, {p.Hkv, p.k_h, 1}, {p.B, p.k_b, 1}}, bf16) &&
+    if (row_map(m.dk, p.k, p.K, {{p.N, p.k_n, 16}, {p.Hkv, p.k_h, 1}, {p.B, p.k_b, 1}}, bf16) &&
         row_map(m.dv, p.v, p.V, {{p.N, p.v_n, 16}, {p.Hkv, p.v_h, 1}, {p.B, p.v_b, 1}}, bf16))
         boxes |= 4;
     return boxes;

@@ -156,6 +156,23 @@ def test_what_a_draft_does_not_read_does_not_reach_it(dt, N, K):
             assert not torch.isfinite(out[real]).all(-1).any()
 
 
+@pytest.mark.parametrize("dt", [FP, BF, HF])
+@pytest.mark.parametrize("N,G,K,lengths", [(13, 8, 64, [200, 128, 0]), (5, 2, 128, [65, 17, 300]), (40, 4, 128, [130, 9, 256]), (150, 2, 64, [70, 0, 128])])
+def test_padding_holds_anything(dt, N, G, K, lengths):
+    """Drafts that are none (parents below -1), inside and behind the others: NaN and infinity in their q, k and v reach nobody, their children included."""
+    import htree_b200 as ht
+    s = make(dt, N, 2 * G, 2, K, K, 16, lengths)
+    parents = tree(len(lengths), N, seed=5, pad=0.2)
+    parents[1, N // 2:] = -2
+    pad = parents < -1
+    clean = ht.draft_attention(**s, parents=parents, return_lse=True)
+    agrees(s, parents, out=clean)
+    for name, value in (("q", math.nan), ("k", math.inf), ("v", math.nan), ("v", -math.inf)):
+        s[name] = torch.where(pad[:, :, None, None], torch.full_like(s[name], value), s[name])
+        out, lse = ht.draft_attention(**s, parents=parents, return_lse=True)
+        assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1])
+
+
 @pytest.mark.parametrize("dt,K", [(FP, 64), (BF, 128), (HF, 64), (BF, 256)])
 def test_strides(dt, K):
     """q, k, v as slices of one projection; the cache as [pages, heads, 2, page, width]; a table with more columns than are passed."""
