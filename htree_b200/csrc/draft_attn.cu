@@ -1532,7 +1532,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                         to_pk[e >> 1] = Frag<T>::pack(v.x, v.y);
                     }
                 };
-                bool anew = __any_sync(0xffffffffu, (empty && mass == mass) || (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu);
+                bool anew = __any_sync(0xffffffffu, (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu);
+                if (!anew && __any_sync(0xffffffffu, empty && mass == mass)) {
+                    // a first reference: the largest of sixteen scores (none is above the one that the maximum would give)
+                    tc_wait_ld(x[0]);
+                    float t = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(t) : "f"(__uint_as_float(x[0][e])));
+                    if (empty && fabsf(t) <= 3.4028234e38f) {
+                        ref = t * p.c - kTcBias<T>;
+                        empty = false;
+                    }
+                    anew = __any_sync(0xffffffffu, empty && fabsf(t) > 3.4028234e38f);
+                }
                 if (!anew) {
                     // the reference stays, unless the weights get too large for the type: their sum tells (none is larger than it)
 #pragma unroll
