@@ -1116,12 +1116,16 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(x));
     return x != 0;
 }
-// 2^t on the FMA pipes, two at a time, t at most 2^7: t = n + f with n the nearest integer (it appears in the low bits of t + 1.5 * 2^23), 2^f
-// by a polynomial of degree 5 (fitted to the smallest largest relative error over [-1/2, 1/2], 2.3e-7 in fp32), n added to the exponent.
-// What is below -126 comes out as 2^-126; NaN and infinity as something that is not small.
-__device__ __forceinline__ float2 exp2_poly(float2 t) {
+// 2^t on the FMA pipes, two at a time: t = n + f with n the nearest integer (it appears in the low bits of t + 1.5 * 2^23), 2^f by a polynomial
+// of degree 5 (fitted to the smallest largest relative error over [-1/2, 1/2], 2.3e-7 in fp32), n added to the exponent.  What is below -126
+// comes out as 2^-126.  Above 126, where n runs through the exponent into the sign, the result means nothing and may be small: `most` is the
+// largest t (NaN if one is), by which the caller has to tell.  (Telling costs 2% of tree_16k, 145 -> 149 us, and 1% of chunk_8k; cutting t off
+// above as well 3.5% of both.)
+constexpr float kPolyMost = 126.f;
+__device__ __forceinline__ float2 exp2_poly(float2 t, float& most) {
     asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(t.x));
     asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(t.y));
+    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(most) : "f"(t.x), "f"(t.y));
     const float2 big = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f);
     const float2 r = fadd2(t, big), n = fadd2(r, minus), f = ffma2(n, make_float2(-1.f, -1.f), t);
     float2 y = ffma2(make_float2(0.0013276470126584172f, 0.0013276470126584172f), f, make_float2(0.009675540961325169f, 0.009675540961325169f));
@@ -1521,13 +1525,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                 float2 sums[2];
                 sums[0] = sums[1] = make_float2(0.f, 0.f);
                 // (A row whose scores are NaN, as those of padding may be, stays so and does not call for a new reference: that its neighbours'
-                // would move with.)  P and its sum, of 16 scores; `mixed`: every kTcPolyEvery-th pair of exponentials on the FMA pipes
+                // would move with.)  P and its sum, of 16 scores; `mixed`: every kTcPolyEvery-th pair of exponentials on the FMA pipes, of which `high`
+                // has the largest exponent
+                float high = 0.f;
                 auto weigh = [&](const uint32_t (&y)[16], uint32_t* to_pk, auto mixed) {
                     const float2 cc = make_float2(p.c, p.c), bb = make_float2(-ref, -ref);
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
                         const float2 t = ffma2(make_float2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), cc, bb);
-                        const float2 v = decltype(mixed)::value && (e >> 1) % kTcPolyEvery == kTcPolyEvery - 1 ? exp2_poly(t) : make_float2(ex2_approx(t.x), ex2_approx(t.y));
+                        const float2 v = decltype(mixed)::value && (e >> 1) % kTcPolyEvery == kTcPolyEvery - 1 ? exp2_poly(t, high) : make_float2(ex2_approx(t.x), ex2_approx(t.y));
                         sums[(e >> 1) & 1] = fadd2(sums[(e >> 1) & 1], v);
                         to_pk[e >> 1] = Frag<T>::pack(v.x, v.y);
                     }
@@ -1546,14 +1552,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) draft_tc_kernel(const __grid_co
                     anew = __any_sync(0xffffffffu, empty && fabsf(t) > 3.4028234e38f);
                 }
                 if (!anew) {
-                    // the reference stays, unless the weights get too large for the type: their sum tells (none is larger than it)
+                    // the reference stays, unless the weights get too large for the type: their sum tells (none is larger than it), and `high`
+                    // where the sum means nothing
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
                         tc_wait_ld(x[c & 1]);
                         if (c < 7) tc_ld16(x[(c + 1) & 1], ts + (c + 1) * 16);
                         weigh(x[c & 1], pk + c * 8, std::true_type{});
                     }
-                    anew = __any_sync(0xffffffffu, (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y) > kTcMost<T>);
+                    anew = __any_sync(0xffffffffu, (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y) > kTcMost<T> || high > kPolyMost);
+                    sums[0].x = fmaf(high, 0.f, sums[0].x);        // (NaN among them stays NaN)
                 } else {
                     tc_wait_ld(x[0]);
                 }

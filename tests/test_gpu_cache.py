@@ -527,3 +527,64 @@ def test_calls_repeat_bit_for_bit(dt):
     for _ in range(5):
         for a, b in zip(first, ht.draft_attention(**s, parents=tree(3, 5), return_lse=True)):
             assert torch.equal(a, b)
+
+
+# Heights, in units of the exponent, around what fp32 holds of a power of two (2^128 is e^88.7), of one with a sign (2^256, 2^384: e^177, e^266) and far beyond.
+HEIGHTS = [60, 86, 88, 89, 90, 92, 100, 110, 150, 176, 178, 220, 265, 267, 300, 350, 400, 600]
+
+
+def steep(dt, N, G, K, lengths, seed=0):
+    """One height for all rows of a request and key/value head (rows of a warp would otherwise look for the maximum together): their scores over a
+    key along a common direction (8 in every element) are that, over other keys next to nothing.  Returns the state and the direction."""
+    s = make(dt, N, 2 * G, 2, K, K, 16, lengths, seed=seed)
+    height = torch.tensor([[HEIGHTS[(5 * b + 9 * h + seed) % len(HEIGHTS)] for h in range(2)] for b in range(len(lengths))], device=DEV, dtype=torch.float32)
+    s["q"] = (0.1 * s["q"].float() + (height / (8 * K ** 0.5)).repeat_interleave(G, 1)[:, None, :, None]).to(dt)
+    for n in ("k", "k_cache"):
+        s[n] = (s[n].float() - s[n].float().mean(-1, keepdim=True)).to(dt)
+    return s, torch.full((K,), 8.0, device=DEV)
+
+
+def at_token(s, b, pos):
+    return s["block_table"][b, pos // 16].long(), pos % 16
+
+
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("N,G,K", [(20, 2, 64), (40, 4, 64), (20, 2, 128), (40, 4, 128), (6, 2, 128)])
+@pytest.mark.parametrize("first", [0, 49, 210])
+def test_one_key_far_above_the_others(dt, N, G, K, first):
+    """At every place of sixteen, among the first tokens, later ones and those of a later tile, few to very many units above the rest."""
+    s, far = steep(dt, N, G, K, [300] * 16, seed=first)
+    for b in range(16):
+        page, place = at_token(s, b, first + b)
+        s["k_cache"][page, place] = far.to(dt)
+    agrees(s, tree(16, N, seed=first))
+
+
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("N,G,K", [(20, 2, 64), (40, 4, 128)])
+def test_first_keys_far_below_the_others(dt, N, G, K):
+    """The first sixteen tokens, a whole tile of 128 or nearly all of them, and the drafts, far below what follows."""
+    lengths = [300, 290, 400, 144, 17, 256, 512, 513]
+    s, far = steep(dt, N, G, K, lengths, seed=1)
+    for b, from_ in enumerate([16, 128, 256, 127, 16, 100, 255, 511]):
+        for pos in range(from_, lengths[b]):
+            page, place = at_token(s, b, pos)
+            s["k_cache"][page, place] += far.to(dt)
+    agrees(s, tree(8, N, seed=2))
+    s["k"][:, 1::3] += far.to(dt)
+    agrees(s)
+
+
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("N,G,K", [(20, 2, 64), (40, 4, 128), (3, 2, 64)])
+@pytest.mark.parametrize("first", [0, 49, 210])
+def test_a_cached_key_that_is_nan_is_seen(dt, N, G, K, first):
+    """At every place of sixteen: the rows of its request and head are NaN, and no others."""
+    import htree_b200 as ht
+    s = make(dt, N, 2 * G, 2, K, K, 16, [300] * 17)
+    for b in range(16):
+        page, place = at_token(s, b, first + b)
+        s["k_cache"][page, place, b % 2, 3] = math.nan
+    out, lse = ht.draft_attention(**s, return_lse=True)
+    hit = torch.tensor([[b % 2 == h and b < 16 for h in range(2)] for b in range(17)], device=DEV).repeat_interleave(G, 1)[:, None].expand(17, N, 2 * G)
+    assert out[hit].isnan().all() and lse[hit].isnan().all() and torch.isfinite(out[~hit]).all() and torch.isfinite(lse[~hit]).all()
