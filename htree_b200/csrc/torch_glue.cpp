@@ -3,6 +3,7 @@
 // (ops.py) validates, keeps the rotary tables and falls back to its own path for whatever this file declines (returns None).
 // For a training step of a thousand positions the interpreter's share, 200 us a step, was twice the kernels' time.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -141,6 +142,21 @@ c10::optional<at::Tensor> plain_forward(const at::Tensor& q, const at::Tensor& k
     return f.out;
 }
 
+// A word of device memory for the reports of the kernels, zero, for as long as the process lives.  Not by the caching allocator and not on the
+// current stream: where that is being captured, both would be the graph's.
+at::Tensor status_word(int64_t device) {
+    const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+    const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    void* p = nullptr;
+    cudaStream_t st = nullptr;
+    C10_CUDA_CHECK(cudaMalloc(&p, sizeof(int32_t)));
+    C10_CUDA_CHECK(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking));
+    C10_CUDA_CHECK(cudaMemsetAsync(p, 0, sizeof(int32_t), st));
+    C10_CUDA_CHECK(cudaStreamSynchronize(st));
+    C10_CUDA_CHECK(cudaStreamDestroy(st));
+    return torch::from_blob(p, {1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)device));
+}
+
 }  // namespace
 
 void bind_cache(py::module& m);      // cache_glue.cpp
@@ -148,5 +164,6 @@ void bind_cache(py::module& m);      // cache_glue.cpp
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     bind_cache(m);
     m.def("autograd_forward", &autograd_forward, py::call_guard<py::gil_scoped_release>());
+    m.def("status_word", &status_word);
     m.def("plain_forward", &plain_forward, py::call_guard<py::gil_scoped_release>());
 }

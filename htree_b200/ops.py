@@ -151,7 +151,11 @@ def _status(device) -> torch.Tensor:
     device = torch.device(device)
     w = _status_words.get(device)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=device)
+        # The first call may be in inference mode, or be captured: the word has to be one that check_status can clear, and neither its memory
+        # nor its zero may belong to a graph, whose replays would clear it.
+        with torch.inference_mode(False):
+            g = _lib.glue() if device.type == "cuda" else None
+            w = g.status_word(device.index) if g else torch.zeros(1, dtype=torch.int32, device=device)
         _status_words[device] = w
     return w
 

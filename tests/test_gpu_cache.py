@@ -588,3 +588,42 @@ def test_a_cached_key_that_is_nan_is_seen(dt, N, G, K, first):
     out, lse = ht.draft_attention(**s, return_lse=True)
     hit = torch.tensor([[b % 2 == h and b < 16 for h in range(2)] for b in range(17)], device=DEV).repeat_interleave(G, 1)[:, None].expand(17, N, 2 * G)
     assert out[hit].isnan().all() and lse[hit].isnan().all() and torch.isfinite(out[~hit]).all() and torch.isfinite(lse[~hit]).all()
+
+
+def _of_no_page():
+    """A call that reports a page outside the cache."""
+    s = make(BF, 2, 4, 2, 64, 64, 16, [20])
+    return dict(s, block_table=torch.full_like(s["block_table"], -1))
+
+
+@pytest.fixture
+def no_status_word(monkeypatch):
+    """As on a device whose first call is still to come."""
+    from htree_b200 import ops
+    monkeypatch.delitem(ops._status_words, torch.device("cuda", torch.cuda.current_device()), raising=False)
+
+
+def test_reports_of_a_first_call_in_inference_mode(no_status_word):
+    import htree_b200 as ht
+    from htree_b200 import ops
+    with torch.inference_mode():
+        ht.draft_attention(**_of_no_page())
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        ops.check_status()
+    ops.check_status()
+
+
+def test_reports_of_a_first_call_in_a_capture(no_status_word):
+    """The word that collects reports is not the graph's: a replay neither makes it nor clears it."""
+    import htree_b200 as ht
+    from htree_b200 import ops
+    good, bad = make(BF, 2, 4, 2, 64, 64, 16, [20]), _of_no_page()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ht.draft_attention(**good)
+    ops.check_status()
+    ht.draft_attention(**bad)
+    graph.replay()
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        ops.check_status()
+    assert torch.equal(out, ht.draft_attention(**good))
