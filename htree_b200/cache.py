@@ -18,7 +18,8 @@ Drafts are not part of the cache until they are accepted, so a rejected one leav
 contiguous k, v of htree_forward, for the layers or the lengths where htree attention takes over.
 
 No call synchronises or reads a tensor on the host, and all can be captured into a CUDA graph; pages, slots and lengths that lie outside
-the cache are left out and reported by check_status.  None of the calls has a backward.  The reference has no counterpart."""
+the cache are left out and reported by check_status.  None of the calls has a derivative: inputs that require a gradient, or carry a tangent,
+are refused.  The reference has no counterpart."""
 from __future__ import annotations
 
 from typing import Optional, Tuple

@@ -2,6 +2,7 @@
 // time for the interpreter to do it).  Python (cache.py) documents them and keeps the status word.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -27,7 +28,10 @@ void want(const at::Tensor& t, const char* name, int64_t dim, at::ScalarType typ
 }
 void want_int32(const at::Tensor& t, const char* name, int64_t dim, const at::Tensor& like) { want(t, name, dim, at::kInt, like); }
 
+// (torch.no_grad() turns gradients off, but not tangents)
 void no_grad(std::initializer_list<const at::Tensor*> ts, const char* what) {
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        for (const at::Tensor* t : ts) TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative: pass it the primal tensors");
     if (!at::GradMode::is_enabled()) return;
     for (const at::Tensor* t : ts)
         TORCH_CHECK(!t->requires_grad(), what, " has no backward: call it under torch.no_grad(), or detach its inputs");

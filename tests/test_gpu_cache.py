@@ -627,3 +627,27 @@ def test_reports_of_a_first_call_in_a_capture(no_status_word):
     with pytest.raises(RuntimeError, match="outside the cache"):
         ops.check_status()
     assert torch.equal(out, ht.draft_attention(**good))
+
+
+def test_tangents_are_refused():
+    """No call has a forward-mode derivative either; without a tangent, or where tangents are off, they run."""
+    import htree_b200 as ht
+    import torch.autograd.forward_ad as fw
+    s = make(BF, 2, 4, 2, 64, 64, 16, [20])
+    slots = torch.zeros(1, 2, dtype=torch.int64, device=DEV)
+    calls = {"q": ht.draft_attention, "k": ht.draft_attention, "v": ht.draft_attention, "k_cache": ht.draft_attention, "v_cache": ht.draft_attention}
+    append = lambda **t: ht.cache_append(t["k"], t["v"], t["k_cache"], t["v_cache"], slots)      # noqa: E731
+    gather = lambda **t: ht.cache_gather(t["k_cache"], t["v_cache"], t["block_table"], t["lengths"], 20)      # noqa: E731
+    want = ht.draft_attention(**s)
+    with fw.dual_level():
+        for name in calls:
+            t = dict(s, **{name: fw.make_dual(s[name], torch.ones_like(s[name]))})
+            for call in [ht.draft_attention] + [append] * (name != "q") + [gather] * name.endswith("cache"):
+                for grad in (torch.enable_grad, torch.no_grad):           # (no_grad leaves tangents on)
+                    with grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                        call(**t)
+            with fw._set_fwd_grad_enabled(False):
+                assert torch.equal(ht.draft_attention(**t), want)
+        assert torch.equal(ht.draft_attention(**s), want)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda q: ht.draft_attention(**dict(s, q=q)), (s["q"],), (torch.ones_like(s["q"]),))
