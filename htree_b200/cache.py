@@ -50,6 +50,7 @@ def cache_plan(lengths: torch.Tensor, counts: torch.Tensor, block_table: torch.T
     back first, in row order; then, in row order, requests take pages from the pool's end as long as it holds what all up to them need.
     taken[b] is counts[b] where request b was served and 0 where it was not (no pages left, or, reported by check_status, more than n
     tokens or than its table row can name); slots[b, i] is the slot (page * page_size + place) of its i-th new token, -1 elsewhere.
+    An entry below 0 among the pages of a request or the free ones is reported when it is given back and when it is asked for slots, which are -1.
     lengths, block_table, pool and top are updated in place."""
     g, status = _calls(block_table)
     return g.cache_plan(lengths, counts, block_table, pool, top, page_size, n, status)

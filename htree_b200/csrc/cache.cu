@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
                             if (j0 + u * W < some[r]) {
                                 const uint32_t to = first[r] + (uint32_t)(j0 + u * W);
                                 if (to < (uint32_t)p.pool_size) p.pool[to] = e[u]; else bad = true;       // more pages than the pool has: a table with repeats
+                                bad |= e[u] < 0;                                                          // a length of more pages than the row has
                                 row[j0 + u * W] = -1;
                             }
                     }
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
 #pragma unroll
                 for (int u = 0; u < 8; ++u) if (j0 + u * W < some[r]) e[u] = p.pool[first[r] - (uint32_t)(j0 + u * W)];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) if (j0 + u * W < some[r]) row[j0 + u * W] = e[u];
+                for (int u = 0; u < 8; ++u) if (j0 + u * W < some[r]) row[j0 + u * W] = e[u];           // (every one is asked for a slot: looked at there)
             }
         }
         if (p.slots_here) {
@@ -178,7 +179,8 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
                     int64_t s = -1;
                     if (i < count[r]) {
                         const uint32_t pos = (uint32_t)(start[r] + i), pg = p.page.div(pos);
-                        s = (int64_t)p.table[(int64_t)(b0 + r) * p.table_stride + pg] * p.page.d + (pos - pg * p.page.d);
+                        const int32_t e = p.table[(int64_t)(b0 + r) * p.table_stride + pg];
+                        if (e >= 0) s = (int64_t)e * p.page.d + (pos - pg * p.page.d); else bad = true;
                     }
                     p.slots[(int64_t)(b0 + r) * p.n + i] = s;
                 }
@@ -226,20 +228,24 @@ __global__ void __launch_bounds__(256) cache_slots_kernel(const __grid_constant_
     const int b = blockIdx.y, c = p.taken[b];
     const int64_t start = (int64_t)p.lengths[b] - c;
     const int32_t* row = p.table + (int64_t)b * p.table_stride;
+    bool bad = false;
     auto slot = [&](int64_t i) -> int64_t {
         if (i >= c) return -1;
         const uint32_t pos = (uint32_t)(start + i), pg = p.page.div(pos);
-        return (int64_t)row[pg] * p.page.d + (pos - pg * p.page.d);
+        const int32_t e = row[pg];
+        if (e < 0) { bad = true; return -1; }
+        return (int64_t)e * p.page.d + (pos - pg * p.page.d);
     };
     constexpr int V = Pairs ? 2 : 1;                 // slots of a store: two where a row starts on 16 bytes
     int64_t* out = p.slots + (int64_t)b * p.n;
 #pragma unroll
     for (int u = 0; u < kSlotsPerThread / V; ++u) {
         const int64_t i = ((int64_t)blockIdx.x * (kSlotsPerThread / V) + u) * 256 * V + threadIdx.x * V;
-        if (i >= p.n) return;
+        if (i >= p.n) break;
         if (Pairs) *reinterpret_cast<longlong2*>(out + i) = make_longlong2(slot(i), slot(i + 1));
         else out[i] = slot(i);
     }
+    if (bad && p.status) atomicOr(p.status, HTREE_STATUS_CACHE);
 }
 
 // ---- append and gather ------------------------------------------------------------------------------------------------------

@@ -344,6 +344,7 @@ typedef struct HtreeCache {
  * counts[b] > 0 grow, in row order, by pages from the pool's end, as long as the pool holds what the rows up to and including
  * it need; a row that gets its pages, or needs none, is served: taken[b] = counts[b], lengths[b] += counts[b] and
  * slots[b*n + i] = slot of the i-th new token for i < counts[b].  All other slots are -1, all other taken 0.
+ * An entry below 0 that is given back, or that slots are asked of (they are -1), is reported (bit 32).
  * lengths, table, pool and top are updated in place. */
 int htree_b200_cache_plan(int32_t B, int32_t M, int32_t page_size, int32_t n, int32_t* lengths, const int32_t* counts, int32_t* table,
                           int64_t table_stride, int32_t* pool, int32_t pool_size, int32_t* top, int64_t* slots, int32_t* taken,

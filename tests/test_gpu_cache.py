@@ -651,3 +651,24 @@ def test_tangents_are_refused():
         assert torch.equal(ht.draft_attention(**s), want)
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda q: ht.draft_attention(**dict(s, q=q)), (s["q"],), (torch.ones_like(s["q"]),))
+
+
+@pytest.mark.parametrize("n,extra", [(64, 0), (20000, 0), (64, 1100)])
+def test_plan_reports_pages_that_are_none(n, extra):
+    """A length of more pages than the table row has: the entry goes round (a page for a page), but is reported when it is given back and when
+    it is taken, and its tokens have no slots.  Slots by the plan itself and by the chip, few rows and more than a thousand."""
+    import htree_b200 as ht
+    from htree_b200 import ops
+    B = 2 + extra
+    lens, table = _ints([40, 0] + [0] * extra), _ints([[3, -1, 5, -1], [-1] * 4] + [[-1] * 4] * extra)
+    pool, top = _ints([0, 1, 2, 9, 9, 9]), _ints([3])
+    ht.cache_plan(lens, _ints([-1] + [0] * (B - 1)), table, pool, top, 16, n)
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        ops.check_status()
+    assert lens[:2].tolist() == [0, 0] and (table == -1).all() and pool.tolist() == [0, 1, 2, 3, -1, 5] and int(top) == 6
+    slots, taken = ht.cache_plan(lens, _ints([0, 60] + [0] * extra), table, pool, top, 16, n)
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        ops.check_status()
+    assert taken[:2].tolist() == [0, 60] and table[1].tolist() == [5, -1, 3, 2]
+    assert slots[1, :60].tolist() == list(range(80, 96)) + [-1] * 16 + list(range(48, 64)) + list(range(32, 44))
+    assert (slots[1, 60:] == -1).all() and (slots[0] == -1).all() and (slots[2:] == -1).all()
