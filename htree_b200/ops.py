@@ -162,7 +162,7 @@ def _status(device) -> torch.Tensor:
 
 def check_status(device=None) -> None:
     """Synchronise and raise if a kernel flagged a problem since the last check: an out-of-range node index (bits 0-3), a
-    bounded wait of the pipelined forward that ran out (bit 4), or tables of a paged cache that do not fit it (bits 5 and 6)."""
+    bounded wait of the pipelined forward or of draft_attention that ran out (bit 4), or tables of a paged cache that do not fit it (bits 5 and 6)."""
     device = torch.device(device if device is not None else torch.cuda.current_device())
     if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
@@ -175,8 +175,8 @@ def check_status(device=None) -> None:
             if v & 0xF:
                 what.append("a node index outside its tree level (clamped)")
             if v & 16:
-                what.append("an asynchronous operand copy of the pipelined forward did not complete within its bounded wait "
-                            "(the affected outputs were not written)")
+                what.append("an asynchronous copy or product did not complete within its bounded wait (the affected outputs of the pipelined "
+                            "forward were not written, those of draft_attention are wrong)")
             if v & 32:
                 what.append("a page, slot, length or token index outside the cache, or a draft before its parent (left out)")
             if v & 64:

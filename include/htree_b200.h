@@ -365,7 +365,7 @@ int htree_b200_cache_gather(const HtreeCache* cache, int32_t B, int32_t M, int32
  *     lse_i = log sum_j exp(s_ij),   out_i = sum_j exp(s_ij - lse_i) v_j
  * parents[b*N + i] < i is the draft that draft i continues, -1 where it continues the cached tokens, below -1 where there is no
  * such draft (its rows become out = 0, lse = -inf and no other draft reads its k, v); a parent >= i is taken as -1 and reported
- * (bit 32).  parents = NULL: every draft continues the one before it.
+ * (bit 32).  parents = NULL: every draft continues the one before it.  Status bit 16: a bounded wait ran out, out and lse are wrong.
  *   q [B,N,H,K], k [B,N,H_kv,K], v [B,N,H_kv,V]: strides in elements of a request, a token, a head; rows 16-byte aligned
  *   out [B,N,H,V] of the cache's type and lse [B,N,H] fp32 (may be NULL): contiguous
  *   workspace  htree_b200_draft_workspace() bytes, 16-byte aligned, of this call alone until its kernels have run

@@ -124,3 +124,14 @@ def test_plain_forms():
     s = torch.einsum("bihd,bjhd->bhij", q.double(), k.double()) * 8 ** -0.5
     w = s.masked_fill(~torch.ones(5, 5).tril().bool(), float("-inf")).softmax(-1)
     assert torch.allclose(out, torch.einsum("bhij,bjhd->bihd", w, v.double()), atol=1e-12) and (tol < 1e-4).all()
+
+
+def test_a_wait_that_ran_out_is_told_as_what_it_is(monkeypatch):
+    """The pipelined forward leaves outputs unwritten, the attention over the cache goes on with what there is: nobody is told that wrong numbers are old ones."""
+    from htree_b200 import ops
+    word = torch.tensor([16], dtype=torch.int32)
+    monkeypatch.setitem(ops._status_words, torch.device("cpu"), word)
+    with pytest.raises(RuntimeError, match="0x10: .*bounded wait .*forward were not written, those of draft_attention are wrong"):
+        ops.check_status("cpu")
+    assert word.item() == 0
+    ops.check_status("cpu")
