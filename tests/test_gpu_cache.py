@@ -672,3 +672,107 @@ def test_plan_reports_pages_that_are_none(n, extra):
     assert taken[:2].tolist() == [0, 60] and table[1].tolist() == [5, -1, 3, 2]
     assert slots[1, :60].tolist() == list(range(80, 96)) + [-1] * 16 + list(range(48, 64)) + list(range(32, 44))
     assert (slots[1, 60:] == -1).all() and (slots[0] == -1).all() and (slots[2:] == -1).all()
+
+
+# What the smaller tests ask of few query rows, of 40 to 160 (tcgen05 in 16 bits, tiles of 64 rows in fp32) and of wide ones.
+MANY = [(BF, 40, 4, 128, 16), (HF, 20, 2, 64, 64), (BF, 20, 2, 128, 128), (HF, 40, 4, 64, 48), (BF, 40, 4, 128, 7), (BF, 20, 3, 64, 256), (FP, 20, 2, 64, 16),
+        (FP, 40, 4, 128, 64), (BF, 40, 2, 256, 16)]
+
+
+@pytest.mark.parametrize("dt,N,G,K,page", MANY)
+def test_pages_outside_the_cache_with_many_rows(dt, N, G, K, page):
+    """Bad pages among good ones, first and last ones, all of a request; lengths beyond the table; a draft before its parent."""
+    import htree_b200 as ht
+    from htree_b200 import ops
+    s = make(dt, N, 2 * G, 2, K, K, page, [700, 520, 300, 129], seed=page)
+    P, bad = s["k_cache"].shape[0], [-1, 2 ** 31 - 1, -2 ** 31]
+    held = [-(-x // page) for x in (700, 520, 300, 129)]
+    for b, at in enumerate([[0, held[0] // 2], [held[1] // 3, held[1] - 1], range(held[2]), [0]]):
+        for i, j in enumerate(at):
+            s["block_table"][b, j] = ([P] + bad)[(b + i) % 4]
+    agrees(s, tree(4, N, pad=0.1))
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        ops.check_status()
+    t = make(dt, N, 2 * G, 2, K, K, page, [page * 3, 0], spare=2)
+    t["block_table"] = t["block_table"][:, :3].contiguous()
+    want = ht.draft_attention(**t)
+    assert torch.equal(ht.draft_attention(**dict(t, lengths=_ints([2 ** 31 - 1, -5]))), want)
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        ops.check_status()
+    par = tree(2, N, seed=3)
+    same, par[0, 1], par[1, 7] = par.clone(), 1, N + 5
+    same[0, 1] = same[1, 7] = -1
+    assert torch.equal(ht.draft_attention(**t, parents=par), ht.draft_attention(**t, parents=same))
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        ops.check_status()
+
+
+@pytest.mark.parametrize("dt,N,G,K", [(BF, 40, 4, 128), (HF, 20, 2, 64), (FP, 40, 1, 128)])
+def test_offsets_beyond_32_bits_with_many_rows(dt, N, G, K):
+    import htree_b200 as ht
+    page, pages = 256, (9 << 28) // (256 * K)                            # 2.4e9 elements
+    small = make(dt, N, G, 1, K, K, page, [1000])
+    kc, vc = (torch.zeros(pages, page, 1, K, dtype=dt, device=DEV) for _ in range(2))
+    used, far = small["block_table"][0, :4].long(), torch.arange(pages - 4, pages, device=DEV)
+    kc[far], vc[far] = small["k_cache"][used], small["v_cache"][used]
+    table = small["block_table"].clone()
+    table[0, :4] = far.int()
+    par = tree(1, N)
+    assert torch.equal(ht.draft_attention(**dict(small, k_cache=kc, v_cache=vc, block_table=table), parents=par), ht.draft_attention(**small, parents=par))
+
+
+@pytest.mark.parametrize("dt,K", [(BF, 128), (HF, 64), (FP, 128)])
+def test_streams_graphs_and_repeats_with_many_rows(dt, K):
+    import htree_b200 as ht
+    s = [make(dt, 40, 8, 2, K, K, 16, [1700, 90, 0], seed=1), make(dt, 20, 4, 2, K, K, 64, [3000, 4], seed=2)]
+    p = [tree(3, 40), tree(2, 20)]
+    want = [ht.draft_attention(**x, parents=y, return_lse=True) for x, y in zip(s, p)]
+    torch.cuda.synchronize()
+    st, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(st[i]):
+                outs[i].append(ht.draft_attention(**s[i], parents=p[i], return_lse=True))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for got in outs[i] for a, b in zip(got, want[i]))
+    graphs, got = [], []
+    for i in (0, 1, 0):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(ht.draft_attention(**s[i], parents=p[i]))
+    for turn in range(4):
+        for x in s:
+            for n in "qkv":
+                x[n].copy_(torch.randn_like(x[n]))
+            x["lengths"] -= 3 * (x["lengths"] > 50).int()
+        for g in graphs:
+            g.replay()
+        for i, out in zip((0, 1, 0), got):
+            assert torch.equal(out, ht.draft_attention(**s[i], parents=p[i]))
+
+
+@pytest.mark.parametrize("dt,K", [(BF, 128), (HF, 64), (FP, 128), (BF, 256)])
+def test_expanded_caches(dt, K):
+    """Heads that share a row of the cache and requests that share drafts, read through strides of zero."""
+    import htree_b200 as ht
+    s = make(dt, 40, 8, 2, K, K, 16, [300, 64])
+    e = dict(s, k_cache=s["k_cache"][:, :, :1].expand(-1, -1, 2, -1), v_cache=s["v_cache"][:, :, :1].expand(-1, -1, 2, -1), k=s["k"][:1].expand(2, -1, -1, -1),
+             q=s["q"][:, :, :1].expand(-1, -1, 8, -1))
+    for N in (40, 1):
+        for n in "qkv":
+            e[n] = e[n][:, :N]
+        f = {n: x.contiguous() for n, x in e.items()}
+        for a, b in zip(ht.draft_attention(**e, return_lse=True), ht.draft_attention(**f, return_lse=True)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dt,scale", [(FP, -0.7), (FP, 0.0), (BF, -1.0), (HF, 0.0), (BF, 3.0)])
+def test_scales_with_many_rows(dt, scale):
+    agrees(make(dt, 40, 8, 2, 128, 128, 16, [150, 300, 0]), tree(3, 40, pad=0.1), scale)
+
+
+@pytest.mark.parametrize("dt,N,K,lengths,is_tree", [(BF, 2500, 128, [300], False), (FP, 1500, 64, [70], False), (HF, 1024, 64, [200], True), (FP, 1024, 32, [5], True),
+                                                    (BF, 700, 256, [100], False), (BF, 1024, 96, [0], True)])
+def test_long_chains_and_large_trees(dt, N, K, lengths, is_tree):
+    agrees(make(dt, N, 1, 1, K, K, 16, lengths), tree(1, N, pad=0.02) if is_tree else None)
