@@ -776,3 +776,17 @@ def test_scales_with_many_rows(dt, scale):
                                                     (BF, 700, 256, [100], False), (BF, 1024, 96, [0], True)])
 def test_long_chains_and_large_trees(dt, N, K, lengths, is_tree):
     agrees(make(dt, N, 1, 1, K, K, 16, lengths), tree(1, N, pad=0.02) if is_tree else None)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_exponentials_on_the_fma_pipes(dt):
+    """Scores that are exact, of which those at places 6, 7, 14 and 15 of every sixteen make the sum: the lse shows their exponentials."""
+    s = make(dt, 40, 1, 1, 8, 8, 16, [128] * 64)
+    s["q"].zero_(); s["k"].zero_(); s["k_cache"].zero_()
+    s["q"][..., 0], s["k"][..., 0], s["k_cache"][..., 0] = 1.0, -1000.0, -1000.0
+    for b, x in enumerate(torch.linspace(-3.0, 6.5, 64).tolist()):
+        pages = s["block_table"][b, :8].long()
+        s["k_cache"][pages[0], 0, 0, 0] = 0.0                         # the reference
+        for place in (6, 7, 14, 15):
+            s["k_cache"][pages, place, 0, 0] = x
+    agrees(s, scale=1.0)
