@@ -38,7 +38,7 @@ struct DraftParams {
     int64_t q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h;                  // strides in bytes
     int64_t ck_page, ck_row, ck_h, cv_page, cv_row, cv_h;
     int64_t table_stride;
-    int32_t B, N, H, Hkv, G, K, V, M, pages;
+    int32_t B, N, H, Hkv, G, K, V, pages;
     int32_t rows, row_tiles, shift, draft_tiles;                           // rows of a row tile, log2 of the keys of a tile
     int32_t room;             // tokens that a row of the table can name
     int32_t whole;            // short tables: parts of whole units, and nothing to join
@@ -1067,7 +1067,7 @@ __global__ void __launch_bounds__(kFmaThreads, D > 128 ? 1 : 2) draft_fma_kernel
     if (bad && p.status) atomicOr(p.status, HTREE_STATUS_CACHE);
 }
 
-// ---- 16-bit types, more than 32 query rows: tcgen05 -----------------------------------------------------------------------------------
+// ---- 16-bit types, more than 32 query rows (16 where rows are wider than 64): tcgen05 -----------------------------------------------------------------------------------
 
 // 128 or 256 query rows a block against tiles of 128 keys, which come from HBM once for all of them.  Per job (a tile and 128 rows, the lanes
 // of tensor memory): S = Q K^T (operands in shared memory, accumulator in tensor memory), P = 2^(cS - reference) by a thread a row, written
@@ -2008,7 +2008,7 @@ static int fill_draft(DraftParams& p, const HtreeCache* c, const HtreeDrafts* d)
     p.ck_page = c->k_page * es; p.ck_row = c->k_row * es; p.ck_h = c->k_head * es;
     p.cv_page = c->v_page * es; p.cv_row = c->v_row * es; p.cv_h = c->v_head * es;
     p.table_stride = d->table_stride;
-    p.B = d->B; p.N = d->N; p.H = d->H; p.Hkv = c->H_kv; p.G = d->H / c->H_kv; p.K = c->K; p.V = c->V; p.M = d->M; p.pages = c->pages;
+    p.B = d->B; p.N = d->N; p.H = d->H; p.Hkv = c->H_kv; p.G = d->H / c->H_kv; p.K = c->K; p.V = c->V; p.pages = c->pages;
     const int64_t room = (int64_t)d->M * c->page_size;
     p.room = (int32_t)(room < kMaxLength ? room : kMaxLength);
     if ((int64_t)d->B * ((p.room + kSlice - 1) / kSlice + (d->N + kSlice - 1) / kSlice) >= (int64_t(1) << 31)) return HTREE_E_UNSUPPORTED;
