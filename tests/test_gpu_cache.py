@@ -790,3 +790,20 @@ def test_exponentials_on_the_fma_pipes(dt):
         for place in (6, 7, 14, 15):
             s["k_cache"][pages, place, 0, 0] = x
     agrees(s, scale=1.0)
+
+
+@pytest.mark.parametrize("dt,N,G,K,page", MANY + [(BF, 1, 4, 64, 16), (HF, 5, 2, 128, 16), (FP, 3, 2, 64, 16)])
+def test_scores_of_minus_infinity(dt, N, G, K, page):
+    """A row whose every score is -inf is an empty row; among others, such a key is one that weighs nothing."""
+    import htree_b200 as ht
+    s = make(dt, N, 2 * G, 2, K, K, page, [300, 300])
+    s["q"][..., 0] = 8.0
+    far = dict(s, k=s["k"].clone(), k_cache=s["k_cache"].clone())
+    for x, low in ((s, -math.inf), (far, -1000.0)):
+        mine = x["block_table"][0, :-(-300 // page)].long()
+        x["k_cache"][mine, ..., 0], x["k"][0, ..., 0] = low, low
+        x["k_cache"][x["block_table"][1, :-(-300 // page):2].long(), :, :, 0], x["k"][1, 1::2, :, 0] = low, low
+    out, lse = ht.draft_attention(**s, return_lse=True)
+    assert (out[0] == 0).all() and (lse[0] == -math.inf).all()
+    want = ht.draft_attention(**far, return_lse=True)
+    assert torch.equal(out[1], want[0][1]) and torch.equal(lse[1], want[1][1]) and torch.isfinite(lse[1]).all()
