@@ -59,8 +59,8 @@ def cache_plan(lengths: torch.Tensor, counts: torch.Tensor, block_table: torch.T
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
                  index: Optional[torch.Tensor] = None) -> None:
     """Rows of k [B, N, H_kv, K] and v [B, N, H_kv, V] into their slots [B, n] (-1: not written): token i of request b, or token
-    index[b, i] (int32), e.g. the accepted drafts.  Slots of one call have to differ: of tokens that share one, any may be kept.  k and v
-    must not lie in the cache themselves."""
+    index[b, i] (int32), e.g. the accepted drafts.  Slots of one call have to differ: what a slot holds that several tokens share is not
+    specified, a mixture of them included.  k and v must not lie in the cache themselves."""
     g, status = _calls(k_cache)
     g.cache_append(k, v, k_cache, v_cache, slots, index, status)
 
@@ -80,9 +80,9 @@ def draft_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: 
     that draft i continues (below i), -1 where it continues the cached tokens, below -1 where there is no such draft (its rows come back
     as zeros).  Without parents every draft continues the one before it: several tokens at once, or a chunk of a prompt.  A draft reads all
     cached tokens, itself, its parent, its parent's parent and so on; what other drafts hold does not reach it.
-    Returns out [B, N, H, V] in q's dtype; with return_lse also the log of the sum of the exponentials, [B, N, H] fp32 (-inf for empty
-    rows), by which outputs over other keys can be joined.  scale is K**-0.5 unless given.  Rows of up to 256 elements, trees of up to
-    1024 drafts, chains of any length."""
+    Returns out [B, N, H, V] in q's dtype; with return_lse also the log of the sum of the exponentials, [B, N, H] fp32, by which outputs over
+    other keys can be joined.  Rows that read nothing, or whose every score is -inf, are zeros with -inf.  scale is K**-0.5 unless given.  Rows
+    of up to 256 elements, trees of up to 1024 drafts, chains of any length."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     g, status = _calls(k_cache)

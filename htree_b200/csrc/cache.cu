@@ -72,7 +72,7 @@ __device__ __forceinline__ int plan_length(const PlanParams& p, int len, bool* b
 // computes the two scans for itself (a few words a request), the blocks share the rows, and cluster barriers separate the pushes, the
 // pops and the slots.  `W` threads work on a row: a warp where there are many rows, all of them where there is one.  What bounds it is
 // latency: entries move eight at a time (one by one, 512 rows of 800 pages took 61 us; so 12), by sixteen blocks of 1024 threads (admitting,
-// extending and ending 512 requests of 16384 tokens in pages of 16: 38 us in three calls, by eight of 512 threads 50; 1024 requests of 2000 in
+// extending and ending 512 requests of 16384 tokens in pages of 16: 40 us in three calls, by eight of 512 threads 50; 1024 requests of 2000 in
 // pages of one: 56 and 108).
 __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_constant__ PlanParams p) {
     __shared__ uint32_t scratch[kPlanThreads / 32];

@@ -261,7 +261,7 @@ __device__ __forceinline__ float finish_lse(float m, float mass) {
 
 // HBM bounds these (fp32 with more than 4 rows: the FMA pipes, at 11 to 15 TFLOP/s); the products only have to keep up: mma.sync in 16
 // bits, FFMA in fp32.  Measured, 32 requests, 8 heads of the cache, 4 query heads each: 16384 tokens of 128 in 359 us in bf16 (6.0 TB/s)
-// and 762 in fp32 (5.6), of 64 in 213 and 413 (5.0 and 5.2), 8192 of 256 in 373 and 938 (5.8 and 4.6).  A tile is 16 keys and belongs to one warp, with a softmax of its own (reference,
+// and 762 in fp32 (5.6), of 64 in 213 and 413 (5.0 and 5.2), 8192 of 256 in 361 to 374 and 927 (5.8 and 4.6).  A tile is 16 keys and belongs to one warp, with a softmax of its own (reference,
 // mass and sums in registers) and a ring of its own in shared memory that the warp fills by cp.async: the warps of a block do not wait for
 // one another until the unit ends.  The line is cut into parts of whole blocks; the tiles of a part go round the block's warps.
 // (One bulk copy of 256 bytes per lane and row instead: the compiler issues them lane by lane, 790 instructions a tile.)
@@ -1076,11 +1076,12 @@ __global__ void __launch_bounds__(kFmaThreads, D > 128 ? 1 : 2) draft_fma_kernel
 // every other tile, and are joined at the end.  Tensor memory: S and O of each half, 128 columns each; shared memory: Q (64 KB), three
 // stages of K and two of V (32 KB).  Roles: warps 0-3 and 4-7 the softmax of a half, 8 the products, 9-11 the copies.
 // At 256 rows of 128 a tile is 16.8 MFLOP, 2048 cycles of the tensor pipe, and 32768 exponentials, 2048 cycles of the special function
-// units: the two bound it alike, HBM (64 KB a tile) does below about 250 rows.  A tile of 256 rows takes 2500 to 2800 cycles as it is (the
-// scores' operands and the copies share the bandwidth of shared memory).  Measured in bf16, 128 wide: 4 requests of 16384, 8 heads, chunks of
-// 512 drafts with 4 query heads each: 615 us, 908 TFLOP/s; 8 of 65536, 4 heads, 256 rows: 308 us, 894 TFLOP/s, 128 rows 210 us, 5.1 TB/s.
+// units: the two bound it alike, HBM (64 KB a tile) does below about 250 rows.  A tile of 256 rows takes 3100 cycles as it is, a part
+// 37000 more (cold, under a profiler); no unit's counter is above half.  Measured in bf16, 128 wide: 4 requests of 16384, 8 heads, chunks of
+// 512 drafts with 4 query heads each: 635 us, 880 TFLOP/s; 8 of 65536, 4 heads, 256 rows: 303 to 313 us, 880 to 907 TFLOP/s, 128 rows 215 us, 5.0 TB/s.
 // A row's weights in a tile may sum to kTcMost before the reference follows (a maximum per tile costs a fifth of the softmax; the sum is there
-// anyway); a reference is set kTcBias below the maximum.  bf16 has fp32's range; fp16 ends at 65504 and keeps all its digits down to 2^-14.
+// anyway); a reference is set kTcBias below a tile's maximum, the first one, where all keys of the tile are read, below that of its first sixteen scores:
+// later ones may be any distance above it, and the sum and exp2_poly's largest exponent tell.  bf16 has fp32's range; fp16 ends at 65504 and keeps all its digits down to 2^-14.
 template <typename T> constexpr float kTcMost = 65536.f;
 template <> constexpr float kTcMost<__half> = 60000.f;
 template <typename T> constexpr float kTcBias = 0.f;
@@ -1878,8 +1879,8 @@ static int64_t part_bytes(const DraftParams& p) { return p.whole ? 0 : (int64_t)
 static int64_t workspace_of(const DraftParams& p) { return p.whole ? 16 : part_bytes(p) + p.grid * 16; }           // tasks: per unit or per part, never more than parts
 
 // Which kernel.  16-bit rows of up to 128 go to the tensor cores, by mma.sync up to 32 query rows, up to 16 with rows of more than 64 (where
-// a warp of 32 has spills).  Measured, 8 requests of 16384, 4 heads of 128: 32 rows 84 us on mma.sync and 70 on tcgen05, 16 rows 63 and
-// 70; 8 heads of 64: 32 rows 78 and 97; 8 requests of 1000, 4 heads of 128: 32 rows 25 and 27, 16 rows 20 and 27.
+// a warp of 32 has spills).  Measured, 8 requests of 16384, 4 heads of 128: 32 rows 104 us on mma.sync (two tiles of sixteen) and 63 on
+// tcgen05, 16 rows 63 and 62; 8 heads of 64: 32 rows 76 and 80; 8 requests of 1000, 4 heads of 128: 32 rows 23.4 and 20.4, 16 rows 18.5 and 19.4.
 // fp32 (4 requests of 16384, 4 heads of 128): 17 to 32 rows 266 us by slices of sixteen rows and 242 by FFMA tiles of 64, 16 rows 147 and
 // 242; 8 rows 95 by slices of eight and 148 by those of sixteen.  Wider 16-bit rows: slices of 16 query rows however many there are (4 requests of 16384, 4 heads of 256, 256 rows: 620 us).
 enum { kSlice4 = 0, kSlice8, kSlice16, kSlice32, kFma, kTc };

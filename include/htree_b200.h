@@ -351,7 +351,8 @@ int htree_b200_cache_plan(int32_t B, int32_t M, int32_t page_size, int32_t n, in
                           int32_t* status, void* stream);
 
 /* Token index[b*n + i] (NULL: token i) of request b of k [B,N,H_kv,K] and v [B,N,H_kv,V] into slots[b*n + i]; -1 = not written.
- * k_stride, v_stride: strides in elements of a request, a token, a head.  Of several tokens for one slot any may be the one kept. */
+ * k_stride, v_stride: strides in elements of a request, a token, a head.  What a slot holds that several tokens
+ * of a call share is not specified (16-byte pieces of different tokens, keys and values apart). */
 int htree_b200_cache_append(const HtreeCache* cache, int32_t B, int32_t N, int32_t n, const void* k, const int64_t* k_stride,
                             const void* v, const int64_t* v_stride, const int64_t* slots, const int32_t* index, int32_t* status,
                             void* stream);
@@ -362,7 +363,7 @@ int htree_b200_cache_gather(const HtreeCache* cache, int32_t B, int32_t M, int32
 
 /* Attention of N drafted tokens per request over its cached tokens and over the drafts that lead to it:
  *     s_ij = scale * q_i . k_j     over j = the lengths[b] cached tokens and the drafts i, parent(i), parent(parent(i)), ...
- *     lse_i = log sum_j exp(s_ij),   out_i = sum_j exp(s_ij - lse_i) v_j
+ *     lse_i = log sum_j exp(s_ij),   out_i = sum_j exp(s_ij - lse_i) v_j      (every s_ij -inf: out = 0, lse = -inf)
  * parents[b*N + i] < i is the draft that draft i continues, -1 where it continues the cached tokens, below -1 where there is no
  * such draft (its rows become out = 0, lse = -inf and no other draft reads its k, v); a parent >= i is taken as -1 and reported
  * (bit 32).  parents = NULL: every draft continues the one before it.  Status bit 16: a bounded wait ran out, out and lse are wrong.
